@@ -473,6 +473,31 @@ int serl_learner_phase_count(serl_learner* h);
 int serl_learner_phase_get(serl_learner* h, int i, const char** name, double* ms_to_next);
 int serl_learner_timing_reset(serl_learner* h);
 
+/* ---- operators of sequence policies (serl_amd/sequence.py): no counterpart in the reference, whose policies see history
+ * through frame stacks and whose only discrete head is the gripper's.  type: 0 fp32, 1 bf16, 2 fp16 of the tensors named
+ * `const void*` / `void*`; strides in elements; all sums, states and statistics are fp32, a value is rounded once, when it
+ * is stored.  Any alignment and stride is taken: rows of whole 16-byte pieces at 16-byte addresses run wide loads.
+ *
+ * Gated linear recurrence: f = sigmoid(gate), h_t = f_t (start_t ? 0 : h_{t-1}) + (1 - f_t) x_t, y_t = h_t over (B, T, D)
+ * (_bs, _ts: strides of a sequence and of a step; channels are contiguous).  h0 (B, D) or NULL = 0; starts: bytes (B, T),
+ * sequence stride starts_bs, or NULL; lengths (B) or NULL: steps t >= lengths[b] (clamped to [0, T]) hold the state and
+ * give y = 0 and zero gradients, whatever the inputs hold there.  h_last (B, D) = the state behind the last step; it may be
+ * h0 itself for T <= 8 (acting: T = 1).  states: NULL, or serl_gated_scan_states_floats floats that the backward pass
+ * reads.  workspace: serl_gated_scan_workspace_bytes (0 for most shapes), for either direction, contents undefined. */
+long long serl_gated_scan_workspace_bytes(int type, int B, int T, int D);
+long long serl_gated_scan_states_floats(int B, int T, int D);
+int serl_gated_scan_fwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,
+                        const void* x, long long x_bs, long long x_ts, const float* h0, const unsigned char* starts,
+                        long long starts_bs, const int* lengths, void* y, long long y_bs, long long y_ts, float* h_last,
+                        float* states, float* workspace, long long workspace_bytes, void* stream);
+/* dy (B, T, D), dh_last (B, D) or NULL -> dgate, dx (B, T, D), dh0 (B, D); T >= 1; the outputs overlap no input */
+int serl_gated_scan_bwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,
+                        const void* x, long long x_bs, long long x_ts, const unsigned char* starts, long long starts_bs,
+                        const int* lengths, const float* states, const void* dy, long long dy_bs, long long dy_ts,
+                        const float* dh_last, void* dgate, long long dgate_bs, long long dgate_ts, void* dx,
+                        long long dx_bs, long long dx_ts, float* dh0, float* workspace, long long workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

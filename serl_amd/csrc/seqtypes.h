@@ -1,0 +1,112 @@
+// Element types and wide loads / stores of the sequence-policy operators (gated_scan.hip, rms_norm.hip, distill.hip).
+// Tensors are fp32, bf16 or fp16; every sum, state and statistic is fp32; a value is rounded once, to nearest even, when
+// it is stored.
+#pragma once
+#include "common.h"
+
+#define SERL_F32 0      // type codes of the C ABI
+#define SERL_BF16 1
+#define SERL_F16 2
+
+typedef uint32_t sq_u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t sq_u32x4 __attribute__((ext_vector_type(4)));   // native vectors stay in registers
+typedef uint16_t sq_u16;
+typedef float sq_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 sq_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 sq_f16x2 __attribute__((ext_vector_type(2)));
+
+struct F32 { typedef uint32_t bits; static constexpr int code = SERL_F32; };
+struct BF16 { typedef uint16_t bits; static constexpr int code = SERL_BF16; };
+struct F16 { typedef uint16_t bits; static constexpr int code = SERL_F16; };
+
+__device__ __forceinline__ float sq_val(F32, uint32_t b) { return __uint_as_float(b); }
+__device__ __forceinline__ float sq_val(BF16, uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ float sq_val(F16, uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+__device__ __forceinline__ uint32_t sq_bits(F32, float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint16_t sq_bits(BF16, float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+__device__ __forceinline__ uint16_t sq_bits(F16, float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+
+// two packed 16-bit values of a dword, and back
+template <typename T> __device__ __forceinline__ void sq_unpack2(uint32_t w, float& a, float& b) {
+  a = sq_val(T(), (uint16_t)(w & 0xffffu));
+  b = sq_val(T(), (uint16_t)(w >> 16));
+}
+template <> __device__ __forceinline__ void sq_unpack2<BF16>(uint32_t w, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ uint32_t sq_pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t sq_pack2<BF16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((sq_f32x2){a, b}, sq_bf16x2));
+}
+template <> __device__ __forceinline__ uint32_t sq_pack2<F16>(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((sq_f32x2){a, b}, sq_f16x2));
+}
+
+// VEC consecutive elements of type T as they lie in memory (VEC * size = a power of two of bytes, naturally aligned; VEC = 1: one element)
+template <typename T, int VEC> struct Raw {
+  static constexpr int BYTES = VEC * (int)sizeof(typename T::bits);
+  static constexpr int W = BYTES / 4;
+  static_assert(BYTES % 4 == 0, "whole dwords");
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const typename T::bits* p) {
+    if constexpr (W % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const sq_u32x4 v = reinterpret_cast<const sq_u32x4*>(p)[i];
+        w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (W == 2) {
+      const sq_u32x2 v = *reinterpret_cast<const sq_u32x2*>(p);
+      w[0] = v.x; w[1] = v.y;
+    } else {
+      static_assert(W == 1, "1, 2 or 4n dwords");
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(typename T::bits* p) const {
+    if constexpr (W % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i)
+        reinterpret_cast<sq_u32x4*>(p)[i] = (sq_u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    } else if constexpr (W == 2) {
+      *reinterpret_cast<sq_u32x2*>(p) = (sq_u32x2){w[0], w[1]};
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    if constexpr (sizeof(typename T::bits) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) sq_unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void put(const float (&v)[VEC]) {
+    if constexpr (sizeof(typename T::bits) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] = sq_pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+  }
+};
+template <typename T> struct Raw<T, 1> {
+  typename T::bits w;
+  __device__ __forceinline__ void load(const typename T::bits* p) { w = *p; }
+  __device__ __forceinline__ void store(typename T::bits* p) const { *p = w; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = sq_val(T(), w); }
+  __device__ __forceinline__ void put(const float (&v)[1]) { w = sq_bits(T(), v[0]); }
+};
+
+static inline bool sq_aligned(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
+static inline int sq_size(int code) { return code == SERL_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float sq_wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}

@@ -342,3 +342,34 @@ def ln_tangent_bwd(outbar, tbar_ext, y, w, a, xhat, rstd, gamma, abar, ubar, gga
 
 def axpy(y, x, a, n, stream):
     call("serl_axpy", y, x, float(a), n, stream)
+
+
+# ---- operators of sequence policies (serl_amd/sequence.py: the same on tensors); dtype: F32, BF16 or F16
+F32, BF16, F16 = 0, 1, 2
+
+
+def _nbytes(r, what):
+    if r < 0:
+        raise ValueError(f"{what}: " + _lib.load().serl_last_error().decode())
+    return int(r)
+
+
+def gated_scan_workspace_bytes(dtype, B, T, D) -> int:
+    return _nbytes(_lib.load().serl_gated_scan_workspace_bytes(dtype, B, T, D), "gated_scan_workspace_bytes")
+
+
+def gated_scan_states_floats(B, T, D) -> int:
+    return _nbytes(_lib.load().serl_gated_scan_states_floats(B, T, D), "gated_scan_states_floats")
+
+
+def gated_scan_fwd(dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, h0, starts, starts_bs, lengths, y, y_bs, y_ts,
+                   h_last, states, workspace, workspace_bytes, stream):
+    call("serl_gated_scan_fwd", dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, h0, starts, starts_bs, lengths,
+         y, y_bs, y_ts, h_last, states, workspace, workspace_bytes, stream)
+
+
+def gated_scan_bwd(dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, starts, starts_bs, lengths, states, dy, dy_bs,
+                   dy_ts, dh_last, dgate, dgate_bs, dgate_ts, dx, dx_bs, dx_ts, dh0, workspace, workspace_bytes, stream):
+    call("serl_gated_scan_bwd", dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, starts, starts_bs, lengths,
+         states, dy, dy_bs, dy_ts, dh_last, dgate, dgate_bs, dgate_ts, dx, dx_bs, dx_ts, dh0, workspace,
+         workspace_bytes, stream)

@@ -1,0 +1,198 @@
+"""Operators of sequence policies on CUDA tensors: a gated linear recurrence (the memory), the root-mean-square norm with
+the residual's addition, and the distillation of a teacher's top logits -- each with its gradient, all arithmetic in HIP
+kernels (csrc/gated_scan.hip, rms_norm.hip, distill.hip).  No counterpart in the reference: its policies see history
+through frame stacks (serl/networks/pixel_multiplexer.py:27) and its only discrete head is the gripper's
+(serl/agents/bc/pixel_hybrid_bc_learner.py:99-107).
+
+Tensors are float32, bfloat16 or float16 on one GPU, channels contiguous (others are copied first); states, statistics and
+sums are float32 and a value is rounded once, when it is stored.  Calls are enqueued on the current stream of the tensors'
+device, wait for nothing, and may be captured into a graph; results and scratch memory come from torch's allocator, call by
+call, so nothing is shared between calls or graphs.  As in the learners, gradients are explicit calls: autograd records
+nothing here.  Wrong types raise TypeError, wrong shapes ValueError, before anything is enqueued.  Results are the same
+bits on every call with the same arguments."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import ops
+
+_CODES = {torch.float32: ops.F32, torch.bfloat16: ops.BF16, torch.float16: ops.F16}
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _shape(t, name, shape):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _type(t, name, *dtypes):
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def _place(*named):
+    """The tensors' common GPU: the context that makes it the current one."""
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the others on {dev}")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _channels(t):
+    """t with contiguous channels (the last dimension)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _out(t, name, like_shape, dtype):
+    """A caller's output tensor: rows may have any stride, but must not share memory with each other."""
+    _shape(t, name, like_shape)
+    _type(t, name, dtype)
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have contiguous channels")
+    return t
+
+
+# ------------------------------------------------------------------------------------------------- gated recurrence
+def _scan_args(gate, x, starts, lengths):
+    if not isinstance(gate, torch.Tensor) or gate.ndim != 3:
+        raise ValueError("gate must be a (B, T, D) tensor")
+    B, T, D = gate.shape
+    _shape(x, "x", (B, T, D))
+    if gate.dtype not in _CODES:
+        raise TypeError(f"gate must be float32, bfloat16 or float16, got {gate.dtype}")
+    _type(x, "x", gate.dtype)
+    if starts is not None:
+        _shape(starts, "starts", (B, T))
+        _type(starts, "starts", torch.bool, torch.uint8)
+    if lengths is not None:
+        _shape(lengths, "lengths", (B,))
+        _type(lengths, "lengths", torch.int32, torch.int64)
+    return B, T, D
+
+
+def _state(t, name, B, D):
+    if t is not None:
+        _shape(t, name, (B, D))
+        _type(t, name, torch.float32)
+
+
+def _masks(starts, lengths, T):
+    if starts is not None:
+        starts = _channels(starts)
+    if lengths is not None:
+        if lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, T).to(torch.int32)
+        lengths = lengths.contiguous()
+    return starts, lengths
+
+
+def _scan_scratch(code, B, T, D, device):
+    n = ops.gated_scan_workspace_bytes(code, B, T, D)
+    return (torch.empty(n // 4, dtype=torch.float32, device=device) if n else None), n
+
+
+def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
+    """h_t = f_t (starts_t ? 0 : h_{t-1}) + (1 - f_t) x_t with f = sigmoid(gate), along the time axis.
+
+    gate, x: (B, T, D); h0: (B, D) float32 state before the first step (None: zeros); starts: (B, T) bool, an episode
+    begins at the step; lengths: (B,) ints, steps from there on hold the state and give y = 0.  T and B may be 0.
+    Returns (y, h_last): y (B, T, D) in gate's type, h_last (B, D) float32; with save=True also the states that
+    gated_scan_backward needs."""
+    B, T, D = _scan_args(gate, x, starts, lengths)
+    _state(h0, "h0", B, D)
+    with _place(("gate", gate), ("x", x), ("h0", h0), ("starts", starts), ("lengths", lengths)):
+        gate, x = _channels(gate), _channels(x)
+        starts, lengths = _masks(starts, lengths, T)
+        if h0 is not None:
+            h0 = h0.contiguous()
+        code, dev = _CODES[gate.dtype], gate.device
+        y = torch.empty((B, T, D), dtype=gate.dtype, device=dev)
+        h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+        saved = torch.empty((B, -(-T // 128), D), dtype=torch.float32, device=dev) if save else None
+        ws, nws = _scan_scratch(code, B, T, D, dev)
+        ops.gated_scan_fwd(code, B, T, D, gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
+                           x.stride(1), _ptr(h0), _ptr(starts), 0 if starts is None else starts.stride(0), _ptr(lengths),
+                           y.data_ptr(), T * D, D, h_last.data_ptr(), _ptr(saved), _ptr(ws), nws, ops.current_stream())
+    return (y, h_last, saved) if save else (y, h_last)
+
+
+def gated_scan_backward(gate, x, saved, dy, dh_last=None, starts=None, lengths=None, out=None):
+    """Gradients of gated_scan: (dgate, dx) in gate's type, dh0 (B, D) float32.  `saved` and the other arguments as in the
+    forward call; dy (B, T, D), dh_last (B, D) float32 or None.  out: (dgate, dx) tensors to write, for instance the two
+    halves of one projection's gradient."""
+    B, T, D = _scan_args(gate, x, starts, lengths)
+    _shape(saved, "saved", (B, -(-T // 128), D))
+    _type(saved, "saved", torch.float32)
+    _shape(dy, "dy", (B, T, D))
+    _type(dy, "dy", gate.dtype)
+    _state(dh_last, "dh_last", B, D)
+    if out is not None:
+        dgate, dx = _out(out[0], "out[0]", (B, T, D), gate.dtype), _out(out[1], "out[1]", (B, T, D), gate.dtype)
+    else:
+        dgate = dx = None
+    with _place(("gate", gate), ("x", x), ("saved", saved), ("dy", dy), ("dh_last", dh_last), ("starts", starts),
+                ("lengths", lengths), ("out[0]", dgate), ("out[1]", dx)):
+        gate, x, dy, saved = _channels(gate), _channels(x), _channels(dy), saved.contiguous()
+        starts, lengths = _masks(starts, lengths, T)
+        if dh_last is not None:
+            dh_last = dh_last.contiguous()
+        code, dev = _CODES[gate.dtype], gate.device
+        if out is None:
+            dgate, dx = (torch.empty((B, T, D), dtype=gate.dtype, device=dev) for _ in range(2))
+        if T == 0:
+            dh0 = torch.zeros((B, D), dtype=torch.float32, device=dev) if dh_last is None else dh_last.clone()
+            return dgate, dx, dh0
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev)
+        ws, nws = _scan_scratch(code, B, T, D, dev)
+        ops.gated_scan_bwd(code, B, T, D, gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
+                           x.stride(1), _ptr(starts), 0 if starts is None else starts.stride(0), _ptr(lengths),
+                           saved.data_ptr(), dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dh_last), dgate.data_ptr(),
+                           dgate.stride(0), dgate.stride(1), dx.data_ptr(), dx.stride(0), dx.stride(1), dh0.data_ptr(),
+                           _ptr(ws), nws, ops.current_stream())
+    return dgate, dx, dh0
+
+
+def gated_scan_step(gate, x, h, starts=None, h_out=None):
+    """One step of gated_scan for an acting policy: gate, x (B, D), state h (B, D) float32, starts (B,) bool or None.
+    Returns (y, h_new); h_out: the tensor to write the new state to (h itself: in place)."""
+    if not isinstance(gate, torch.Tensor) or gate.ndim != 2:
+        raise ValueError("gate must be a (B, D) tensor")
+    B, D = gate.shape
+    _shape(x, "x", (B, D))
+    if gate.dtype not in _CODES:
+        raise TypeError(f"gate must be float32, bfloat16 or float16, got {gate.dtype}")
+    _type(x, "x", gate.dtype)
+    if h is None:
+        raise TypeError("h must be a tensor")
+    _state(h, "h", B, D)
+    if starts is not None:
+        _shape(starts, "starts", (B,))
+        _type(starts, "starts", torch.bool, torch.uint8)
+    if h_out is not None:
+        _state(h_out, "h_out", B, D)
+        if not h_out.is_contiguous():
+            raise ValueError("h_out must be contiguous")
+    with _place(("gate", gate), ("x", x), ("h", h), ("starts", starts), ("h_out", h_out)):
+        gate, x, h = _channels(gate), _channels(x), h.contiguous()
+        y = torch.empty((B, D), dtype=gate.dtype, device=gate.device)
+        if h_out is None:
+            h_out = torch.empty((B, D), dtype=torch.float32, device=gate.device)
+        ops.gated_scan_fwd(_CODES[gate.dtype], B, 1, D, gate.data_ptr(), gate.stride(0), 0, x.data_ptr(), x.stride(0), 0,
+                           h.data_ptr(), _ptr(starts), 0 if starts is None else starts.stride(0), None, y.data_ptr(), D, D,
+                           h_out.data_ptr(), None, None, 0, ops.current_stream())
+    return y, h_out

@@ -1,0 +1,299 @@
+"""The operators of sequence policies (serl_amd/sequence.py) against plain 64-bit statements of the same formulas.
+
+Tolerances.  A stored value carries one rounding, half a step: HALF[dtype] of its size.  What is computed in 32 bits before
+it is bounded by counting roundings of 2^-24 (U below); the counts stand beside the checks."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+HALF = {d: torch.finfo(d).eps / 2 for d in DTYPES}
+U = 2.0 ** -24
+
+
+def seq():
+    from serl_amd import sequence
+    return sequence
+
+
+def within(got, ref, tol, what):
+    """|got - ref| <= tol element by element (tol: a number or a tensor like ref); ref finite."""
+    got = got.detach().double().cpu()
+    ref = ref.detach().double().cpu()
+    tol = torch.as_tensor(tol, dtype=torch.float64)
+    if not ref.numel():
+        assert got.shape == ref.shape, what
+        return
+    bad = ~((got - ref).abs() <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((got - ref).abs().nan_to_num(math.inf).max()):.3e}, tolerance {float(tol.max()):.3e}"
+
+
+# ------------------------------------------------------------------------------------------------- gated recurrence
+def scan_inputs(dev, dtype, B, T, D, seed, h0=True, starts=False, lengths=False):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    gate = (r(B, T, D) * 2 + 1).clamp_(-6, 4).to(dtype)      # f <= sigmoid(4) = 0.982: a memory of 56 steps
+    x, dy = r(B, T, D).to(dtype), r(B, T, D).to(dtype)
+    out = dict(gate=gate, x=x, dy=dy, dh_last=r(B, D), h0=r(B, D) if h0 else None, starts=None, lengths=None)
+    if starts:
+        out["starts"] = torch.rand((B, T), generator=g) < 0.15
+        out["starts"][0, :2] = True
+    if lengths:
+        out["lengths"] = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+        out["lengths"][0] = T
+        out["lengths"][-1] = 0 if B > 1 else max(0, T - 1)
+    return {k: None if v is None else v.to(dev) for k, v in out.items()}
+
+
+def scan_reference(gate, x, h0, starts, lengths, dy=None, dh_last=None):
+    """The recurrence step by step in 64 bits, its gradients by autograd."""
+    gate, x = (t.double().cpu().requires_grad_() for t in (gate, x))
+    B, T, D = gate.shape
+    first = torch.zeros((B, D), dtype=torch.float64) if h0 is None else h0.double().cpu()
+    first.requires_grad_()
+    h, ys = first, []
+    f = torch.sigmoid(gate)
+    for t in range(T):
+        prev = h if starts is None else torch.where(starts[:, t, None].cpu(), torch.zeros_like(h), h)
+        new = f[:, t] * prev + (1 - f[:, t]) * x[:, t]
+        live = torch.ones((B, 1), dtype=torch.bool) if lengths is None else (t < lengths.cpu().long())[:, None]
+        h = torch.where(live, new, h)
+        ys.append(torch.where(live, new, torch.zeros_like(new)))
+    y = torch.stack(ys, 1)
+    if dy is None:
+        return y, h
+    total = (y * dy.double().cpu()).sum() + (h * dh_last.double().cpu()).sum()
+    return (y, h) + torch.autograd.grad(total, (gate, x, first))
+
+
+# 56 steps of memory, each with at most 6 roundings of the gate, the products and the joins of tiles
+SCAN_STATE = 56 * 6 * U
+
+
+def check_scan(i, dtype, with_backward=True):
+    s = seq()
+    y, h, saved = s.gated_scan(i["gate"], i["x"], h0=i["h0"], starts=i["starts"], lengths=i["lengths"], save=True)
+    y2, h2 = s.gated_scan(i["gate"], i["x"], h0=i["h0"], starts=i["starts"], lengths=i["lengths"])
+    assert torch.equal(y, y2) and torch.equal(h, h2) and y.dtype == dtype and h.dtype == torch.float32
+    ry, rh, rg, rx, r0 = scan_reference(i["gate"], i["x"], i["h0"], i["starts"], i["lengths"], i["dy"], i["dh_last"])
+    hm = max(1.0, float(rh.detach().abs().max()), float(ry.detach().abs().max()))
+    within(y, ry, SCAN_STATE * hm + HALF[dtype] * ry.detach().abs() + 2.0 ** -26, "y")
+    within(h, rh, SCAN_STATE * hm, "h_last")
+    if not with_backward:
+        return
+    dg, dx, d0 = s.gated_scan_backward(i["gate"], i["x"], saved, i["dy"], dh_last=i["dh_last"], starts=i["starts"],
+                                       lengths=i["lengths"])
+    # |G| is at most the sum of what reaches a step: bounded by (56 + 1) of the largest |dy|, |dh_last|
+    gm = 57 * max(float(i["dy"].abs().max()), float(i["dh_last"].abs().max()))
+    xm = float(i["x"].abs().max())
+    within(d0, r0, SCAN_STATE * gm, "dh0")
+    within(dx, rx, SCAN_STATE * gm + HALF[dtype] * rx.abs() + 2.0 ** -26, "dx")
+    # dgate = G (h - x) f (1 - f): the errors of G and of h, each by the other's size, with f (1 - f) <= 1/4; 2^-26: half
+    # a step among fp16's smallest numbers
+    within(dg, rg, 2 * SCAN_STATE * gm * (hm + xm) / 4 + HALF[dtype] * rg.abs() + 2.0 ** -26, "dgate")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", [(1, 1, 1), (3, 1, 64), (2, 5, 7), (4, 8, 64), (2, 9, 16), (1, 31, 24), (2, 127, 40), (1, 128, 136),
+                                   (2, 129, 33), (3, 257, 96), (2, 385, 65), (1, 1100, 8), (2, 1537, 19), (1, 4700, 72)])
+def test_gated_scan_matches_the_recurrence(dev, dtype, B, T, D):
+    for k, opt in enumerate(({}, {"starts": True}, {"lengths": True, "h0": False}, {"starts": True, "lengths": True})):
+        check_scan(scan_inputs(dev, dtype, B, T, D, 100 * k + T + D, **opt), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_gated_scan_gradient_matches_differences(dev, dtype):
+    """<gradient, direction> against the central difference of the kernel's own outputs (state only, so fp32)."""
+    s = seq()
+    B, T, D = 2, 150, 24
+    i = scan_inputs(dev, torch.float32, B, T, D, 5, starts=True)
+    y, h, saved = s.gated_scan(i["gate"], i["x"], h0=i["h0"], starts=i["starts"], save=True)
+    dg, dx, d0 = s.gated_scan_backward(i["gate"], i["x"], saved, i["dy"], dh_last=i["dh_last"], starts=i["starts"])
+    g = torch.Generator(device=dev).manual_seed(1)
+    vg, vx, v0 = (torch.randn(t.shape, generator=g, device=dev) for t in (i["gate"], i["x"], i["h0"]))
+
+    def value(e):
+        y, h = s.gated_scan(i["gate"] + e * vg, i["x"] + e * vx, h0=i["h0"] + e * v0, starts=i["starts"])
+        return float((y.double() * i["dy"]).sum() + (h.double() * i["dh_last"]).sum())
+    e = 2.0 ** -9
+    want = float((dg.double() * vg).sum() + (dx.double() * vx).sum() + (d0.double() * v0).sum())
+    got = (value(e) - value(-e)) / (2 * e)
+    # size of the value's terms sqrt(B T D) ~ 85, each off by SCAN_STATE, over 2 e; the cubic term e^2 / 6 of the same size times 57^2
+    n = math.sqrt(B * T * D)
+    assert abs(got - want) <= n * 4 * SCAN_STATE / (2 * e) + n * e * e / 6 * 57 ** 2, (got, want)
+
+
+def test_gated_scan_step_equals_a_scan_of_one_step_and_may_run_in_place(dev):
+    s = seq()
+    for dtype in DTYPES:
+        for B, D in ((1, 1), (3, 7), (64, 1024), (5, 40)):
+            i = scan_inputs(dev, dtype, B, 6, D, B, starts=True)
+            h = i["h0"].clone()
+            y, h_last = s.gated_scan(i["gate"], i["x"], h0=i["h0"], starts=i["starts"])
+            for t in range(6):
+                before = h.clone()
+                yt, new = s.gated_scan_step(i["gate"][:, t], i["x"][:, t], h, starts=i["starts"][:, t])
+                assert torch.equal(h, before)
+                ys, hs = s.gated_scan_step(i["gate"][:, t], i["x"][:, t], h, starts=i["starts"][:, t], h_out=h)
+                assert hs is h and torch.equal(h, new) and torch.equal(yt, ys) and torch.equal(yt, y[:, t])
+            assert torch.equal(h, h_last)
+
+
+def test_gated_scan_takes_views_and_writes_views(dev):
+    """gate and x as halves of one projection, gradients into the halves of one buffer, odd offsets, a batch stride of 0."""
+    s = seq()
+    for dtype in (torch.float32, torch.bfloat16):
+        for D, off in ((64, 0), (64, 1), (33, 3)):
+            i = scan_inputs(dev, dtype, 3, 140, D, D + off, starts=True, lengths=True)
+            both = torch.full((3, 140, 2 * D + off + 5), float("nan"), dtype=dtype, device=dev)
+            both[..., off:off + D], both[..., off + D:off + 2 * D] = i["gate"], i["x"]
+            gate, x = both[..., off:off + D], both[..., off + D:off + 2 * D]
+            a = s.gated_scan(i["gate"], i["x"], i["h0"], i["starts"], i["lengths"], save=True)
+            b = s.gated_scan(gate, x, i["h0"], i["starts"], i["lengths"], save=True)
+            grads = torch.full_like(both, 7.0)
+            out = grads[..., off:off + D], grads[..., off + D:off + 2 * D]
+            ga = s.gated_scan_backward(i["gate"], i["x"], a[2], i["dy"], i["dh_last"], i["starts"], i["lengths"])
+            s.gated_scan_backward(gate, x, b[2], i["dy"], i["dh_last"], i["starts"], i["lengths"], out=out)
+            tol = 2 * 60 * 6 * U * 57 * 6
+            for u, v in zip(a[:2] + ga[:2], b[:2] + out):      # another order of joins than with wide loads
+                within(v, u, tol + 2 * HALF[dtype] * u.double().abs().cpu(), "view")
+            assert bool((grads[..., :off] == 7).all()) and bool((grads[..., off + 2 * D:] == 7).all())
+    i = scan_inputs(dev, torch.float32, 1, 50, 16, 3)
+    y, h = s.gated_scan(i["gate"].expand(4, 50, 16), i["x"].expand(4, 50, 16), h0=i["h0"].expand(4, 16))
+    y1, h1 = s.gated_scan(i["gate"], i["x"], h0=i["h0"])
+    assert torch.equal(y, y1.expand_as(y)) and torch.equal(h, h1.expand_as(h))
+    # channels that are not contiguous are copied first
+    y2, _ = s.gated_scan(i["gate"].transpose(1, 2).contiguous().transpose(1, 2), i["x"], h0=i["h0"])
+    assert torch.equal(y2, y1)
+
+
+@pytest.mark.parametrize("T", [6, 300, 2100])
+def test_gated_scan_keeps_what_is_masked_out(dev, T):
+    """NaN and infinities behind a sequence's length do nothing; those of an episode end with it."""
+    s = seq()
+    B, D = 3, 24
+    for dtype in (torch.float32, torch.bfloat16):
+        i = scan_inputs(dev, dtype, B, T, D, T)
+        n = torch.tensor([0, T // 2, T - 1], dtype=torch.int32, device=dev)
+        clean = s.gated_scan(i["gate"], i["x"], i["h0"], lengths=n, save=True)
+        cg = s.gated_scan_backward(i["gate"], i["x"], clean[2], i["dy"], i["dh_last"], lengths=n)
+        bad = {k: i[k].clone() for k in ("gate", "x", "dy")}
+        for b in range(B):
+            bad["gate"][b, int(n[b]):] = float("nan")
+            bad["x"][b, int(n[b]):] = float("inf")
+            bad["dy"][b, int(n[b]):] = float("nan")
+        got = s.gated_scan(bad["gate"], bad["x"], i["h0"], lengths=n.long(), save=True)
+        gg = s.gated_scan_backward(bad["gate"], bad["x"], got[2], bad["dy"], i["dh_last"], lengths=n)
+        for u, v in zip(clean + cg, got + gg):
+            assert torch.equal(u, v)
+        for b in range(B):
+            assert not got[0][b, int(n[b]):].any() and not gg[0][b, int(n[b]):].any() and not gg[1][b, int(n[b]):].any()
+        assert torch.equal(got[1][0], i["h0"][0]) and torch.equal(gg[2][0], i["dh_last"][0])
+        # an episode full of NaN between two clean ones
+        lo, hi = T // 3, T // 2
+        st = torch.zeros((B, T), dtype=torch.bool, device=dev)
+        st[:, lo] = st[:, hi] = True
+        clean = s.gated_scan(i["gate"], i["x"], i["h0"], starts=st, save=True)
+        cg = s.gated_scan_backward(i["gate"], i["x"], clean[2], i["dy"], i["dh_last"], starts=st)
+        bad = {k: i[k].clone() for k in ("gate", "x", "dy")}
+        for k in bad:
+            bad[k][:, lo:hi] = float("nan")
+        got = s.gated_scan(bad["gate"], bad["x"], i["h0"], starts=st, save=True)
+        gg = s.gated_scan_backward(bad["gate"], bad["x"], got[2], bad["dy"], i["dh_last"], starts=st)
+        for u, v in zip(clean[:1] + cg[:2], got[:1] + gg[:2]):
+            assert torch.equal(u[:, :lo], v[:, :lo]) and torch.equal(u[:, hi:], v[:, hi:])
+            assert bool(v[:, lo:hi].isnan().all())
+        assert torch.equal(clean[1], got[1]) and torch.equal(cg[2], gg[2])
+
+
+def test_gated_scan_extreme_gates(dev):
+    """Gates at the ends of the type: remember exactly, replace exactly, infinities included."""
+    s = seq()
+    for dtype in DTYPES:
+        big = torch.finfo(dtype).max
+        gate = torch.tensor([big, float("inf"), -big, float("-inf"), 200.0, -200.0], dtype=dtype, device=dev).repeat(2, 40, 4)
+        x = torch.randn((2, 40, 24), device=dev).to(dtype)
+        h0 = torch.randn((2, 24), device=dev)
+        y, h, saved = s.gated_scan(gate, x, h0=h0, save=True)
+        keep = gate[0, 0] > 0
+        assert torch.equal(h[:, keep], h0[:, keep]) and torch.equal(y[:, :, ~keep], x[:, :, ~keep])
+        dg, dx, d0 = s.gated_scan_backward(gate, x, saved, torch.ones_like(x))
+        assert not dg.any() and not dx[:, :, keep].any() and bool((dx[:, :, ~keep] == 1).all())
+        assert bool((d0[:, keep] == 40).all()) and not d0[:, ~keep].any()
+
+
+def test_gated_scan_empty_sizes(dev):
+    s = seq()
+    h0 = torch.randn((3, 8), device=dev)
+    e = torch.empty((3, 0, 8), device=dev)
+    y, h, saved = s.gated_scan(e, e, h0=h0, save=True)
+    assert y.shape == (3, 0, 8) and torch.equal(h, h0) and saved.shape == (3, 0, 8)
+    assert not s.gated_scan(e, e)[1].any()
+    dg, dx, d0 = s.gated_scan_backward(e, e, saved, e, dh_last=h0)
+    assert dg.shape == dx.shape == (3, 0, 8) and torch.equal(d0, h0)
+    for shape in ((0, 5, 8), (2, 5, 0)):
+        e = torch.empty(shape, device=dev)
+        y, h, saved = s.gated_scan(e, e, save=True)
+        assert y.shape == shape and h.shape == (shape[0], shape[2])
+        assert s.gated_scan_backward(e, e, saved, e)[0].shape == shape
+
+
+def test_gated_scan_offsets_beyond_32_bits(dev):
+    """Steps that lie 2^26 elements apart: the last ones are beyond 2^32 bytes and 2^31 elements."""
+    s = seq()
+    T, D, far = 40, 16, 1 << 26
+    store = torch.empty((T - 1) * far + 2 * D, dtype=torch.bfloat16, device=dev)
+    gate, x = (torch.as_strided(store, (1, T, D), (0, far, 1), o) for o in (0, D))
+    i = scan_inputs(dev, torch.bfloat16, 1, T, D, 9)
+    gate.copy_(i["gate"])
+    x.copy_(i["x"])
+    a = s.gated_scan(i["gate"], i["x"], i["h0"], save=True)
+    b = s.gated_scan(gate, x, i["h0"], save=True)
+    ga = s.gated_scan_backward(i["gate"], i["x"], a[2], i["dy"], i["dh_last"])
+    gb = s.gated_scan_backward(gate, x, b[2], i["dy"], i["dh_last"])
+    for u, v in zip(a + ga, b + gb):
+        assert torch.equal(u, v)
+
+
+def replayed(dev, fn, outputs_of):
+    """fn captured and replayed with eager work between the replays: every replay gives the eager call's bits."""
+    want = [t.clone() for t in outputs_of(fn())]
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        fn()
+    torch.cuda.current_stream(dev).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = outputs_of(fn())
+    for k in range(4):
+        for t in out:
+            t.zero_()
+        eager = outputs_of(fn())
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v, w in zip(out, eager, want):
+            assert torch.equal(u, w) and torch.equal(v, w), f"replay {k}"
+
+
+def test_gated_scan_in_graphs_and_on_other_streams(dev):
+    s = seq()
+    for T in (1, 60, 2000):
+        i = scan_inputs(dev, torch.bfloat16, 2, T, 72, T, starts=True, lengths=True)
+
+        def train():
+            y, h, saved = s.gated_scan(i["gate"], i["x"], i["h0"], i["starts"], i["lengths"], save=True)
+            return (y, h) + s.gated_scan_backward(i["gate"], i["x"], saved, i["dy"], i["dh_last"], i["starts"], i["lengths"])
+        replayed(dev, train, list)
+        want = train()
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            got = train()
+        side.synchronize()
+        for u, v in zip(want, got):
+            assert torch.equal(u, v)
