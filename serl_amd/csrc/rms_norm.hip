@@ -1,0 +1,398 @@
+// Root-mean-square norm with the residual's addition:
+//   s = x + residual,  rstd = 1 / sqrt(mean(s^2) + eps),  y = s rstd w
+// its backward pass, and the form whose output is 8 bits (OCP e4m3) with one scale per row.  No counterpart in the
+// reference (its networks use LayerNorm, rowops.hip).
+//
+// Bound by memory: a row is read once into registers, reduced, and written; a wave takes a row of up to 1024 16-bit
+// elements (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
+// STORED (rounded to the residual's type): later layers and the backward pass see the values that were normed.
+#include "seqtypes.h"
+
+#define RMS_MAXN 32768
+#define RMS_PARTS 512        // rows of partial weight gradients: at most this many workgroups in the backward pass
+
+struct RmsArgs {
+  const void *x, *res, *w, *ds;      // backward: x = dy, res = s
+  long long ldx, ldres, ldds;
+  void *y, *sum; long long ldy, ldsum;
+  float *scale, *rstd_out, *part;
+  const float* rstd_in;
+  int R, N, w_f32; float eps;
+};
+
+// VEC weights from column n on, in the tensors' own 16-bit type or fp32
+template <typename T, int VEC>
+__device__ __forceinline__ void rms_weight(const RmsArgs& a, int n, float (&w)[VEC]) {
+  if (T::code == SERL_F32 || a.w_f32) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) w[v] = ((const float*)a.w)[n + v];
+  } else {
+    Raw<T, VEC> r;
+    r.load((const typename T::bits*)a.w + n);
+    r.get(w);
+  }
+}
+
+__device__ __forceinline__ unsigned rms_wave_max(unsigned v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const unsigned p = (unsigned)__shfl_xor((int)v, o);
+    v = v > p ? v : p;
+  }
+  return v;
+}
+
+// e4m3 codes of four values: rounded to nearest even, clipped to +-448 (an infinity as well), NaN stays NaN
+__device__ __forceinline__ float rms_clip(float v) { return v != v ? v : fminf(fmaxf(v, -448.f), 448.f); }
+__device__ __forceinline__ uint32_t rms_e4m3x4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(rms_clip(a), rms_clip(b), 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(rms_clip(c), rms_clip(d), r, true);
+  return (uint32_t)r;
+}
+
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC>
+__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(const RmsArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float red[WAVES];
+  __shared__ unsigned redm[WAVES];
+  const int t = threadIdx.x % THREADS, wave = t >> 6, lane = t & 63;
+  const int row = THREADS == 64 ? (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) : (int)blockIdx.x;
+  if (THREADS == 64 && row >= a.R) return;
+  const typename TX::bits* x = (const typename TX::bits*)a.x + row * a.ldx;
+  Raw<TX, VEC> rx[NV];
+  Raw<TR, VEC> rr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {        // unconditional: a column behind the row reads the row's first ones, not used
+    const int n = (i * THREADS + t) * VEC;
+    rx[i].load(x + (n < a.N ? n : 0));
+  }
+  if (a.res) {
+    const typename TR::bits* res = (const typename TR::bits*)a.res + row * a.ldres;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = (i * THREADS + t) * VEC;
+      rr[i].load(res + (n < a.N ? n : 0));
+    }
+  }
+  float s[NV][VEC], ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const bool in = (i * THREADS + t) * VEC < a.N;
+    rx[i].get(s[i]);
+    if (a.res) {
+      float r[VEC];
+      rr[i].get(r);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s[i][v] += r[v];
+      rr[i].put(s[i]);
+      rr[i].get(s[i]);
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) ss = in ? fmaf(s[i][v], s[i][v], ss) : ss;
+  }
+  if (a.sum) {
+    typename TR::bits* sum = (typename TR::bits*)a.sum + row * a.ldsum;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = (i * THREADS + t) * VEC;
+      if (n < a.N) rr[i].store(sum + n);
+    }
+  }
+  ss = sq_wave_sum(ss);
+  if constexpr (WAVES > 1) {
+    if (lane == 0) red[wave] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) ss += red[w];
+  }
+  const float rstd = rsqrtf(ss / (float)a.N + a.eps);
+  if (a.rstd_out && t == 0) a.rstd_out[row] = rstd;
+  unsigned top = 0;                     // |y| as bits: ordered like the values, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int n = (i * THREADS + t) * VEC;
+    float w[VEC];
+    rms_weight<TX, VEC>(a, n < a.N ? n : 0, w);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      s[i][v] = s[i][v] * rstd * w[v];
+      if (FP8) {
+        const unsigned m = __float_as_uint(s[i][v]) & 0x7fffffffu;
+        top = n < a.N && m > top ? m : top;
+      }
+    }
+    if (!FP8 && n < a.N) {
+      rx[i].put(s[i]);
+      rx[i].store((typename TX::bits*)a.y + row * a.ldy + n);
+    }
+  }
+  if constexpr (FP8) {
+    top = rms_wave_max(top);
+    if constexpr (WAVES > 1) {
+      if (lane == 0) redm[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) top = redm[w] > top ? redm[w] : top;
+    }
+    float scale = __uint_as_float(top) / 448.f;
+    scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;      // so that 1 / scale is finite
+    scale = top == 0 ? 1.f : scale;
+    if (t == 0) a.scale[row] = scale;
+    const float inv = 1.f / scale;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = (i * THREADS + t) * VEC;
+      unsigned char* q = (unsigned char*)a.y + row * a.ldy + n;
+      if (n < a.N) {
+        if constexpr (VEC == 8) {
+          *(sq_u32x2*)q = (sq_u32x2){rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv),
+                                     rms_e4m3x4(s[i][4] * inv, s[i][5] * inv, s[i][6] * inv, s[i][7] * inv)};
+        } else if constexpr (VEC == 4) {
+          *(uint32_t*)q = rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv);
+        } else {
+          *q = (unsigned char)(rms_e4m3x4(s[i][0] * inv, 0.f, 0.f, 0.f) & 0xffu);
+        }
+      }
+    }
+  }
+}
+
+// dx = rstd (w dy - xh mean(w dy xh)) + ds with xh = s rstd; dw = sum over rows of dy xh.  A workgroup (THREADS = 64: a
+// wave) takes every gridDim-th row and keeps its share of dw in registers; the shares are added in a fixed order by
+// rms_dw_kernel, so the result does not depend on timing.
+template <typename TY, typename TS, int THREADS, int NV, int VEC>
+__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_bwd_kernel(const RmsArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float red[2][WAVES];
+  const int t = threadIdx.x % THREADS, wave = t >> 6, lane = t & 63;
+  const int first = THREADS == 64 ? (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) : (int)blockIdx.x;
+  const int step = THREADS == 64 ? (int)gridDim.x * 4 : (int)gridDim.x;
+  float w[NV][VEC], dw[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int n = (i * THREADS + t) * VEC;
+    rms_weight<TY, VEC>(a, n < a.N ? n : 0, w[i]);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) dw[i][v] = 0.f;
+  }
+  int buf = 0;
+  for (int row = first; row < a.R; row += step, buf ^= 1) {
+    const typename TY::bits* dy = (const typename TY::bits*)a.x + row * a.ldx;
+    const typename TS::bits* s = (const typename TS::bits*)a.res + row * a.ldres;
+    const typename TS::bits* ds = (const typename TS::bits*)a.ds + row * a.ldds;
+    const float rstd = a.rstd_in[row];
+    Raw<TY, VEC> ry[NV];
+    Raw<TS, VEC> rs[NV], rd[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = (i * THREADS + t) * VEC, m = n < a.N ? n : 0;
+      ry[i].load(dy + m);
+      rs[i].load(s + m);
+    }
+    if (a.ds) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int n = (i * THREADS + t) * VEC;
+        rd[i].load(ds + (n < a.N ? n : 0));
+      }
+    }
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const bool in = (i * THREADS + t) * VEC < a.N;
+      float y[VEC], x[VEC];
+      ry[i].get(y);
+      rs[i].get(x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float d = y[v] * (x[v] * rstd);
+        dw[i][v] += d;
+        dot = in ? fmaf(w[i][v], d, dot) : dot;
+      }
+    }
+    dot = sq_wave_sum(dot);
+    if constexpr (WAVES > 1) {
+      if (lane == 0) red[buf][wave] = dot;
+      __syncthreads();
+      dot = 0.f;
+#pragma unroll
+      for (int q = 0; q < WAVES; ++q) dot += red[buf][q];
+    }
+    dot /= (float)a.N;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = (i * THREADS + t) * VEC;
+      float y[VEC], x[VEC], d[VEC];
+      ry[i].get(y);
+      rs[i].get(x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) d[v] = 0.f;
+      if (a.ds) rd[i].get(d);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) d[v] = fmaf(rstd, fmaf(-(x[v] * rstd), dot, y[v] * w[i][v]), d[v]);
+      rs[i].put(d);
+      if (n < a.N) rs[i].store((typename TS::bits*)a.y + row * a.ldy + n);
+    }
+  }
+  float* part = a.part + (long long)first * a.N;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int n = (i * THREADS + t) * VEC;
+    if (n < a.N)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) part[n + v] = dw[i][v];
+  }
+}
+
+// dw[n] = sum over the parts, 32 columns x 32 part lanes per workgroup, the lanes' sums added in order
+__global__ __launch_bounds__(1024) void rms_dw_kernel(const float* part, int parts, int N, float* dw) {
+  __shared__ float sum[32][33];
+  const int c = threadIdx.x & 31, p0 = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (n < N) {
+#pragma unroll 8
+    for (int p = p0; p < parts; p += 32) s += part[(long long)p * N + n];
+  }
+  sum[p0][c] = s;
+  __syncthreads();
+  if (p0 == 0 && n < N) {
+    s = 0.f;
+#pragma unroll
+    for (int p = 0; p < 32; ++p) s += sum[p][c];
+    dw[n] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC>
+static void rms_go_fwd(const RmsArgs& a, hipStream_t st) {
+  const unsigned grid = THREADS == 64 ? (unsigned)cdiv(a.R, 4) : (unsigned)a.R;
+  hipLaunchKernelGGL((rms_fwd_kernel<TX, TR, FP8, THREADS, NV, VEC>), dim3(grid), dim3(THREADS == 64 ? 256 : THREADS), 0, st, a);
+}
+template <typename TX, typename TR, bool FP8>
+static void rms_pick_fwd(const RmsArgs& a, bool wide, hipStream_t st) {
+  constexpr int V = TX::code == SERL_F32 ? 4 : 8;
+  const int n = cdiv(a.N, wide ? V : 1);          // vectors of a row
+  if (!wide) {
+    if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, 1>(a, st);
+    else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 256, 16, 1>(a, st);
+    else rms_go_fwd<TX, TR, FP8, 1024, 32, 1>(a, st);
+  } else if (n <= 64) rms_go_fwd<TX, TR, FP8, 64, 1, V>(a, st);
+  else if (n <= 128) rms_go_fwd<TX, TR, FP8, 64, 2, V>(a, st);
+  else if (n <= 256) rms_go_fwd<TX, TR, FP8, 256, 1, V>(a, st);
+  else if (n <= 512) rms_go_fwd<TX, TR, FP8, 256, 2, V>(a, st);
+  else if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, V>(a, st);
+  else if (n <= 2048) rms_go_fwd<TX, TR, FP8, 1024, 2, V>(a, st);
+  else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 1024, 4, V>(a, st);
+  else rms_go_fwd<TX, TR, FP8, 1024, 8, V>(a, st);      // fp32 only: RMS_MAXN elements
+}
+
+// rows of the partial weight gradients: one per row of the input up to RMS_PARTS workgroups
+static int rms_parts(int R) { return R < RMS_PARTS ? (R + 3) / 4 * 4 : RMS_PARTS; }
+
+template <typename TY, typename TS, int THREADS, int NV, int VEC>
+static void rms_go_bwd(const RmsArgs& a, hipStream_t st) {
+  const int parts = rms_parts(a.R);
+  hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC>), dim3(THREADS == 64 ? parts / 4 : parts),
+                     dim3(THREADS == 64 ? 256 : THREADS), 0, st, a);
+}
+template <typename TY, typename TS>
+static void rms_pick_bwd(const RmsArgs& a, bool wide, hipStream_t st) {
+  constexpr int V = TY::code == SERL_F32 ? 4 : 8;
+  const int n = cdiv(a.N, wide ? V : 1);
+  if (!wide) {
+    if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, 1>(a, st);
+    else if (n <= 4096) rms_go_bwd<TY, TS, 256, 16, 1>(a, st);
+    else rms_go_bwd<TY, TS, 1024, 32, 1>(a, st);
+  } else if (n <= 64) rms_go_bwd<TY, TS, 64, 1, V>(a, st);
+  else if (n <= 128) rms_go_bwd<TY, TS, 64, 2, V>(a, st);
+  else if (n <= 256) rms_go_bwd<TY, TS, 256, 1, V>(a, st);
+  else if (n <= 512) rms_go_bwd<TY, TS, 256, 2, V>(a, st);
+  else if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, V>(a, st);
+  else if (n <= 2048) rms_go_bwd<TY, TS, 1024, 2, V>(a, st);
+  else if (n <= 4096) rms_go_bwd<TY, TS, 1024, 4, V>(a, st);
+  else rms_go_bwd<TY, TS, 1024, 8, V>(a, st);
+}
+
+static bool rms_wide(int type, int elems, const void* p, long long ld) {
+  const int e = type == SERL_F32 ? 4 : 2;
+  return !p || (sq_aligned(p, 16) && ld % elems == 0 && (ld * e) % 16 == 0);
+}
+
+// x and y of type `type`, residual and sum of type `stream_type` (the same, or fp32), weight of type `type` or fp32.
+static int rms_check(const char* what, int type, int stream_type, int weight_type, int R, int N) {
+  SERL_CHECK_ARG(type >= 0 && type <= 2, "%s: type must be 0 (fp32), 1 (bf16) or 2 (fp16)", what);
+  SERL_CHECK_ARG(stream_type == type || stream_type == SERL_F32, "%s: the residual's type must be x's or fp32", what);
+  SERL_CHECK_ARG(weight_type == type || weight_type == SERL_F32, "%s: the weight's type must be x's or fp32", what);
+  SERL_CHECK_ARG(R >= 0 && N >= 1 && N <= RMS_MAXN, "%s: N must be in [1, %d], R >= 0", what, RMS_MAXN);
+  return SERL_OK;
+}
+
+extern "C" int serl_rms_norm_fwd(int type, int stream_type, int weight_type, int R, int N, const void* x, long long ldx,
+                                 const void* residual, long long ldres, const void* weight, float eps, void* y,
+                                 long long ldy, int y_fp8, float* scale, void* sum, long long ldsum, float* rstd,
+                                 void* stream) {
+  const int bad = rms_check("rms_norm_fwd", type, stream_type, weight_type, R, N);
+  if (bad) return bad;
+  if (R == 0) return SERL_OK;
+  SERL_CHECK_ARG(x && weight && y, "rms_norm_fwd: null pointer");
+  SERL_CHECK_ARG((residual != nullptr) == (sum != nullptr), "rms_norm_fwd: residual and sum go together");
+  SERL_CHECK_ARG(residual || stream_type == type, "rms_norm_fwd: without a residual its type is x's");
+  SERL_CHECK_ARG(!y_fp8 || scale, "rms_norm_fwd: 8-bit output needs the scales' buffer");
+  SERL_CHECK_ARG(ldx >= 0 && ldres >= 0 && (R <= 1 || (ldy >= N && (!sum || ldsum >= N))),
+                 "rms_norm_fwd: negative row stride, or output rows overlap");
+  const int V = type == SERL_F32 ? 4 : 8;
+  const bool wide = N % V == 0 && rms_wide(type, V, x, ldx) && rms_wide(stream_type, V, residual, ldres) &&
+                    rms_wide(stream_type, V, sum, ldsum) && sq_aligned(weight, 16) &&
+                    (y_fp8 ? sq_aligned(y, V) && ldy % V == 0 : rms_wide(type, V, y, ldy));
+  RmsArgs a{};
+  a.x = x; a.ldx = ldx; a.res = residual; a.ldres = ldres; a.w = weight; a.w_f32 = weight_type == SERL_F32; a.y = y;
+  a.ldy = ldy; a.scale = scale; a.sum = sum; a.ldsum = ldsum; a.rstd_out = rstd; a.R = R; a.N = N; a.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+#define RMS_GO(TX, TR) (y_fp8 ? rms_pick_fwd<TX, TR, true>(a, wide, st) : rms_pick_fwd<TX, TR, false>(a, wide, st))
+  if (type == SERL_F32) RMS_GO(F32, F32);
+  else if (type == SERL_BF16) { if (stream_type == SERL_F32) RMS_GO(BF16, F32); else RMS_GO(BF16, BF16); }
+  else { if (stream_type == SERL_F32) RMS_GO(F16, F32); else RMS_GO(F16, F16); }
+#undef RMS_GO
+  SERL_CHECK_LAUNCH("rms_norm_fwd");
+  return SERL_OK;
+}
+
+extern "C" long long serl_rms_norm_bwd_workspace_bytes(int R, int N) {
+  if (R < 0 || N < 1 || N > RMS_MAXN) {
+    serl_set_error("rms_norm_bwd: N must be in [1, %d], R >= 0", RMS_MAXN);
+    return -1;
+  }
+  return (long long)rms_parts(R) * N * 4;
+}
+
+extern "C" int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int R, int N, const void* dy, long long lddy,
+                                 const void* sum, long long ldsum, const float* rstd, const void* weight, const void* ds,
+                                 long long ldds, void* dx, long long lddx, float* dweight, float* workspace,
+                                 long long workspace_bytes, void* stream) {
+  const int bad = rms_check("rms_norm_bwd", type, stream_type, weight_type, R, N);
+  if (bad) return bad;
+  SERL_CHECK_ARG(dweight && (R == 0 || (dy && sum && rstd && weight && dx)), "rms_norm_bwd: null pointer");
+  SERL_CHECK_ARG(lddy >= 0 && ldsum >= 0 && ldds >= 0 && (R <= 1 || lddx >= N),
+                 "rms_norm_bwd: negative row stride, or output rows overlap");
+  const int parts = rms_parts(R);
+  const long long need = (long long)parts * N * 4;
+  SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
+                 "rms_norm_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
+  const int V = type == SERL_F32 ? 4 : 8;
+  const bool wide = N % V == 0 && rms_wide(type, V, dy, lddy) && rms_wide(stream_type, V, sum, ldsum) &&
+                    rms_wide(stream_type, V, ds, ldds) && rms_wide(stream_type, V, dx, lddx) && sq_aligned(weight, 16);
+  RmsArgs a{};
+  a.x = dy; a.ldx = lddy; a.res = sum; a.ldres = ldsum; a.rstd_in = rstd; a.w = weight; a.w_f32 = weight_type == SERL_F32;
+  a.ds = ds; a.ldds = ldds; a.y = dx; a.ldy = lddx; a.part = workspace; a.R = R; a.N = N;
+  hipStream_t st = (hipStream_t)stream;
+  if (R > 0) {
+    if (type == SERL_F32) rms_pick_bwd<F32, F32>(a, wide, st);
+    else if (type == SERL_BF16) { if (stream_type == SERL_F32) rms_pick_bwd<BF16, F32>(a, wide, st); else rms_pick_bwd<BF16, BF16>(a, wide, st); }
+    else { if (stream_type == SERL_F32) rms_pick_bwd<F16, F32>(a, wide, st); else rms_pick_bwd<F16, F16>(a, wide, st); }
+  }
+  hipLaunchKernelGGL(rms_dw_kernel, dim3(cdiv(N, 32)), dim3(1024), 0, st, (const float*)workspace, parts, N, dweight);
+  SERL_CHECK_LAUNCH("rms_norm_bwd");
+  return SERL_OK;
+}

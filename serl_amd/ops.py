@@ -373,3 +373,19 @@ def gated_scan_bwd(dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, starts
     call("serl_gated_scan_bwd", dtype, B, T, D, gate, gate_bs, gate_ts, x, x_bs, x_ts, starts, starts_bs, lengths,
          states, dy, dy_bs, dy_ts, dh_last, dgate, dgate_bs, dgate_ts, dx, dx_bs, dx_ts, dh0, workspace,
          workspace_bytes, stream)
+
+
+def rms_norm_fwd(dtype, stream_dtype, weight_dtype, R, N, x, ldx, residual, ldres, weight, eps, y, ldy, y_fp8, scale, sum_,
+                 ldsum, rstd, stream):
+    call("serl_rms_norm_fwd", dtype, stream_dtype, weight_dtype, R, N, x, ldx, residual, ldres, weight, float(eps), y, ldy,
+         int(y_fp8), scale, sum_, ldsum, rstd, stream)
+
+
+def rms_norm_bwd_workspace_bytes(R, N) -> int:
+    return _nbytes(_lib.load().serl_rms_norm_bwd_workspace_bytes(R, N), "rms_norm_bwd_workspace_bytes")
+
+
+def rms_norm_bwd(dtype, stream_dtype, weight_dtype, R, N, dy, lddy, sum_, ldsum, rstd, weight, ds, ldds, dx, lddx, dweight,
+                 workspace, workspace_bytes, stream):
+    call("serl_rms_norm_bwd", dtype, stream_dtype, weight_dtype, R, N, dy, lddy, sum_, ldsum, rstd, weight, ds, ldds, dx,
+         lddx, dweight, workspace, workspace_bytes, stream)

@@ -196,3 +196,95 @@ def gated_scan_step(gate, x, h, starts=None, h_out=None):
                            h.data_ptr(), _ptr(starts), 0 if starts is None else starts.stride(0), None, y.data_ptr(), D, D,
                            h_out.data_ptr(), None, None, 0, ops.current_stream())
     return y, h_out
+
+
+# --------------------------------------------------------------------------------- root-mean-square norm + residual
+def _rows(t):
+    """t as (R, N) rows with contiguous channels (a view wherever its strides allow one)."""
+    t = _channels(t)
+    return t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _width(t, name):
+    if not isinstance(t, torch.Tensor) or t.ndim < 1:
+        raise ValueError(f"{name} must be a (..., N) tensor")
+    if not 1 <= t.shape[-1] <= 32768:
+        raise ValueError(f"{name}: N must be in [1, 32768], got {t.shape[-1]}")
+
+
+def _norm_args(x, weight, residual):
+    _width(x, "x")
+    if x.dtype not in _CODES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    _shape(weight, "weight", (x.shape[-1],))
+    _type(weight, "weight", x.dtype, torch.float32)
+    if residual is not None:
+        _shape(residual, "residual", x.shape)
+        _type(residual, "residual", x.dtype, torch.float32)
+
+
+def _norm(x, weight, residual, eps, fp8, save):
+    _norm_args(x, weight, residual)
+    with _place(("x", x), ("weight", weight), ("residual", residual)):
+        shape, N = x.shape, x.shape[-1]
+        rows, res, weight = _rows(x), None if residual is None else _rows(residual), weight.contiguous()
+        R, dev = rows.shape[0], x.device
+        y = torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if fp8 else None
+        total = x if res is None else torch.empty(shape, dtype=residual.dtype, device=dev)
+        rstd = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if save else None
+        code = _CODES[x.dtype]
+        ops.rms_norm_fwd(code, code if res is None else _CODES[residual.dtype], _CODES[weight.dtype], R, N, rows.data_ptr(),
+                         rows.stride(0), _ptr(res), 0 if res is None else res.stride(0), weight.data_ptr(), eps, y.data_ptr(),
+                         N, fp8, _ptr(scale), None if res is None else total.data_ptr(), N, _ptr(rstd), ops.current_stream())
+    return y, scale, total, rstd
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, save=False):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension (1 .. 32768), s = x + residual.
+
+    residual: x's shape, in x's type or float32 (a residual stream kept in 32 bits); weight (N,) in x's type or float32.
+    Returns (y, s): y in x's type, s in the residual's (rounded to it before it is normed), or x itself without a residual;
+    with save=True also rstd (...,) float32 for rms_norm_backward."""
+    y, _, total, rstd = _norm(x, weight, residual, eps, False, save)
+    return (y, total, rstd) if save else (y, total)
+
+
+def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
+    """rms_norm with its output in 8 bits: (q, scale, s), q float8_e4m3fn and scale (...,) float32 per row such that
+    y = q * scale; scale = max(|y|) / 448, at least 2^-126, and 1 for a row of zeros.  A row that holds a NaN has the
+    scale NaN."""
+    y, scale, total, _ = _norm(x, weight, residual, eps, True, False)
+    return y, scale, total
+
+
+def rms_norm_backward(dy, s, rstd, weight, ds=None):
+    """Gradients of rms_norm: (dx, dweight).  s and rstd as the forward call returned them; dy in the type of its x; ds: the
+    gradient that reaches s itself (the residual stream behind), in s's type.  dx, in s's type, is the gradient of x and of
+    the residual alike; dweight (N,) float32."""
+    _width(s, "s")
+    _shape(dy, "dy", s.shape)
+    if dy.dtype not in _CODES:
+        raise TypeError(f"dy must be float32, bfloat16 or float16, got {dy.dtype}")
+    _type(s, "s", dy.dtype, torch.float32)
+    _shape(rstd, "rstd", s.shape[:-1])
+    _type(rstd, "rstd", torch.float32)
+    _shape(weight, "weight", (s.shape[-1],))
+    _type(weight, "weight", dy.dtype, torch.float32)
+    if ds is not None:
+        _shape(ds, "ds", s.shape)
+        _type(ds, "ds", s.dtype)
+    with _place(("s", s), ("dy", dy), ("rstd", rstd), ("weight", weight), ("ds", ds)):
+        shape, N = s.shape, s.shape[-1]
+        sr, yr, dr = _rows(s), _rows(dy), None if ds is None else _rows(ds)
+        weight, rstd = weight.contiguous(), rstd.contiguous()
+        R, dev = sr.shape[0], s.device
+        dx = torch.empty(shape, dtype=s.dtype, device=dev)
+        dw = torch.empty((N,), dtype=torch.float32, device=dev)
+        n = ops.rms_norm_bwd_workspace_bytes(R, N)
+        ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
+        ops.rms_norm_bwd(_CODES[dy.dtype], _CODES[s.dtype], _CODES[weight.dtype], R, N, yr.data_ptr(), yr.stride(0),
+                         sr.data_ptr(), sr.stride(0), rstd.data_ptr(), weight.data_ptr(), _ptr(dr),
+                         0 if dr is None else dr.stride(0), dx.data_ptr(), N, dw.data_ptr(), _ptr(ws), n,
+                         ops.current_stream())
+    return dx, dw

@@ -81,3 +81,44 @@ def test_gated_scan_entry_point_refusals():
         bwd(states=None)
     with pytest.raises(ValueError, match="rows of dgate or dx overlap"):
         bwd(dx_bs=4)
+
+
+def test_rms_norm_refusals():
+    x, w = t(4, 8), t(8)
+    with pytest.raises(ValueError, match=r"x must be a \(\.\.\., N\) tensor"):
+        sequence.rms_norm(t(), w)
+    with pytest.raises(ValueError, match="N must be in"):
+        sequence.rms_norm(t(4, 0), t(0))
+    with pytest.raises(ValueError, match="N must be in"):
+        sequence.rms_norm_fp8(t(1, 32769), t(32769))
+    with pytest.raises(TypeError, match="x must be float32"):
+        sequence.rms_norm(x.double(), w)
+    with pytest.raises(ValueError, match="weight must have the shape"):
+        sequence.rms_norm(x, t(9))
+    with pytest.raises(TypeError, match="weight must be"):
+        sequence.rms_norm(x.half(), w.bfloat16())
+    with pytest.raises(ValueError, match="residual must have the shape"):
+        sequence.rms_norm(x, w, residual=t(3, 8))
+    with pytest.raises(TypeError, match="residual must be"):
+        sequence.rms_norm(x, w, residual=x.half())
+    with pytest.raises(TypeError, match="x must be a CUDA tensor"):
+        sequence.rms_norm(x, w)
+    with pytest.raises(ValueError, match="rstd must have the shape"):
+        sequence.rms_norm_backward(x, x, t(5), w)
+    with pytest.raises(TypeError, match="ds must be"):
+        sequence.rms_norm_backward(x.half(), x, t(4), w, ds=x.half())
+    with pytest.raises(TypeError, match="s must be"):
+        sequence.rms_norm_backward(x, x.half(), t(4), w)
+    fwd = lambda **k: ops.rms_norm_fwd(*{**dict(  # noqa: E731
+        dtype=1, stream=1, weight=1, R=4, N=8, x=16, ldx=8, residual=16, ldres=8, w=16, eps=1e-6, y=16, ldy=8, y_fp8=0,
+        scale=None, sum=16, ldsum=8, rstd=None, st=0), **k}.values())
+    for match, kw in (("type must be", dict(dtype=5)), ("residual's type", dict(stream=2)), ("weight's type", dict(weight=2)),
+                      ("N must be", dict(N=0)), ("N must be", dict(R=-1)), ("null pointer", dict(w=None)),
+                      ("go together", dict(sum=None)), ("its type is x's", dict(residual=None, sum=None, stream=0)),
+                      ("scales' buffer", dict(y_fp8=1)), ("overlap", dict(ldy=7)), ("negative", dict(ldx=-8))):
+        with pytest.raises(ValueError, match=match):
+            fwd(**kw)
+    with pytest.raises(ValueError, match=r"workspace of 128 bytes needed, 127 available"):
+        ops.rms_norm_bwd(1, 1, 1, 4, 8, 16, 8, 16, 8, 16, 16, None, 0, 16, 8, 16, 16, 127, 0)
+    with pytest.raises(ValueError, match="N must be"):
+        ops.rms_norm_bwd_workspace_bytes(4, 40000)

@@ -13,6 +13,7 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 HALF = {d: torch.finfo(d).eps / 2 for d in DTYPES}
 U = 2.0 ** -24
+SMALL = 2.0 ** -25      # half a step among fp16's subnormal numbers: they are multiples of 2^-24 (smallest_normal 2^-14 * eps 2^-10)
 
 
 def seq():
@@ -81,7 +82,7 @@ def check_scan(i, dtype, with_backward=True):
     assert torch.equal(y, y2) and torch.equal(h, h2) and y.dtype == dtype and h.dtype == torch.float32
     ry, rh, rg, rx, r0 = scan_reference(i["gate"], i["x"], i["h0"], i["starts"], i["lengths"], i["dy"], i["dh_last"])
     hm = max(1.0, float(rh.detach().abs().max()), float(ry.detach().abs().max()))
-    within(y, ry, SCAN_STATE * hm + HALF[dtype] * ry.detach().abs() + 2.0 ** -26, "y")
+    within(y, ry, SCAN_STATE * hm + HALF[dtype] * ry.detach().abs() + SMALL, "y")
     within(h, rh, SCAN_STATE * hm, "h_last")
     if not with_backward:
         return
@@ -91,10 +92,10 @@ def check_scan(i, dtype, with_backward=True):
     gm = 57 * max(float(i["dy"].abs().max()), float(i["dh_last"].abs().max()))
     xm = float(i["x"].abs().max())
     within(d0, r0, SCAN_STATE * gm, "dh0")
-    within(dx, rx, SCAN_STATE * gm + HALF[dtype] * rx.abs() + 2.0 ** -26, "dx")
+    within(dx, rx, SCAN_STATE * gm + HALF[dtype] * rx.abs() + SMALL, "dx")
     # dgate = G (h - x) f (1 - f): the errors of G and of h, each by the other's size, with f (1 - f) <= 1/4; 2^-26: half
     # a step among fp16's smallest numbers
-    within(dg, rg, 2 * SCAN_STATE * gm * (hm + xm) / 4 + HALF[dtype] * rg.abs() + 2.0 ** -26, "dgate")
+    within(dg, rg, 2 * SCAN_STATE * gm * (hm + xm) / 4 + HALF[dtype] * rg.abs() + SMALL, "dgate")
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -297,3 +298,178 @@ def test_gated_scan_in_graphs_and_on_other_streams(dev):
         side.synchronize()
         for u, v in zip(want, got):
             assert torch.equal(u, v)
+
+
+# ------------------------------------------------------------------------------------------- root-mean-square norm
+def norm_inputs(dev, dtype, stream, R, N, seed, wtype=None):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    return dict(x=r(R, N).to(dtype).to(dev), residual=None if stream is None else (3 * r(R, N)).to(stream).to(dev),
+                weight=(1 + 0.3 * r(N)).to(wtype or dtype).to(dev), dy=r(R, N).to(dtype).to(dev),
+                ds=r(R, N).to(stream or dtype).to(dev))
+
+
+# mean of squares: a thread adds at most 32 of them, 6 shuffle steps and 16 waves; half of that for the root, then the
+# division, the root and the two products
+NORM_Y = (54 / 2 + 6) * U
+
+
+def check_norm(i, dtype, eps=1e-6):
+    s = seq()
+    R, N = i["x"].shape
+    y, total, rstd = s.rms_norm(i["x"], i["weight"], residual=i["residual"], eps=eps, save=True)
+    y2, total2 = s.rms_norm(i["x"], i["weight"], residual=i["residual"], eps=eps)
+    assert torch.equal(y, y2) and torch.equal(total, total2) and y.dtype == dtype and rstd.dtype == torch.float32
+    if i["residual"] is None:
+        assert total is i["x"]
+    else:
+        full = i["x"].double() + i["residual"].double()
+        assert total.dtype == i["residual"].dtype
+        within(total, full, (HALF[total.dtype] + U) * full.abs().cpu() + SMALL, "sum")
+    v, w = total.double().cpu(), i["weight"].double().cpu()
+    r = 1 / torch.sqrt((v * v).mean(1, keepdim=True) + eps)
+    ref = v * r * w
+    within(rstd, r[:, 0], NORM_Y * r[:, 0], "rstd")
+    within(y, ref, (NORM_Y + HALF[dtype]) * ref.abs() + SMALL, "y")
+    q, scale, total3 = s.rms_norm_fp8(i["x"], i["weight"], residual=i["residual"], eps=eps)
+    assert q.dtype == torch.float8_e4m3fn and torch.equal(total3, total)
+    top = ref.abs().amax(1)
+    within(scale, top / 448, (NORM_Y + 2 * U) * top / 448, "scale")
+    # e4m3: half a step is 2^-4 of the value, or 2^-10 of the scale among its smallest numbers
+    back = q.double().cpu() * scale.double().cpu()[:, None]
+    within(back, ref, (2.0 ** -4 + 2 * NORM_Y + 4 * U) * ref.abs() + 2.0 ** -10 * scale.double().cpu()[:, None], "8 bits")
+    for ds in (i["ds"], None):
+        dx, dw = s.rms_norm_backward(i["dy"], total, rstd, i["weight"], ds=ds)
+        assert dx.dtype == total.dtype and dw.dtype == torch.float32 and dw.shape == (N,)
+        vv, ww = v.clone().requires_grad_(), w.clone().requires_grad_()
+        out = vv / torch.sqrt((vv * vv).mean(1, keepdim=True) + eps) * ww
+        rx, rw = torch.autograd.grad((out * i["dy"].double().cpu()).sum(), (vv, ww))
+        add = 0 if ds is None else ds.double().cpu()
+        dyw, xh = i["dy"].double().cpu() * w, v * r
+        size = r * (dyw.abs() + xh.abs() * (dyw * xh).abs().mean(1, keepdim=True)) + (0 if ds is None else add.abs())
+        within(dx, rx + add, 2 * (NORM_Y + 54 * U) * size + HALF[dx.dtype] * (rx + add).abs() + SMALL, "dx")
+        # a share adds R / 512 rows, a lane of the last step 16 shares, then 32 lanes
+        within(dw, rw, (R / 512 + 52 + NORM_Y / U) * U * (i["dy"].double().cpu() * xh).abs().sum(0) + 1e-30, "dweight")
+
+
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, None), (torch.float32, torch.float32), (torch.bfloat16, None),
+                                          (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                          (torch.float16, torch.float16), (torch.float16, torch.float32)], ids=str)
+def test_rms_norm_matches_its_formulas(dev, dtype, stream):
+    for R, N in ((1, 1), (3, 7), (5, 64), (1, 512), (6, 520), (2, 1000), (3, 1001), (2, 1024), (3, 2048), (2, 2056), (5, 4096),
+                 (2, 4097), (3, 8192), (1, 12288), (2, 16384), (1, 20000), (2, 32767), (1, 32768)):
+        check_norm(norm_inputs(dev, dtype, stream, R, N, R + N), dtype)
+    check_norm(norm_inputs(dev, dtype, stream, 3, 264, 1, wtype=torch.float32), dtype, eps=0.5)
+
+
+@pytest.mark.parametrize("R,N", [(513, 40), (2051, 33), (700, 1100), (1030, 2064)])
+def test_rms_norm_many_rows(dev, R, N):
+    for dtype in (torch.float32, torch.bfloat16):
+        check_norm(norm_inputs(dev, dtype, dtype, R, N, R), dtype)
+
+
+def test_rms_norm_views_shapes_and_empty_rows(dev):
+    s = seq()
+    i = norm_inputs(dev, torch.bfloat16, torch.bfloat16, 24, 72, 4)
+    y, total, rstd = s.rms_norm(i["x"], i["weight"], i["residual"], save=True)
+    dx, dw = s.rms_norm_backward(i["dy"], total, rstd, i["weight"], i["ds"])
+    for off, pad in ((0, 8), (1, 3), (8, 0)):
+        def view(t):
+            big = torch.full((24, off + 72 + pad), float("nan"), dtype=t.dtype, device=dev)
+            big[:, off:off + 72] = t
+            return big[:, off:off + 72]
+        v = {k: view(i[k]) for k in ("x", "residual", "dy", "ds")}
+        y2, total2, rstd2 = s.rms_norm(v["x"], i["weight"], v["residual"], save=True)
+        assert torch.equal(total, total2)
+        within(rstd2, rstd, 2 * NORM_Y * rstd.double().cpu(), "rstd")
+        within(y2, y, 2 * (NORM_Y + HALF[torch.bfloat16]) * y.double().abs().cpu(), "y")
+        dx2, dw2 = s.rms_norm_backward(v["dy"], view(total), rstd, i["weight"], v["ds"])
+        within(dx2, dx, 2 * HALF[torch.bfloat16] * dx.double().abs().cpu() + 1e-4, "dx")
+        within(dw2, dw, 2 * (52 * U) * 24 * 20 * torch.ones(72), "dw")
+    shaped = s.rms_norm(i["x"].view(2, 3, 4, 72), i["weight"], i["residual"].view(2, 3, 4, 72), save=True)
+    assert shaped[0].shape == (2, 3, 4, 72) and shaped[2].shape == (2, 3, 4) and torch.equal(shaped[0].view(24, 72), y)
+    assert torch.equal(s.rms_norm_backward(i["dy"].view(2, 3, 4, 72), shaped[1], shaped[2], i["weight"], i["ds"].view(2, 3, 4, 72))[1], dw)
+    one = s.rms_norm_fp8(i["x"][3], i["weight"], i["residual"][3])
+    assert one[0].shape == (72,) and one[1].shape == () and torch.equal(one[2], total[3])
+    t = s.rms_norm(i["x"].t().contiguous().t(), i["weight"], i["residual"], save=True)     # channels not contiguous: copied
+    assert torch.equal(t[0], y)
+    e = i["x"][:0]
+    y, total, rstd = s.rms_norm(e, i["weight"], e, save=True)
+    dx, dw = s.rms_norm_backward(e, total, rstd, i["weight"])
+    assert y.shape == dx.shape == (0, 72) and dw.shape == (72,) and not dw.any()
+    assert s.rms_norm_fp8(e, i["weight"])[1].shape == (0,)
+
+
+def test_rms_norm_special_rows(dev):
+    """Rows of zeros, of the type's smallest and largest values, with infinities and NaN; each leaves the others alone."""
+    s = seq()
+    for dtype in DTYPES:
+        for N in (64, 72, 2048, 101):
+            i = norm_inputs(dev, dtype, None, 7, N, N)
+            x, w = i["x"], i["weight"]
+            x[1] = 0
+            x[2, 5], x[3, 5] = float("nan"), float("inf")
+            x[4] = torch.finfo(dtype).smallest_normal
+            x[5] = 100.0
+            y, _ = s.rms_norm(x, w)
+            q, scale, _ = s.rms_norm_fp8(x, w)
+            clean = [0, 6]
+            y0, _ = s.rms_norm(x[clean], w)
+            q0, scale0, _ = s.rms_norm_fp8(x[clean], w)
+            assert torch.equal(y[clean], y0) and torch.equal(scale[clean], scale0)
+            assert torch.equal(q[clean].view(torch.uint8), q0.view(torch.uint8))
+            assert not y[1].any() and float(scale[1]) == 1 and not q[1].float().any()
+            assert bool(y[2].isnan().all()) and bool(scale[2].isnan())                 # the whole row's mean is NaN
+            assert bool(y[3, 5].isnan()) and not y[3, :5].any() and bool(scale[3].isnan())      # inf / inf, finite / inf
+            assert bool(y[4].isfinite().all()) and bool(scale[4].isfinite()) and float(scale[4]) >= 2.0 ** -126
+            assert int(q[5].float().abs().max()) == 448
+    # a row so small that its scale is at its least value, and y = x / sqrt(eps) = 1000 x: 1000 2^-140 / 2^-126 = 0.06104, and
+    # e4m3 has 0.0586 and 0.0625 there
+    x = torch.full((1, 64), 2.0 ** -140, device=dev)
+    w = torch.ones(64, device=dev)
+    q, scale, _ = s.rms_norm_fp8(x, w)
+    assert float(scale[0]) == 2.0 ** -126 and bool((q.float() == 0.0625).all())
+
+
+def test_rms_norm_offsets_beyond_32_bits(dev):
+    s = seq()
+    R, N, far = 40, 64, 1 << 26
+    store = torch.empty((R - 1) * far + N, dtype=torch.bfloat16, device=dev)
+    i = norm_inputs(dev, torch.bfloat16, torch.bfloat16, R, N, 3)
+    x = torch.as_strided(store, (R, N), (far, 1))
+    x.copy_(i["x"])
+    for a, b in zip(s.rms_norm(i["x"], i["weight"], i["residual"], save=True), s.rms_norm(x, i["weight"], i["residual"], save=True)):
+        assert torch.equal(a, b)
+    for a, b in zip(s.rms_norm_backward(i["x"], i["residual"], torch.ones(R, device=dev), i["weight"], i["ds"]),
+                    s.rms_norm_backward(x, i["residual"], torch.ones(R, device=dev), i["weight"], i["ds"])):
+        assert torch.equal(a, b)
+
+
+def test_rms_norm_gradient_matches_differences(dev):
+    s = seq()
+    i = norm_inputs(dev, torch.float32, torch.float32, 40, 100, 8)
+    y, total, rstd = s.rms_norm(i["x"], i["weight"], i["residual"], save=True)
+    dx, dw = s.rms_norm_backward(i["dy"], total, rstd, i["weight"], i["ds"])
+    g = torch.Generator(device=dev).manual_seed(1)
+    vx, vw = torch.randn(40, 100, generator=g, device=dev), torch.randn(100, generator=g, device=dev)
+
+    def value(e):
+        y, total = s.rms_norm(i["x"] + e * vx, i["weight"] + e * vw, i["residual"])
+        return float((y.double() * i["dy"]).sum() + (total.double() * i["ds"]).sum())
+    e = 2.0 ** -8
+    want, got = float((dx.double() * vx).sum() + (dw.double() * vw).sum()), (value(e) - value(-e)) / (2 * e)
+    # 4000 terms of size 4 each off by some 4 U on their own, and the cubic term e^2 of a value of size sqrt(4000) * 3
+    assert abs(got - want) <= math.sqrt(4000) * 4 * 8 * U / (2 * e) + math.sqrt(4000) * 3 * e * e, (got, want)
+
+
+def test_rms_norm_in_graphs(dev):
+    s = seq()
+    for R, N in ((3, 64), (900, 1000), (70, 4099)):
+        i = norm_inputs(dev, torch.bfloat16, torch.float32, R, N, N)
+
+        def train():
+            y, total, rstd = s.rms_norm(i["x"], i["weight"], i["residual"], save=True)
+            return (y, total) + s.rms_norm_backward(i["dy"], total, rstd, i["weight"], i["ds"])
+        replayed(dev, train, list)
+        replayed(dev, lambda: s.rms_norm_fp8(i["x"], i["weight"], i["residual"]),
+                 lambda o: [o[0].view(torch.uint8), o[1], o[2]])
