@@ -515,6 +515,20 @@ int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int R, int N, 
                       long long ldds, void* dx, long long lddx, float* dweight, float* workspace,
                       long long workspace_bytes, void* stream);
 
+/* Distillation from a teacher's top logits, value and gradient in one call: q = softmax(teacher / T) over a row's K slots,
+ * p = softmax(logits / T) over its V columns; loss[r] = coef[r] T^2 sum_k q_k (log q_k - log p[index_k]) and dlogits =
+ * coef[r] T (p - sum_k q_k [column = index_k]) (a column named by several slots gets all of them).  logits and dlogits
+ * (R, V) of `type`, teacher (R, K) of `teacher_type` = type or fp32, index (R, K) int64 or int32, 1 <= K <= 512, row
+ * strides ld* in elements; temperature T in [2^-20, 2^20]; coef (R) fp32 or NULL = 1; loss (R) fp32; dlogits NULL (value only), another buffer, or logits
+ * itself.  A slot is absent if its index is outside [0, V) or its logit is -inf.  A row without a slot, or with coef 0, gives
+ * loss 0 and a gradient of 0 whatever it holds; elsewhere NaN are carried on.  workspace: serl_topk_distill_workspace_bytes,
+ * contents undefined. */
+long long serl_topk_distill_workspace_bytes(int type, int R, int V, int K);
+int serl_topk_distill(int type, int teacher_type, int index64, int R, int V, int K, const void* logits, long long ldl,
+                      const void* teacher, long long ldt, const void* index, long long ldi, float temperature,
+                      const float* coef, float* loss, void* dlogits, long long ldd, float* workspace,
+                      long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -126,13 +126,15 @@ _SIGS = {
     "serl_rms_norm_fwd": [c_i] * 5 + [c_p, c_ll, c_p, c_ll, c_p, c_f, c_p, c_ll, c_i, c_p, c_p, c_ll, c_p, c_p],
     "serl_rms_norm_bwd_workspace_bytes": [c_i, c_i],
     "serl_rms_norm_bwd": [c_i] * 5 + [c_p, c_ll, c_p, c_ll, c_p, c_p, c_p, c_ll, c_p, c_ll, c_p, c_p, c_ll, c_p],
+    "serl_topk_distill_workspace_bytes": [c_i] * 4,
+    "serl_topk_distill": [c_i] * 6 + [c_p, c_ll, c_p, c_ll, c_p, c_ll, c_f, c_p, c_p, c_p, c_ll, c_p, c_ll, c_p],
     "serl_dropout": [c_p, c_i, c_i, c_i, c_u, c_u, c_f, c_i, c_i, c_p],
 }
 _RESTYPE = {"serl_conv2d_wgrad_workspace_bytes": c_ll, "serl_convs_weight_bytes": c_ll,
             "serl_convs_wgrad_noalloc_max_bytes": c_ll, "serl_learner_workspace_bytes": c_ll, "serl_mbv3_param_floats": c_ll,
             "serl_mbv3_workspace_bytes": c_ll, "serl_convs_dgrad_wgrad1_workspace_bytes": c_ll,
             "serl_gated_scan_workspace_bytes": c_ll, "serl_gated_scan_states_floats": c_ll,
-            "serl_rms_norm_bwd_workspace_bytes": c_ll}
+            "serl_rms_norm_bwd_workspace_bytes": c_ll, "serl_topk_distill_workspace_bytes": c_ll}
 
 EXPORTS = tuple(_SIGS) + ("serl_last_error",)
 

@@ -1,0 +1,494 @@
+// Distillation from a teacher's top logits: with q = softmax(teacher / tau) over a row's K slots and
+// p = softmax(logits / tau) over all V columns,
+//   loss_r = c_r tau^2 sum_k q_k (log q_k - log p[i_k]),   dlogits = c_r tau (p - sum_k q_k [column = i_k])
+// value and gradient in one pass, like the other losses (rowops.hip).  No counterpart in the reference (its only discrete
+// head has two outcomes).
+//
+// Bound by memory: one read and one write of (R, V).  A row stays in the registers of one workgroup between the softmax's
+// statistics and the gradient (up to 1024 threads x 20 pieces of 16 bytes: 160 Ki 16-bit columns); the workgroup walks
+// through rows, and each piece's registers are refilled with the next row's as soon as its gradient is stored, so loads and
+// stores overlap.  Few long rows, and rows too long for registers, are cut into pieces of their own workgroups: one launch
+// for the statistics, one that joins them and writes the gradient (it reads the row again, from the caches where they hold it).
+//
+// Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
+// single threads (`head` and `tail`).  The teacher's columns are stored a second time, behind a barrier that all dense
+// stores of the row have passed.
+#include "seqtypes.h"
+
+#define DIST_MAXK 512
+#define DIST_LOG2E 1.44269504088896340736f
+#define DIST_LN2 0.69314718055994530942f
+
+struct DistArgs {
+  const void *logits, *teacher, *index;
+  void* dlogits;
+  long long ldl, ldt, ldi, ldd;
+  const float* coef;
+  float *loss, *part, *taken;         // part: (R, pieces, 2) m and s; taken: (R, K) the student's logits at the slots
+  int R, V, K, teacher_f32, index64, pieces, piece_vecs;
+  float tau;
+};
+
+// all V columns of a row: [0, nh) head, nvec whole pieces of VEC, then the tail
+struct DistRow { int nh, nvec, nt; };
+template <typename T, int VEC>
+__device__ __forceinline__ DistRow dist_row(const void* p, int V) {
+  DistRow r;
+  const int mis = (int)(((uintptr_t)p / sizeof(typename T::bits)) % VEC);
+  r.nh = mis ? VEC - mis : 0;
+  r.nvec = (V - r.nh) / VEC;
+  r.nt = V - r.nh - r.nvec * VEC;
+  return r;
+}
+// the single column that thread t takes besides its pieces, or -1: threads [0, nh) the head, [VEC, VEC + nt) the tail
+template <int VEC>
+__device__ __forceinline__ int dist_extra(const DistRow& r, int t) {
+  if (VEC == 1) return -1;
+  if (t < r.nh) return t;
+  return t >= VEC && t < VEC + r.nt ? r.nh + r.nvec * VEC + t - VEC : -1;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t dist_minus_inf() {
+  return T::code == SERL_F32 ? 0xff800000u : T::code == SERL_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+}
+template <typename T, int VEC> __device__ __forceinline__ void dist_mask(Raw<T, VEC>& r, bool keep) {
+  if constexpr (VEC == 1) {
+    r.w = keep ? r.w : (typename T::bits)dist_minus_inf<T>();
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<T, VEC>::W; ++i) r.w[i] = keep ? r.w[i] : dist_minus_inf<T>();
+  }
+}
+
+// A partial softmax sum is kept as (m, s): m the part's largest x as it is, s = sum of 2^((x - m) k2), k2 = log2(e) / tau.
+// Differences are taken before the scaling, so columns masked with the type's lowest value count as such (a row of nothing
+// else is uniform).  An empty or all -inf part is (-inf, 0); NaN live in s alone.
+__device__ __forceinline__ float dist_ref(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ float dist_exp(float x, float ref, float k2) { return __builtin_amdgcn_exp2f((x - ref) * k2); }
+__device__ __forceinline__ void dist_join(float& m, float& s, float m2, float s2, float k2) {
+  const float n = fmaxf(m, m2), ref = dist_ref(n);
+  s = s * dist_exp(m, ref, k2) + s2 * dist_exp(m2, ref, k2);
+  m = n;
+}
+
+// a row's teacher in LDS: slot columns (-1: absent), weights q and the student's logits there
+struct DistTeacher { int* idx; float *q, *lg; };
+__device__ __forceinline__ DistTeacher dist_tables(float* lds, int K, int buf) {
+  DistTeacher d;
+  d.idx = (int*)lds + (buf * 3) * K;
+  d.q = lds + (buf * 3 + 1) * K;
+  d.lg = lds + (buf * 3 + 2) * K;
+  return d;
+}
+__device__ __forceinline__ long long dist_column(const DistArgs& a, int row, int k) {
+  return a.index64 ? ((const long long*)a.index)[row * a.ldi + k] : (long long)((const int*)a.index)[row * a.ldi + k];
+}
+// By one wave.  A slot is absent if its column is outside [0, V) or its logit is -inf; NaN and +inf are carried on.
+// TAKEN: the student's logits are those that dist_stats_kernel took (the row may be half overwritten by now).
+// Returns whether any slot is there.
+template <typename T, bool TAKEN>
+__device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const DistTeacher& d, int lane) {
+  const typename T::bits* logits = (const typename T::bits*)a.logits + row * a.ldl;
+  const float inv = 1.f / a.tau;
+  float top = -INFINITY;
+  bool any = false;
+#pragma unroll 2
+  for (int k = lane; k < a.K; k += 64) {
+    const long long id = dist_column(a, row, k);
+    const float tv = a.teacher_f32 ? ((const float*)a.teacher)[row * a.ldt + k]
+                                   : sq_val(T(), ((const typename T::bits*)a.teacher)[row * a.ldt + k]);
+    const bool ok = id >= 0 && id < a.V && !(tv == -INFINITY);
+    const float lg = TAKEN ? a.taken[(long long)row * a.K + k] : sq_val(T(), logits[ok ? id : 0]);
+    d.idx[k] = ok ? (int)id : -1;
+    d.q[k] = tv * inv;
+    d.lg[k] = lg;
+    top = ok ? fmaxf(top, tv * inv) : top;
+    any |= ok;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float sum = 0.f;
+  for (int k = lane; k < a.K; k += 64) {
+    const float e = d.idx[k] >= 0 ? expf(d.q[k] - top) : 0.f;
+    d.q[k] = e;
+    sum += e;
+  }
+  sum = sq_wave_sum(sum);
+  const float r = 1.f / sum;
+  for (int k = lane; k < a.K; k += 64) d.q[k] = d.idx[k] >= 0 ? d.q[k] * r : 0.f;
+  return __any(any);
+}
+// loss without c tau^2, by the wave that staged the teacher
+__device__ __forceinline__ float dist_loss(const DistArgs& a, const DistTeacher& d, float m, float sum, int lane) {
+  const float k2 = DIST_LOG2E / a.tau, l2 = log2f(sum);
+  float s = 0.f;
+  for (int k = lane; k < a.K; k += 64) {
+    const float q = d.q[k];
+    s += q == 0.f ? 0.f : q * (logf(q) - ((d.lg[k] - m) * k2 - l2) * DIST_LN2);
+  }
+  return sq_wave_sum(s);
+}
+// the teacher's columns [lo, hi): scale (p - q summed over the slots of the column), slots in order
+template <typename T>
+__device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistTeacher& d, float m, float inv_sum, float scale,
+                                         int lo, int hi, int t, int threads) {
+  typename T::bits* out = (typename T::bits*)a.dlogits + row * a.ldd;
+  const float k2 = DIST_LOG2E / a.tau;
+  for (int k = t; k < a.K; k += threads) {
+    const int id = d.idx[k];
+    if (id < lo || id >= hi) continue;
+    float q = 0.f;
+    for (int j = 0; j < a.K; ++j) q += d.idx[j] == id ? d.q[j] : 0.f;
+    out[id] = sq_bits(T(), scale * (dist_exp(d.lg[k], m, k2) * inv_sum - q));
+  }
+}
+
+// -------------------------------------------------------------------------------------------- rows held in registers
+template <typename T, int VEC, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
+  constexpr int WAVES = THREADS / 64;
+  extern __shared__ float tables[];           // 3 x K x {column, q, logit}: of the last, this and the next row
+  __shared__ float red[2][WAVES][2];
+  __shared__ int alive[3];
+  typedef typename T::bits bits;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const float k2 = DIST_LOG2E / a.tau;
+  Raw<T, VEC> raw[NV];
+  Raw<T, 1> extra;
+  int row = blockIdx.x;
+  const bits* p = (const bits*)a.logits + row * a.ldl;
+  DistRow w = dist_row<T, VEC>(p, a.V);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = i * THREADS + t;
+    raw[i].load(p + w.nh + (long long)(j < w.nvec ? j : 0) * VEC);
+  }
+  extra.load(p + max(0, dist_extra<VEC>(w, t)));
+  if (wave == 0) {
+    const bool any = dist_stage<T, false>(a, row, dist_tables(tables, a.K, 0), lane);
+    if (lane == 0) alive[0] = any;
+  }
+  int buf = 0, tab = 0, last = -1;
+  float last_m = 0.f, last_inv = 0.f, last_scale = 0.f;
+  for (; row < a.R; row += gridDim.x, buf ^= 1) {
+    const int ex = dist_extra<VEC>(w, t);
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      dist_mask<T, VEC>(raw[i], i * THREADS + t < w.nvec);
+      float x[VEC];
+      raw[i].get(x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[v]);
+    }
+    dist_mask<T, 1>(extra, ex >= 0);
+    float xe[1];
+    extra.get(xe);
+    m = fmaxf(m, xe[0]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float wref = dist_ref(m);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float x[VEC];
+      raw[i].get(x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s += dist_exp(x[v], wref, k2);
+    }
+    s += dist_exp(xe[0], wref, k2);
+    s = sq_wave_sum(s);
+    if (lane == 0) { red[buf][wave][0] = m; red[buf][wave][1] = s; }
+    __syncthreads();
+    if (last >= 0) dist_fix<T>(a, last, dist_tables(tables, a.K, tab == 0 ? 2 : tab - 1), last_m, last_inv, last_scale, 0, a.V, t, THREADS);
+    if constexpr (WAVES > 1) {
+      m = red[buf][0][0]; s = red[buf][0][1];
+#pragma unroll
+      for (int q = 1; q < WAVES; ++q) dist_join(m, s, red[buf][q][0], red[buf][q][1], k2);
+    }
+    const float c = a.coef ? a.coef[row] : 1.f;
+    const bool dead = !alive[tab] || c == 0.f;
+    if (wave == 0) {
+      const float l = dist_loss(a, dist_tables(tables, a.K, tab), m, s, lane);
+      if (lane == 0) a.loss[row] = dead ? 0.f : c * a.tau * a.tau * l;
+    }
+    const int next = row + (int)gridDim.x;
+    const bool more = next < a.R;
+    const bits* pn = (const bits*)a.logits + (more ? next : row) * a.ldl;
+    const DistRow wn = dist_row<T, VEC>(pn, a.V);
+    const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
+    bits* out = a.dlogits ? (bits*)a.dlogits + row * a.ldd : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = i * THREADS + t;
+      if (out) {
+        float x[VEC];
+        raw[i].get(x);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
+        Raw<T, VEC> g;
+        g.put(x);
+        if (j < w.nvec) g.store(out + w.nh + (long long)j * VEC);
+      }
+      raw[i].load(pn + wn.nh + (long long)(more && j < wn.nvec ? j : 0) * VEC);      // no next row: one cached line
+    }
+    if (out && ex >= 0) {
+      Raw<T, 1> g;
+      xe[0] = dead ? 0.f : dist_exp(xe[0], m, k2) * mul;
+      g.put(xe);
+      g.store(out + ex);
+    }
+    extra.load(pn + (more ? max(0, dist_extra<VEC>(wn, t)) : 0));
+    last = out && !dead ? row : -1;
+    last_m = m; last_inv = inv; last_scale = scale;
+    tab = tab == 2 ? 0 : tab + 1;
+    if (wave == 0 && more) {
+      const bool any = dist_stage<T, false>(a, next, dist_tables(tables, a.K, tab), lane);
+      if (lane == 0) alive[tab] = any;
+    }
+    w = wn;
+  }
+  __syncthreads();
+  if (last >= 0) dist_fix<T>(a, last, dist_tables(tables, a.K, tab == 0 ? 2 : tab - 1), last_m, last_inv, last_scale, 0, a.V, t, THREADS);
+}
+
+// ------------------------------------------------------------------------------------------------- rows cut in pieces
+#define DIST_CUT 256
+template <typename T, int VEC>
+__global__ __launch_bounds__(DIST_CUT) void dist_stats_kernel(const DistArgs a) {
+  __shared__ float red[4][2];
+  typedef typename T::bits bits;
+  const int t = threadIdx.x, row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+  const bits* p = (const bits*)a.logits + row * a.ldl;
+  const DistRow w = dist_row<T, VEC>(p, a.V);
+  const int j0 = piece * a.piece_vecs, j1 = min(w.nvec, j0 + a.piece_vecs);
+  const float k2 = DIST_LOG2E / a.tau;
+  const int ex = piece == 0 ? dist_extra<VEC>(w, t) : -1;
+  Raw<T, 1> extra;
+  extra.load(p + max(0, ex));
+  dist_mask<T, 1>(extra, ex >= 0);
+  float xe[1];
+  extra.get(xe);
+  float m = fmaxf(xe[0], -INFINITY), s = dist_exp(xe[0], dist_ref(m), k2);
+  constexpr int U = 4;
+  for (int jb = j0; jb < j1; jb += DIST_CUT * U) {
+    Raw<T, VEC> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * DIST_CUT + t;
+      raw[u].load(p + w.nh + (long long)(j < j1 ? j : j1 - 1) * VEC);
+    }
+    float x[U][VEC], n = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      dist_mask<T, VEC>(raw[u], jb + u * DIST_CUT + t < j1);
+      raw[u].get(x[u]);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) n = fmaxf(n, x[u][v]);
+    }
+    n = fmaxf(m, n);
+    const float ref = dist_ref(n);
+    s *= dist_exp(m, ref, k2);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s += dist_exp(x[u][v], ref, k2);
+    m = n;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+    dist_join(m, s, m2, s2, k2);
+  }
+  if ((t & 63) == 0) { red[t >> 6][0] = m; red[t >> 6][1] = s; }
+  __syncthreads();
+  if (t == 0) {
+    for (int q = 1; q < 4; ++q) dist_join(m, s, red[q][0], red[q][1], k2);
+    float* o = a.part + ((long long)row * a.pieces + piece) * 2;
+    o[0] = m; o[1] = s;
+  }
+  if (piece == 0) {         // before any workgroup of the next launch overwrites the row, if it is in place
+    for (int k = t; k < a.K; k += DIST_CUT) {
+      const long long id = dist_column(a, row, k);
+      a.taken[(long long)row * a.K + k] = sq_val(T(), p[id >= 0 && id < a.V ? id : 0]);
+    }
+  }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
+  extern __shared__ float tables[];
+  __shared__ int alive;
+  typedef typename T::bits bits;
+  const int t = threadIdx.x, lane = t & 63, row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+  const bits* p = (const bits*)a.logits + row * a.ldl;
+  const DistRow w = dist_row<T, VEC>(p, a.V);
+  const int j0 = piece * a.piece_vecs, j1 = min(w.nvec, j0 + a.piece_vecs);
+  const float k2 = DIST_LOG2E / a.tau;
+  const DistTeacher d = dist_tables(tables, a.K, 0);
+  // every wave joins the row's statistics; wave 0 takes the teacher
+  float m = -INFINITY, s = 0.f;
+  for (int q = lane; q < a.pieces; q += 64) {
+    const float* o = a.part + ((long long)row * a.pieces + q) * 2;
+    dist_join(m, s, o[0], o[1], k2);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+    dist_join(m, s, m2, s2, k2);
+  }
+  const float c = a.coef ? a.coef[row] : 1.f;
+  if (t < 64) {
+    const bool any = dist_stage<T, true>(a, row, d, lane);
+    if (lane == 0) alive = any;
+    if (piece == 0) {
+      const float l = dist_loss(a, d, m, s, lane);
+      if (lane == 0) a.loss[row] = any && c != 0.f ? c * a.tau * a.tau * l : 0.f;
+    }
+  }
+  __syncthreads();
+  if (!a.dlogits) return;
+  const bool dead = !alive || c == 0.f;
+  const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
+  bits* out = (bits*)a.dlogits + row * a.ldd;
+  constexpr int U = 4;
+  for (int jb = j0; jb < j1; jb += DIST_CUT * U) {
+    Raw<T, VEC> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * DIST_CUT + t;
+      raw[u].load(p + w.nh + (long long)(j < j1 ? j : j1 - 1) * VEC);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = jb + u * DIST_CUT + t;
+      float x[VEC];
+      raw[u].get(x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
+      raw[u].put(x);
+      if (j < j1) raw[u].store(out + w.nh + (long long)j * VEC);
+    }
+  }
+  const int ex = piece == 0 ? dist_extra<VEC>(w, t) : -1;
+  if (ex >= 0) {
+    Raw<T, 1> e;
+    e.load(p + ex);
+    float x[1];
+    e.get(x);
+    x[0] = dead ? 0.f : dist_exp(x[0], m, k2) * mul;
+    e.put(x);
+    e.store(out + ex);
+  }
+  __syncthreads();
+  if (dead) return;
+  dist_fix<T>(a, row, d, m, inv, scale, w.nh + j0 * VEC, w.nh + j1 * VEC, t, DIST_CUT);
+  if (piece == 0) {
+    dist_fix<T>(a, row, d, m, inv, scale, 0, w.nh, t, DIST_CUT);
+    dist_fix<T>(a, row, d, m, inv, scale, w.nh + w.nvec * VEC, a.V, t, DIST_CUT);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+// pieces a row is cut into (1: a workgroup holds whole rows in registers)
+struct DistPlan { int pieces, piece_vecs; };
+static int dist_vec(int type, bool wide) { return !wide ? 1 : type == SERL_F32 ? 4 : 8; }
+static DistPlan dist_plan(int type, int R, int V, bool wide) {
+  const int vec = dist_vec(type, wide), n = cdiv(V, vec);
+  const int most = wide ? 1024 * 20 : 256 * 16;                    // vectors of a row that fit the registers
+  DistPlan p{1, n};
+  int want = 1;
+  if (n > most) want = cdiv(n, 4096);
+  if (R < 128 && n > 1024) {                                       // few rows: share each among enough workgroups
+    const int share = cdiv(512, R < 1 ? 1 : R), fit = cdiv(n, 1024);
+    const int q = share < fit ? share : fit;
+    want = want > q ? want : q;
+  }
+  if (want > 1) {
+    p.piece_vecs = cdiv(n, want);
+    p.pieces = cdiv(n, p.piece_vecs);
+  }
+  return p;
+}
+
+template <typename T, int VEC, int THREADS, int NV>
+static void dist_go(const DistArgs& a, hipStream_t st) {
+  // persistent: as many workgroups as fit the 256 CUs at once
+  const int fit = THREADS == 1024 ? 256 : THREADS == 256 ? 256 * 4 : 256 * 16;
+  hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
+                     3 * 3 * a.K * sizeof(float), st, a);
+}
+template <typename T, int VEC>
+static void dist_launch(const DistArgs& a, hipStream_t st) {
+  if (a.pieces > 1) {
+    const dim3 grid((unsigned)(a.R * a.pieces)), blk(DIST_CUT);
+    hipLaunchKernelGGL((dist_stats_kernel<T, VEC>), grid, blk, 0, st, a);
+    hipLaunchKernelGGL((dist_grad_kernel<T, VEC>), grid, blk, 3 * a.K * sizeof(float), st, a);
+    return;
+  }
+  const int n = cdiv(a.V, VEC);
+  if constexpr (VEC == 1) {
+    if (n <= 256) dist_go<T, 1, 64, 4>(a, st);
+    else dist_go<T, 1, 256, 16>(a, st);
+  } else {
+    if (n <= 64) dist_go<T, VEC, 64, 1>(a, st);
+    else if (n <= 256) dist_go<T, VEC, 64, 4>(a, st);
+    else if (n <= 1024) dist_go<T, VEC, 256, 4>(a, st);
+    else if (n <= 2048) dist_go<T, VEC, 256, 8>(a, st);
+    else if (n <= 4096) dist_go<T, VEC, 1024, 4>(a, st);
+    else if (n <= 8192) dist_go<T, VEC, 1024, 8>(a, st);
+    else if (n <= 16384) dist_go<T, VEC, 1024, 16>(a, st);
+    else dist_go<T, VEC, 1024, 20>(a, st);
+  }
+}
+
+static long long dist_ws(const DistPlan& p, int R, int K) {
+  return p.pieces > 1 ? (long long)R * p.pieces * 8 + (long long)R * K * 4 : 0;
+}
+
+extern "C" long long serl_topk_distill_workspace_bytes(int type, int R, int V, int K) {
+  if (type < 0 || type > 2 || R < 0 || V < 1 || K < 1 || K > DIST_MAXK) {
+    serl_set_error("topk_distill: bad type or sizes");
+    return -1;
+  }
+  const long long a = dist_ws(dist_plan(type, R, V, true), R, K), b = dist_ws(dist_plan(type, R, V, false), R, K);
+  return a > b ? a : b;
+}
+
+extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R, int V, int K, const void* logits,
+                                 long long ldl, const void* teacher, long long ldt, const void* index, long long ldi,
+                                 float temperature, const float* coef, float* loss, void* dlogits, long long ldd,
+                                 float* workspace, long long workspace_bytes, void* stream) {
+  SERL_CHECK_ARG(type >= 0 && type <= 2, "topk_distill: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  SERL_CHECK_ARG(teacher_type == type || teacher_type == SERL_F32, "topk_distill: the teacher's type must be the logits' or fp32");
+  SERL_CHECK_ARG(R >= 0 && V >= 1 && V < 0x7ff00000 && K >= 1 && K <= DIST_MAXK,
+                 "topk_distill: R >= 0, V >= 1 and K in [1, %d]", DIST_MAXK);
+  SERL_CHECK_ARG(temperature >= 0x1p-20f && temperature <= 0x1p20f, "topk_distill: the temperature must be in [2^-20, 2^20]");
+  if (R == 0) return SERL_OK;
+  SERL_CHECK_ARG(logits && teacher && index && loss, "topk_distill: null pointer");
+  SERL_CHECK_ARG(ldl >= 0 && ldt >= 0 && ldi >= 0 && (!dlogits || R <= 1 || ldd >= V),
+                 "topk_distill: negative row stride, or output rows overlap");
+  SERL_CHECK_ARG(!dlogits || dlogits != logits || R <= 1 || ldl == ldd, "topk_distill: in place needs the same row stride");
+  const int es = sq_size(type), vec = dist_vec(type, true);
+  // wide: logits and gradient of a row have the same distance to a 16-byte boundary
+  const bool wide = V >= 2 * vec && sq_aligned(logits, es) &&
+                    (!dlogits || (((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0 && (R <= 1 || (ldl - ldd) % vec == 0)));
+  const DistPlan p = dist_plan(type, R, V, wide);
+  const long long need = dist_ws(p, R, K);
+  SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
+                 "topk_distill: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
+  SERL_CHECK_ARG((long long)R * p.pieces <= 0x7fffffffll, "topk_distill: too many rows");
+  DistArgs a{};
+  a.logits = logits; a.ldl = ldl; a.teacher = teacher; a.ldt = ldt; a.index = index; a.ldi = ldi; a.dlogits = dlogits;
+  a.ldd = ldd; a.coef = coef; a.loss = loss; a.part = workspace;
+  a.taken = workspace ? workspace + (long long)R * p.pieces * 2 : nullptr; a.R = R; a.V = V; a.K = K;
+  a.teacher_f32 = teacher_type == SERL_F32; a.index64 = index64 != 0; a.tau = temperature; a.pieces = p.pieces;
+  a.piece_vecs = p.piece_vecs;
+  hipStream_t st = (hipStream_t)stream;
+#define DIST_GO(T, W) (wide ? dist_launch<T, W>(a, st) : dist_launch<T, 1>(a, st))
+  if (type == SERL_F32) DIST_GO(F32, 4);
+  else if (type == SERL_BF16) DIST_GO(BF16, 8);
+  else DIST_GO(F16, 8);
+#undef DIST_GO
+  SERL_CHECK_LAUNCH("topk_distill");
+  return SERL_OK;
+}

@@ -389,3 +389,13 @@ def rms_norm_bwd(dtype, stream_dtype, weight_dtype, R, N, dy, lddy, sum_, ldsum,
                  workspace, workspace_bytes, stream):
     call("serl_rms_norm_bwd", dtype, stream_dtype, weight_dtype, R, N, dy, lddy, sum_, ldsum, rstd, weight, ds, ldds, dx,
          lddx, dweight, workspace, workspace_bytes, stream)
+
+
+def topk_distill_workspace_bytes(dtype, R, V, K) -> int:
+    return _nbytes(_lib.load().serl_topk_distill_workspace_bytes(dtype, R, V, K), "topk_distill_workspace_bytes")
+
+
+def topk_distill(dtype, teacher_dtype, index64, R, V, K, logits, ldl, teacher, ldt, index, ldi, temperature, coef, loss,
+                 dlogits, ldd, workspace, workspace_bytes, stream):
+    call("serl_topk_distill", dtype, teacher_dtype, int(index64), R, V, K, logits, ldl, teacher, ldt, index, ldi,
+         float(temperature), coef, loss, dlogits, ldd, workspace, workspace_bytes, stream)

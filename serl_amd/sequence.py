@@ -288,3 +288,56 @@ def rms_norm_backward(dy, s, rstd, weight, ds=None):
                          0 if dr is None else dr.stride(0), dx.data_ptr(), N, dw.data_ptr(), _ptr(ws), n,
                          ops.current_stream())
     return dx, dw
+
+
+# ------------------------------------------------------------------------------ distillation from a teacher's top logits
+def topk_distill(logits, teacher, index, temperature=1.0, coef=None, grad=True, out=None):
+    """loss_r = coef_r T^2 KL(q || p), q = softmax(teacher / T) over a row's K slots, p = softmax(logits / T) over its V
+    columns, and its gradient with respect to the logits, coef_r T (p - q), in one pass over them.
+
+    logits: (R, V); teacher: (R, K) logits in logits' type or float32, 1 <= K <= 512; index: (R, K) int64 or int32 columns of
+    them; coef: (R,) float32 weights (None: ones).  A slot is absent if its index is outside [0, V) or its logit -inf; a row
+    without slots, or with coef 0, gives loss 0 and gradient 0 whatever it holds.  A column named twice gets both shares.
+    Returns (loss (R,) float32, dlogits in logits' type), dlogits None with grad=False; out: the tensor for dlogits, which may
+    be logits itself."""
+    if not isinstance(logits, torch.Tensor) or logits.ndim != 2:
+        raise ValueError("logits must be a (R, V) tensor")
+    if logits.dtype not in _CODES:
+        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    R, V = logits.shape
+    if V < 1:
+        raise ValueError("logits must have at least one column")
+    if not isinstance(teacher, torch.Tensor) or teacher.ndim != 2:
+        raise ValueError("teacher must be a (R, K) tensor")
+    K = teacher.shape[1]
+    if not 1 <= K <= 512:
+        raise ValueError(f"teacher: K must be in [1, 512], got {K}")
+    _shape(teacher, "teacher", (R, K))
+    _type(teacher, "teacher", logits.dtype, torch.float32)
+    _shape(index, "index", (R, K))
+    _type(index, "index", torch.int64, torch.int32)
+    if coef is not None:
+        _shape(coef, "coef", (R,))
+        _type(coef, "coef", torch.float32)
+    temperature = float(temperature)
+    if not 2.0 ** -20 <= temperature <= 2.0 ** 20:
+        raise ValueError(f"temperature must be in [2^-20, 2^20], got {temperature}")
+    if out is not None:
+        if not grad:
+            raise ValueError("out is given, but no gradient is asked for")
+        _out(out, "out", (R, V), logits.dtype)
+    with _place(("logits", logits), ("teacher", teacher), ("index", index), ("coef", coef), ("out", out)):
+        logits = _channels(logits)
+        teacher, index = _channels(teacher), _channels(index)
+        if coef is not None:
+            coef = coef.contiguous()
+        dev, code = logits.device, _CODES[logits.dtype]
+        loss = torch.empty((R,), dtype=torch.float32, device=dev)
+        if grad and out is None:
+            out = torch.empty((R, V), dtype=logits.dtype, device=dev)
+        n = ops.topk_distill_workspace_bytes(code, R, V, K)
+        ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
+        ops.topk_distill(code, _CODES[teacher.dtype], index.dtype == torch.int64, R, V, K, logits.data_ptr(), logits.stride(0),
+                         teacher.data_ptr(), teacher.stride(0), index.data_ptr(), index.stride(0), temperature, _ptr(coef),
+                         loss.data_ptr(), _ptr(out), 0 if out is None else out.stride(0), _ptr(ws), n, ops.current_stream())
+    return loss, out

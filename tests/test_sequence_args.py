@@ -122,3 +122,42 @@ def test_rms_norm_refusals():
         ops.rms_norm_bwd(1, 1, 1, 4, 8, 16, 8, 16, 8, 16, 16, None, 0, 16, 8, 16, 16, 127, 0)
     with pytest.raises(ValueError, match="N must be"):
         ops.rms_norm_bwd_workspace_bytes(4, 40000)
+
+
+def test_topk_distill_refusals():
+    x, te, ix = t(4, 9), t(4, 3), t(4, 3, dtype=torch.int64)
+    for err, match, args, kw in (
+            (ValueError, r"logits must be a \(R, V\)", (t(9), te, ix), {}),
+            (TypeError, "logits must be float32", (x.double(), te, ix), {}),
+            (ValueError, "at least one column", (t(4, 0), te, ix), {}),
+            (ValueError, r"teacher must be a \(R, K\)", (x, t(4), ix), {}),
+            (ValueError, r"K must be in \[1, 512\]", (x, t(4, 0), t(4, 0, dtype=torch.int64)), {}),
+            (ValueError, r"K must be in \[1, 512\]", (x, t(4, 513), t(4, 513, dtype=torch.int64)), {}),
+            (ValueError, "teacher must have the shape", (x, t(5, 3), ix), {}),
+            (TypeError, "teacher must be", (x, te.half(), ix), {}),
+            (ValueError, "index must have the shape", (x, te, ix[:, :2]), {}),
+            (TypeError, "index must be", (x, te, te), {}),
+            (ValueError, "coef must have the shape", (x, te, ix), dict(coef=t(3))),
+            (TypeError, "coef must be", (x, te, ix), dict(coef=t(4).half())),
+            (ValueError, "temperature must be in", (x, te, ix), dict(temperature=0)),
+            (ValueError, "temperature must be in", (x, te, ix), dict(temperature=float("nan"))),
+            (ValueError, "temperature must be in", (x, te, ix), dict(temperature=float("inf"))),
+            (ValueError, "no gradient is asked for", (x, te, ix), dict(grad=False, out=x)),
+            (ValueError, "out must have the shape", (x, te, ix), dict(out=t(4, 8))),
+            (TypeError, "out must be", (x, te, ix), dict(out=x.half())),
+            (ValueError, "contiguous channels", (x, te, ix), dict(out=t(9, 4).t())),
+            (TypeError, "logits must be a CUDA tensor", (x, te, ix), {})):
+        with pytest.raises(err, match=match):
+            sequence.topk_distill(*args, **kw)
+    go = lambda **k: ops.topk_distill(*{**dict(  # noqa: E731
+        dtype=1, tt=1, i64=1, R=4, V=9, K=3, logits=16, ldl=9, teacher=16, ldt=3, index=16, ldi=3, tau=1.0, coef=None, loss=16,
+        d=32, ldd=9, ws=None, n=0, st=0), **k}.values())
+    for match, kw in (("type must be", dict(dtype=4)), ("teacher's type", dict(tt=2)), (r"K in \[1, 512\]", dict(K=600)),
+                      ("temperature must be", dict(tau=-1.0)), ("null pointer", dict(index=None)), ("overlap", dict(ldd=8)),
+                      ("negative", dict(ldt=-3)), ("same row stride", dict(d=16, ldd=10)),
+                      (r"workspace of \d+ bytes needed, 0 available", dict(V=300000, ldl=300000, ldd=300000))):
+        with pytest.raises(ValueError, match=match):
+            go(**kw)
+    with pytest.raises(ValueError, match="bad type or sizes"):
+        ops.topk_distill_workspace_bytes(1, 4, 0, 3)
+    assert ops.topk_distill_workspace_bytes(1, 2048, 131072, 128) >= 0

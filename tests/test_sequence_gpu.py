@@ -473,3 +473,247 @@ def test_rms_norm_in_graphs(dev):
         replayed(dev, train, list)
         replayed(dev, lambda: s.rms_norm_fp8(i["x"], i["weight"], i["residual"]),
                  lambda o: [o[0].view(torch.uint8), o[1], o[2]])
+
+
+# -------------------------------------------------------------------------------------------- top-logit distillation
+def distill_inputs(dev, dtype, R, V, K, seed, coef=True, absent=0.1, twice=True, tdtype=None, itype=torch.int64):
+    g = torch.Generator().manual_seed(seed)
+    logits = (torch.randn((R, V), generator=g) * 2.5).to(dtype)
+    index = torch.randint(0, V, (R, K), generator=g)
+    if twice and K > 2:
+        index[:, 1] = index[:, 0]                       # the same column from two slots
+    teacher = (torch.randn((R, K), generator=g) * 2 + 4).to(tdtype or dtype)
+    gone = torch.rand((R, K), generator=g) < absent
+    teacher[gone & (torch.arange(K) % 2 == 0)] = -math.inf
+    far = torch.tensor([-1, V, V + 7, 2 ** 31 - 1, -2 ** 31], dtype=torch.int64)[torch.randint(0, 5, (R, K), generator=g)]
+    index = torch.where(gone & (torch.arange(K) % 2 == 1), far, index)
+    c = torch.rand(R, generator=g) * 2 - 0.5 if coef else None
+    if coef and R > 2:
+        c[1] = 0
+    if R > 3:
+        teacher[2] = -math.inf                          # nothing there
+        index[3] = -1
+    return {k: None if v is None else v.to(dev) for k, v in dict(logits=logits, teacher=teacher, index=index.to(itype), coef=c).items()}
+
+
+def distill_reference(i, tau):
+    x, t, ix = i["logits"].double().cpu() / tau, i["teacher"].double().cpu() / tau, i["index"].cpu().long()
+    R, V = x.shape
+    ok = (ix >= 0) & (ix < V) & (t > -math.inf)
+    c = torch.ones(R, dtype=torch.float64) if i["coef"] is None else i["coef"].double().cpu()
+    live = ok.any(1) & (c != 0)
+    q = torch.softmax(torch.where(ok, t, torch.tensor(-1e300, dtype=torch.float64)), 1) * ok
+    logp = torch.log_softmax(x, 1)
+    lp = logp.gather(1, ix.clamp(0, V - 1))
+    each = torch.where(q > 0, q * (torch.log(q.clamp_min(1e-320)) - lp), torch.zeros_like(q))
+    d = torch.exp(logp).scatter_add(1, ix.clamp(0, V - 1), -q)
+    zero = torch.zeros((), dtype=torch.float64)
+    loss = torch.where(live, c * tau * tau * each.sum(1), zero)
+    return loss, torch.where(live[:, None], (c * tau)[:, None] * d, zero), q, lp, c
+
+
+def check_distill(i, dtype, tau):
+    s = seq()
+    loss, d = s.topk_distill(i["logits"], i["teacher"], i["index"], temperature=tau, coef=i["coef"])
+    loss2, none = s.topk_distill(i["logits"], i["teacher"], i["index"], temperature=tau, coef=i["coef"], grad=False)
+    assert none is None and torch.equal(loss, loss2) and d.dtype == dtype and loss.dtype == torch.float32
+    rl, rd, q, lp, c = distill_reference(i, tau)
+    V, span = i["logits"].shape[1], float((i["logits"].double().max() - i["logits"].double().min()) / tau)
+    # an exponent (x - m) k2 of at most `span` nats has three roundings (the difference, k2, the product); the sum's terms 8
+    # columns a step and at most 80 steps a thread, the joins 10 more; exp2, the reciprocal and two products 1 ulp each
+    rel = (3 * span + 8 + 90 + 10) * U
+    p = (rd / (c * tau)[:, None].where((c != 0)[:, None], torch.ones(1, dtype=torch.float64))).abs()
+    qcol = torch.zeros_like(rd).scatter_add(1, i["index"].cpu().long().clamp(0, V - 1), q)
+    tol = (c.abs() * tau)[:, None] * (rel * (p + 2 * qcol) + 1e-37) + HALF[dtype] * rd.abs() + (SMALL if dtype == torch.float16 else 2.0 ** -134)
+    within(d, rd, tol, "dlogits")
+    tspan = float(i["teacher"].double().abs().nan_to_num(posinf=0).max()) / tau
+    # log q and log p of a size up to span + log V, each with the roundings above, weights q with those of K <= 512 slots
+    size = span + tspan + math.log(V) + 7
+    within(loss, rl, c.abs() * tau * tau * (rel + (3 * tspan + 30) * U + 6 * U) * size * (q.sum(1) + 1e-30), "loss")
+    inplace = i["logits"].clone()
+    loss3, d3 = s.topk_distill(inplace, i["teacher"], i["index"], temperature=tau, coef=i["coef"], out=inplace)
+    assert d3 is inplace and torch.equal(loss3, loss) and torch.equal(d3, d)
+
+
+DISTILL_SIZES = [(1, 1, 1), (5, 3, 2), (4, 17, 5), (6, 64, 64), (300, 256, 8), (3, 257, 9), (7, 1000, 33), (2, 2048, 512), (5, 4099, 100),
+                 (2, 8192, 16), (130, 8200, 16), (2, 16387, 100), (131, 20001, 20), (2, 32768, 3), (129, 40003, 50), (1, 65536, 64), (3, 131072, 128),
+                 (130, 131075, 40), (2, 163840, 30), (129, 163841, 7), (2, 200003, 77)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("R,V,K", DISTILL_SIZES)
+def test_topk_distill_matches_its_formulas(dev, dtype, R, V, K):
+    tau = (1.0, 0.5, 2.0, 3.7)[(R + V + K) % 4]
+    check_distill(distill_inputs(dev, dtype, R, V, K, V + K, tdtype=(None, torch.float32)[V % 2],
+                                 itype=(torch.int64, torch.int32)[K % 2], coef=V % 3 > 0), dtype, tau)
+
+
+def test_topk_distill_views_and_misaligned_rows(dev):
+    """Row strides and offsets of every distance to a 16-byte boundary, in and out at different ones, expanded teachers."""
+    s = seq()
+    for dtype in (torch.float32, torch.bfloat16):
+        for V in (40, 1001, 3000, 70001):
+            i = distill_inputs(dev, dtype, 6, V, 12, V)
+            want = s.topk_distill(i["logits"], i["teacher"], i["index"], 1.5, i["coef"])
+            rl, rd, q, lp, c = distill_reference(i, 1.5)
+            for off, pad, ooff, opad in ((1, 0, 1, 0), (3, 5, 3, 5), (0, 1, 2, 3), (7, 8, 0, 0)):
+                big = torch.full((6, off + V + pad), float("nan"), dtype=dtype, device=dev)
+                x = big[:, off:off + V]
+                x.copy_(i["logits"])
+                buf = torch.full((6, ooff + V + opad), 7.0, dtype=dtype, device=dev)
+                out = buf[:, ooff:ooff + V]
+                loss, d = s.topk_distill(x, i["teacher"], i["index"], 1.5, i["coef"], out=out)
+                # twice the tolerance of one result: both are within it of the formulas'
+                within(loss, want[0], 1e-4 * (1 + want[0].double().abs().cpu()), "loss")
+                within(d, want[1], 2e-5 + 2 * HALF[dtype] * want[1].double().abs().cpu(), "dlogits")
+                assert bool((buf[:, :ooff] == 7).all()) and bool((buf[:, ooff + V:] == 7).all())
+                assert bool(x.isfinite().all())
+    i = distill_inputs(dev, torch.float32, 5, 300, 6, 1, absent=0)
+    one = s.topk_distill(i["logits"][:1], i["teacher"][:1], i["index"][:1])
+    more = s.topk_distill(i["logits"][:1].expand(5, 300), i["teacher"][:1].expand(5, 6), i["index"][:1].expand(5, 6))
+    assert torch.equal(more[0], one[0].expand(5)) and torch.equal(more[1], one[1].expand(5, 300))
+    t = s.topk_distill(i["logits"].t().contiguous().t(), i["teacher"], i["index"])
+    assert torch.equal(t[1], s.topk_distill(i["logits"], i["teacher"], i["index"])[1])
+
+
+@pytest.mark.parametrize("R,V", [(8, 64), (8, 1500), (8, 9001), (200, 9001), (8, 70000), (200, 70000)])
+def test_topk_distill_masks_infinities_and_nan(dev, R, V):
+    s = seq()
+    for dtype in DTYPES:
+        i = distill_inputs(dev, dtype, R, V, 6, V, coef=False, absent=0, twice=False)
+        x, t, ix = i["logits"], i["teacher"], i["index"]
+        t[2] = 1.0
+        for r in range(R):
+            ix[r] = torch.tensor([0, 3, 5, 9, V - 1, V // 2], device=dev)
+        base = s.topk_distill(x, t, ix)
+        coef = torch.ones(R, device=dev)
+        coef[0], t[1], ix[4] = 0, -math.inf, V                   # three ways to be left out
+        x[0], x[1] = float("nan"), float("inf")
+        x[4] = -math.inf
+        low = torch.finfo(dtype).min
+        x[3, :] = low                                            # nothing but the mask: uniform
+        x[5, 20:] = low                                          # masked columns, some the teacher's
+        x[6, 20:] = -math.inf
+        t[6, 4:] = -math.inf
+        x[7, 11] = float("nan")
+        loss, d = s.topk_distill(x, t, ix, coef=coef)
+        for r in (0, 1, 4):
+            assert float(loss[r]) == 0 and not d[r].any()
+        for r in [2] + list(range(8, R)):
+            assert torch.equal(loss[r], base[0][r]) and torch.equal(d[r], base[1][r])
+        cols = torch.ones(V, dtype=torch.bool, device=dev)
+        cols[ix[3]] = False
+        within(d[3][cols], torch.full((int(cols.sum()),), 1 / V), (HALF[dtype] + 200 * U) / V + SMALL, "uniform")
+        assert not d[5, 20:V // 2].any() and not d[6, 20:].any()
+        # the teacher's two masked columns cost q |low| each (log p = low - log of the sum), the others a few nats
+        masked = float(torch.softmax(t[5].double(), 0)[4:].sum())
+        assert float(loss[5]) >= 0.99 * masked * -low - 100 and bool(loss[6].isfinite()) and bool(d[5].isfinite().all())
+        assert bool(loss[7].isnan()) and bool(d[7].isnan().all())
+        xi = x.clone()
+        loss2, d2 = s.topk_distill(xi, t, ix, coef=coef, out=xi)
+        assert torch.equal(loss2.nan_to_num(5), loss.nan_to_num(5)) and torch.equal(d2.nan_to_num(5), d.nan_to_num(5))
+        # a student that rules the teacher's column out: the loss is infinite, the gradient -q there
+        x[2, 9] = -math.inf
+        loss, d = s.topk_distill(x[2:3], t[2:3], ix[2:3])
+        assert float(loss) == math.inf and abs(float(d[0, 9]) + 1 / 6) <= HALF[dtype] / 6 + 1e-6
+        t[2, 0] = float("nan")
+        loss, d = s.topk_distill(x[2:3], t[2:3], ix[2:3])
+        assert bool(loss.isnan().all()) and bool(d[0, ix[2]].isnan().all())
+
+
+def test_topk_distill_gradient_matches_differences(dev):
+    s = seq()
+    for V in (50, 3000, 40000):
+        i = distill_inputs(dev, torch.float32, 8, V, 16, V)
+        loss, d = s.topk_distill(i["logits"], i["teacher"], i["index"], 2.0, i["coef"])
+        v = torch.randn(8, V, generator=torch.Generator(device=dev).manual_seed(1), device=dev)
+
+        def value(e):
+            return float(s.topk_distill(i["logits"] + e * v, i["teacher"], i["index"], 2.0, i["coef"], grad=False)[0].double().sum())
+        e = 2.0 ** -6
+        want, got = float((d.double() * v).sum()), (value(e) - value(-e)) / (2 * e)
+        # 8 rows of losses up to 2 * 4 * 20, off by some 100 U each, and the cubic term of tau^2 log-sum-exp: e^2 |v|^3 / tau
+        assert abs(got - want) <= 8 * 160 * 100 * U / (2 * e) + 8 * 2 * e * e * 8, (V, got, want)
+
+
+def test_topk_distill_no_rows_and_offsets_beyond_32_bits(dev):
+    s = seq()
+    e = torch.empty((0, 50), device=dev)
+    loss, d = s.topk_distill(e, e[:, :4], e[:, :4].long())
+    assert loss.shape == (0,) and d.shape == (0, 50)
+    far = 1 << 26
+    for V in (100, 12000):
+        i = distill_inputs(dev, torch.bfloat16, 40, V, 6, 2)
+        store = torch.empty(39 * far + V, dtype=torch.bfloat16, device=dev)
+        x = torch.as_strided(store, (40, V), (far, 1))
+        x.copy_(i["logits"])
+        want = s.topk_distill(i["logits"], i["teacher"], i["index"], 1.0, i["coef"])
+        loss, d = s.topk_distill(x, i["teacher"], i["index"], 1.0, i["coef"])
+        # rows at another distance to a 16-byte boundary are summed in another order: each result is within half a step of the
+        # formulas' and what 32 bits lose (as in check_distill, below 2^-15 of p <= 1 and of the loss for these spans)
+        for again in range(2):
+            within(loss, want[0], 2.0 ** -14 * (1 + want[0].double().abs().cpu()), "loss")
+            within(d, want[1], 2.0 ** -14 + 2 * HALF[torch.bfloat16] * want[1].double().abs().cpu(), "dlogits")
+            if not again:
+                loss, d = s.topk_distill(x, i["teacher"], i["index"], 1.0, i["coef"], out=x)
+                assert d is x
+
+
+def test_topk_distill_in_graphs(dev):
+    s = seq()
+    for R, V in ((64, 256), (3, 50000), (300, 5001)):
+        i = distill_inputs(dev, torch.bfloat16, R, V, 10, V)
+        replayed(dev, lambda: s.topk_distill(i["logits"], i["teacher"], i["index"], 1.0, i["coef"]), list)
+
+
+# --------------------------------------------------------------------------------------------------- used together
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_a_recurrent_policy_learns_a_step_from_its_teacher(dev, dtype):
+    """norm -> projection -> recurrence -> norm of the residual stream -> logits -> distillation loss, and all the way back,
+    against the same network by autograd in 64 bits; and the trained direction lowers the loss."""
+    s = seq()
+    B, T, D, V, K = 3, 70, 32, 40, 5
+    g = torch.Generator().manual_seed(0)
+    r = lambda *sh, sc=1.0: (torch.randn(sh, generator=g) * sc).to(dtype).to(dev)  # noqa: E731
+    x, w1, w2 = r(B, T, D), 1 + r(D, sc=0.2), 1 + r(D, sc=0.2)
+    proj, head = r(D, 2 * D, sc=D ** -0.5), r(D, V, sc=D ** -0.5)
+    teacher, index = r(B * T, K, sc=2.0), torch.randint(0, V, (B * T, K), generator=g).to(dev)
+    starts = (torch.rand((B, T), generator=g) < 0.1).to(dev)
+    coef = torch.full((B * T,), 1.0 / (B * T), device=dev)
+
+    def forward(x):
+        n1, s1, r1 = s.rms_norm(x, w1, save=True)
+        both = n1 @ proj
+        gate, cand = both[..., :D], both[..., D:]
+        y, h, saved = s.gated_scan(gate, cand, starts=starts, save=True)
+        n2, s2, r2 = s.rms_norm(y, w2, residual=x, save=True)
+        logits = (n2 @ head).view(B * T, V)
+        return locals()
+    f = forward(x)
+    loss, dlogits = s.topk_distill(f["logits"], teacher, index, 1.5, coef)
+    dn2 = (dlogits @ head.t()).view(B, T, D)
+    ds2, dw2 = s.rms_norm_backward(dn2, f["s2"], f["r2"], w2)
+    dboth = torch.empty_like(f["both"])
+    s.gated_scan_backward(f["gate"], f["cand"], f["saved"], ds2, starts=starts, out=(dboth[..., :D], dboth[..., D:]))
+    dx, dw1 = s.rms_norm_backward(dboth @ proj.t(), f["s1"], f["r1"], w1, ds=ds2)
+
+    X, W1, W2, P, H = (t.double().cpu().requires_grad_() for t in (x, w1, w2, proj, head))
+    n1 = X / torch.sqrt((X * X).mean(-1, keepdim=True) + 1e-6) * W1
+    both = n1 @ P
+    h, ys = torch.zeros((B, D), dtype=torch.float64), []
+    for t in range(T):
+        h = torch.where(starts[:, t, None].cpu(), torch.zeros_like(h), h)
+        fg = torch.sigmoid(both[:, t, :D])
+        h = fg * h + (1 - fg) * both[:, t, D:]
+        ys.append(h)
+    s2 = X + torch.stack(ys, 1)
+    logits = ((s2 / torch.sqrt((s2 * s2).mean(-1, keepdim=True) + 1e-6) * W2) @ H).view(B * T, V)
+    q = torch.softmax(teacher.double().cpu() / 1.5, 1)
+    lp = torch.log_softmax(logits / 1.5, 1).gather(1, index.cpu())
+    total = (1.5 ** 2 * (q * (torch.log(q) - lp)).sum(1)).mean()
+    gx, gw1, gw2 = torch.autograd.grad(total, (X, W1, W2))
+    # seven stored tensors each way, a relative error of half a step each, and fp32's sums: 40 half steps of the largest gradient
+    tol = 40 * max(HALF[dtype], 16 * U)
+    for got, want in ((dx, gx), (dw1, gw1), (dw2, gw2)):
+        within(got, want, tol * want.abs().max(), "gradient")
+    assert abs(float(loss.sum()) - float(total)) <= tol * float(total)
