@@ -48,6 +48,39 @@ __device__ __forceinline__ int dist_extra(const DistRow& r, int t) {
   return t >= VEC && t < VEC + r.nt ? r.nh + r.nvec * VEC + t - VEC : -1;
 }
 
+// The three passes over a row each unpack its registers anew: without this the compiler keeps the 32-bit values of the first
+// pass for the others, twice the registers, and spills.
+template <typename T, int VEC> __device__ __forceinline__ void dist_again(Raw<T, VEC>& r) {
+  if constexpr (VEC > 1) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, VEC>::W; ++i) asm volatile("" : "+v"(r.w[i]));
+  }
+}
+
+// larger of three, without the canonicalising moves that fmaxf takes for values that come from memory; a NaN may or may not be
+// passed over (it is in the sum then)
+__device__ __forceinline__ float dist_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int VEC> __device__ __forceinline__ float dist_max(float m, const float (&x)[VEC]) {
+  if constexpr (VEC == 1) return dist_max3(m, x[0], x[0]);
+#pragma unroll
+  for (int v = 0; v + 1 < VEC; v += 2) m = dist_max3(m, x[v], x[v + 1]);
+  return m;
+}
+
+// piece j of a row's whole pieces (`base`: the first one): a uniform address and a 32-bit offset per thread
+template <typename T, int VEC>
+__device__ __forceinline__ void dist_load(Raw<T, VEC>& r, const typename T::bits* base, int j) {
+  r.load((const typename T::bits*)((const char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void dist_store(const Raw<T, VEC>& r, typename T::bits* base, int j) {
+  r.store((typename T::bits*)((char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
+}
+
 template <typename T> __device__ __forceinline__ uint32_t dist_minus_inf() {
   return T::code == SERL_F32 ? 0xff800000u : T::code == SERL_BF16 ? 0xff80ff80u : 0xfc00fc00u;
 }
@@ -71,6 +104,8 @@ __device__ __forceinline__ void dist_join(float& m, float& s, float m2, float s2
   m = n;
 }
 
+__device__ __forceinline__ float dist_uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
 // a row's teacher in LDS: slot columns (-1: absent), weights q and the student's logits there
 struct DistTeacher { int* idx; float *q, *lg; };
 __device__ __forceinline__ DistTeacher dist_tables(float* lds, int K, int buf) {
@@ -92,7 +127,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
   const float inv = 1.f / a.tau;
   float top = -INFINITY;
   bool any = false;
-#pragma unroll 2
+#pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
     const long long id = dist_column(a, row, k);
     const float tv = a.teacher_f32 ? ((const float*)a.teacher)[row * a.ldt + k]
@@ -108,6 +143,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   float sum = 0.f;
+#pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
     const float e = d.idx[k] >= 0 ? expf(d.q[k] - top) : 0.f;
     d.q[k] = e;
@@ -122,6 +158,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
 __device__ __forceinline__ float dist_loss(const DistArgs& a, const DistTeacher& d, float m, float sum, int lane) {
   const float k2 = DIST_LOG2E / a.tau, l2 = log2f(sum);
   float s = 0.f;
+#pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
     const float q = d.q[k];
     s += q == 0.f ? 0.f : q * (logf(q) - ((d.lg[k] - m) * k2 - l2) * DIST_LN2);
@@ -134,6 +171,7 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
                                          int lo, int hi, int t, int threads) {
   typename T::bits* out = (typename T::bits*)a.dlogits + row * a.ldd;
   const float k2 = DIST_LOG2E / a.tau;
+#pragma unroll 1
   for (int k = t; k < a.K; k += threads) {
     const int id = d.idx[k];
     if (id < lo || id >= hi) continue;
@@ -161,7 +199,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = i * THREADS + t;
-    raw[i].load(p + w.nh + (long long)(j < w.nvec ? j : 0) * VEC);
+    dist_load(raw[i], p + w.nh, j < w.nvec ? j : 0);
   }
   extra.load(p + max(0, dist_extra<VEC>(w, t)));
   if (wave == 0) {
@@ -173,13 +211,14 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
   for (; row < a.R; row += gridDim.x, buf ^= 1) {
     const int ex = dist_extra<VEC>(w, t);
     float m = -INFINITY, s = 0.f;
+    int tm = t;          // the pieces' numbers are computed where they are used, not kept over the loop in registers
+    asm volatile("" : "+v"(tm));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      dist_mask<T, VEC>(raw[i], i * THREADS + t < w.nvec);
+      dist_mask<T, VEC>(raw[i], i * THREADS + tm < w.nvec);
       float x[VEC];
       raw[i].get(x);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[v]);
+      m = dist_max<VEC>(m, x);
     }
     dist_mask<T, 1>(extra, ex >= 0);
     float xe[1];
@@ -191,6 +230,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float x[VEC];
+      dist_again(raw[i]);
       raw[i].get(x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) s += dist_exp(x[v], wref, k2);
@@ -200,11 +240,16 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     if (lane == 0) { red[buf][wave][0] = m; red[buf][wave][1] = s; }
     __syncthreads();
     if (last >= 0) dist_fix<T>(a, last, dist_tables(tables, a.K, tab == 0 ? 2 : tab - 1), last_m, last_inv, last_scale, 0, a.V, t, THREADS);
-    if constexpr (WAVES > 1) {
-      m = red[buf][0][0]; s = red[buf][0][1];
+    if constexpr (WAVES > 1) {              // lane 0's join for everybody: the order of the parts, and so the bits, are its own
+      m = red[buf][lane & (WAVES - 1)][0]; s = red[buf][lane & (WAVES - 1)][1];
 #pragma unroll
-      for (int q = 1; q < WAVES; ++q) dist_join(m, s, red[buf][q][0], red[buf][q][1], k2);
+      for (int o = 1; o < WAVES; o <<= 1) {
+        const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
+        dist_join(m, s, m2, s2, k2);
+      }
     }
+    m = dist_uniform(m);
+    s = dist_uniform(s);
     const float c = a.coef ? a.coef[row] : 1.f;
     const bool dead = !alive[tab] || c == 0.f;
     if (wave == 0) {
@@ -215,21 +260,24 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     const bool more = next < a.R;
     const bits* pn = (const bits*)a.logits + (more ? next : row) * a.ldl;
     const DistRow wn = dist_row<T, VEC>(pn, a.V);
+    const int nn = more ? wn.nvec : 0;
     const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
     bits* out = a.dlogits ? (bits*)a.dlogits + row * a.ldd : nullptr;
+    asm volatile("" : "+v"(tm));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = i * THREADS + t;
+      const int j = i * THREADS + tm;
       if (out) {
         float x[VEC];
+        dist_again(raw[i]);
         raw[i].get(x);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
         Raw<T, VEC> g;
         g.put(x);
-        if (j < w.nvec) g.store(out + w.nh + (long long)j * VEC);
+        if (j < w.nvec) dist_store(g, out + w.nh, j);
       }
-      raw[i].load(pn + wn.nh + (long long)(more && j < wn.nvec ? j : 0) * VEC);      // no next row: one cached line
+      dist_load(raw[i], pn + wn.nh, j < nn ? j : 0);      // no next row (nn = 0): one cached line
     }
     if (out && ex >= 0) {
       Raw<T, 1> g;
@@ -275,15 +323,14 @@ __global__ __launch_bounds__(DIST_CUT) void dist_stats_kernel(const DistArgs a) 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = jb + u * DIST_CUT + t;
-      raw[u].load(p + w.nh + (long long)(j < j1 ? j : j1 - 1) * VEC);
+      dist_load(raw[u], p + w.nh, j < j1 ? j : j1 - 1);
     }
     float x[U][VEC], n = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       dist_mask<T, VEC>(raw[u], jb + u * DIST_CUT + t < j1);
       raw[u].get(x[u]);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) n = fmaxf(n, x[u][v]);
+      n = dist_max<VEC>(n, x[u]);
     }
     n = fmaxf(m, n);
     const float ref = dist_ref(n);
@@ -356,7 +403,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = jb + u * DIST_CUT + t;
-      raw[u].load(p + w.nh + (long long)(j < j1 ? j : j1 - 1) * VEC);
+      dist_load(raw[u], p + w.nh, j < j1 ? j : j1 - 1);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -366,7 +413,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
       raw[u].put(x);
-      if (j < j1) raw[u].store(out + w.nh + (long long)j * VEC);
+      if (j < j1) dist_store(raw[u], out + w.nh, j);
     }
   }
   const int ex = piece == 0 ? dist_extra<VEC>(w, t) : -1;
@@ -460,8 +507,8 @@ extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R,
                                  float* workspace, long long workspace_bytes, void* stream) {
   SERL_CHECK_ARG(type >= 0 && type <= 2, "topk_distill: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   SERL_CHECK_ARG(teacher_type == type || teacher_type == SERL_F32, "topk_distill: the teacher's type must be the logits' or fp32");
-  SERL_CHECK_ARG(R >= 0 && V >= 1 && V < 0x7ff00000 && K >= 1 && K <= DIST_MAXK,
-                 "topk_distill: R >= 0, V >= 1 and K in [1, %d]", DIST_MAXK);
+  SERL_CHECK_ARG(R >= 0 && V >= 1 && V <= 0x3fffffff && K >= 1 && K <= DIST_MAXK,
+                 "topk_distill: R >= 0, V in [1, 2^30) and K in [1, %d]", DIST_MAXK);
   SERL_CHECK_ARG(temperature >= 0x1p-20f && temperature <= 0x1p20f, "topk_distill: the temperature must be in [2^-20, 2^20]");
   if (R == 0) return SERL_OK;
   SERL_CHECK_ARG(logits && teacher && index && loss, "topk_distill: null pointer");
