@@ -48,15 +48,6 @@ __device__ __forceinline__ int dist_extra(const DistRow& r, int t) {
   return t >= VEC && t < VEC + r.nt ? r.nh + r.nvec * VEC + t - VEC : -1;
 }
 
-// The three passes over a row each unpack its registers anew: without this the compiler keeps the 32-bit values of the first
-// pass for the others, twice the registers, and spills.
-template <typename T, int VEC> __device__ __forceinline__ void dist_again(Raw<T, VEC>& r) {
-  if constexpr (VEC > 1) {
-#pragma unroll
-    for (int i = 0; i < Raw<T, VEC>::W; ++i) asm volatile("" : "+v"(r.w[i]));
-  }
-}
-
 // larger of three, without the canonicalising moves that fmaxf takes for values that come from memory; a NaN may or may not be
 // passed over (it is in the sum then)
 __device__ __forceinline__ float dist_max3(float a, float b, float c) {
@@ -230,7 +221,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float x[VEC];
-      dist_again(raw[i]);
+      sq_again(raw[i]);
       raw[i].get(x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) s += dist_exp(x[v], wref, k2);
@@ -269,7 +260,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
       const int j = i * THREADS + tm;
       if (out) {
         float x[VEC];
-        dist_again(raw[i]);
+        sq_again(raw[i]);
         raw[i].get(x);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;

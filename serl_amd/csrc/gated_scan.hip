@@ -13,7 +13,7 @@
 #include "seqtypes.h"
 
 #define SCAN_CKPT 128       // steps between the states that the forward pass keeps for the backward pass
-#define SCAN_THREADS 256
+#define SCAN_THREADS 256    // of the kernel for a few steps
 #define SCAN_MAXSEG 32      // most pieces the time axis is split into
 
 struct ScanArgs {
@@ -30,20 +30,21 @@ struct ScanArgs {
   int B, T, D, ndb, nseg, seg_len;                           // channel blocks; pieces of the time axis and their length
 };
 
-// f and 1 - f, both to within 2 ulp: the smaller one is computed, the larger is one minus it (a memory of n steps needs
-// 1 - f = 1/n to its full relative precision, and f's rounding unbiased).
+// f and 1 - f, both to within 2 ulp of themselves: a memory of n steps needs 1 - f = 1/n to its full relative precision, and
+// f's rounding unbiased, so the one above a half is one minus the other.  z = +inf: f = 1, 1 - f = 0 exactly.
 __device__ __forceinline__ void scan_gate(float z, float& f, float& rest) {
-  const float u = __expf(-fabsf(z));
-  const float r = __builtin_amdgcn_rcpf(1.f + u);
-  const float small = u * r, big = fmaf(-u, r, 1.f);
-  f = z >= 0.f ? big : small;
-  rest = z >= 0.f ? small : big;
-  if (z != z) f = rest = z;
+  const float e = __expf(z);
+  rest = __builtin_amdgcn_rcpf(1.f + e);
+  f = z > 0.f ? 1.f - rest : e * rest;
 }
 
-// k c + b where k = 0 cuts whatever c is: an infinity or NaN of one episode ends with it
-__device__ __forceinline__ float scan_apply(float k, float c, float b) { return k == 0.f ? b : fmaf(k, c, b); }
-__device__ __forceinline__ float scan_times(float k, float kp) { return k == 0.f || kp == 0.f ? 0.f : k * kp; }
+// k c + b where k = 0 cuts whatever c is (0 * NaN = 0 in the legacy product): an infinity or NaN of one episode ends with it
+__device__ __forceinline__ float scan_times(float k, float c) {
+  float r;
+  asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(k), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float scan_apply(float k, float c, float b) { return scan_times(k, c) + b; }
 
 __device__ __forceinline__ int scan_len(const ScanArgs& a, int b) {
   if (!a.lengths) return a.T;
@@ -51,33 +52,30 @@ __device__ __forceinline__ int scan_len(const ScanArgs& a, int b) {
   return n < 0 ? 0 : (n > a.T ? a.T : n);
 }
 
-// state in front of piece `seg`: the maps of the pieces before it applied to h0
-template <int VEC>
-__device__ __forceinline__ void scan_join_fwd(const ScanArgs& a, int b, int seg, int d0, float (&c)[VEC]) {
-  const float* p = a.seg + ((long long)b * a.nseg * 2) * a.D + d0;
+// state in front of piece `seg` for channel ch: the maps of the pieces before it applied to h0
+__device__ __forceinline__ float scan_join_fwd(const ScanArgs& a, int b, int seg, int ch, float c) {
+  const float* p = a.seg + ((long long)b * a.nseg * 2) * a.D + ch;
 #pragma unroll 4
-  for (int s = 0; s < seg; ++s, p += 2 * (long long)a.D) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) c[v] = scan_apply(p[v], c[v], p[a.D + v]);
-  }
+  for (int s = 0; s < seg; ++s, p += 2 * (long long)a.D) c = scan_apply(p[0], c, p[a.D]);
+  return c;
 }
 // the same from the end: the gradient that leaves piece seg + 1 towards piece `seg`
-template <int VEC>
-__device__ __forceinline__ void scan_join_bwd(const ScanArgs& a, int b, int seg, int d0, float (&c)[VEC]) {
-  const float* p = a.seg + ((long long)b * a.nseg + a.nseg - 1) * 2 * a.D + d0;
+__device__ __forceinline__ float scan_join_bwd(const ScanArgs& a, int b, int seg, int ch, float c) {
+  const float* p = a.seg + ((long long)b * a.nseg + a.nseg - 1) * 2 * a.D + ch;
 #pragma unroll 4
-  for (int s = a.nseg - 1; s > seg; --s, p -= 2 * (long long)a.D) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) c[v] = scan_apply(p[v], c[v], p[a.D + v]);
-  }
+  for (int s = a.nseg - 1; s > seg; --s, p -= 2 * (long long)a.D) c = scan_apply(p[0], c, p[a.D]);
+  return c;
 }
 
 // Joins the maps (k, b) of the threads of one channel in the order of time (REV: against it).  In: the thread's own map.
-// Out: `in` = the state that reaches the thread's steps when `carry` enters the tile; carry = the state that leaves it.
-// Lanes of a wave are (64 / CG) time chunks of CG channel groups; waves follow each other in time.
-template <int VEC, int CG, bool REV>
-__device__ __forceinline__ void scan_join_tile(float (&k)[VEC], float (&b)[VEC], float (&carry)[VEC], float (&in)[VEC],
+// Out: `in` = the state that reaches the thread's steps when the tile is entered with `carry`; carry = the state that leaves
+// it, all = the product of k so far.  Lanes of a wave are (64 / CG) time chunks of CG channel groups; waves follow each other
+// in time.  Between waves every wave walks the maps of all of them, one channel per lane (`carry` and `all` are kept so).
+template <int VEC, int CG, int WAVES, bool REV>
+__device__ __forceinline__ void scan_join_tile(float (&k)[VEC], float (&b)[VEC], float& carry, float& all, float (&in)[VEC],
                                                float* lds, int wave, int lane) {
+  constexpr int CH = VEC * CG;
+  static_assert(CH <= 64, "a lane per channel");
 #pragma unroll
   for (int o = CG; o < 64; o <<= 1) {
     const bool has = REV ? lane + o < 64 : lane >= o;
@@ -85,143 +83,219 @@ __device__ __forceinline__ void scan_join_tile(float (&k)[VEC], float (&b)[VEC],
     for (int v = 0; v < VEC; ++v) {
       const float kp = REV ? __shfl_down(k[v], o) : __shfl_up(k[v], o);
       const float bp = REV ? __shfl_down(b[v], o) : __shfl_up(b[v], o);
-      b[v] = has ? scan_apply(k[v], bp, b[v]) : b[v];
-      k[v] = has ? scan_times(k[v], kp) : k[v];
+      const float bj = scan_apply(k[v], bp, b[v]), kj = scan_times(k[v], kp);      // unconditional: no branch per lane
+      b[v] = has ? bj : b[v];
+      k[v] = has ? kj : k[v];
     }
   }
-  const int cg = lane & (CG - 1);
+  const int c0 = (lane & (CG - 1)) * VEC;
   if (REV ? lane < CG : lane >= 64 - CG) {        // the whole wave's map
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      lds[((wave * 2) * VEC + v) * CG + cg] = k[v];
-      lds[((wave * 2 + 1) * VEC + v) * CG + cg] = b[v];
+      lds[wave * 2 * CH + c0 + v] = k[v];
+      lds[(wave * 2 + 1) * CH + c0 + v] = b[v];
     }
   }
   __syncthreads();
+  float own = carry;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    const int w = REV ? WAVES - 1 - i : i;
+    const float kw = lds[w * 2 * CH + (lane & (CH - 1))], bw = lds[(w * 2 + 1) * CH + (lane & (CH - 1))];
+    own = w == wave ? carry : own;
+    carry = scan_apply(kw, carry, bw);
+    all = scan_times(kw, all);
+  }
   const bool first = REV ? lane + CG >= 64 : lane < CG;
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    float ke = REV ? __shfl_down(k[v], CG & 63) : __shfl_up(k[v], CG & 63);
-    float be = REV ? __shfl_down(b[v], CG & 63) : __shfl_up(b[v], CG & 63);
-    if (first) { ke = 1.f; be = 0.f; }
-    float c = carry[v], mine = c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int w = REV ? 3 - i : i;
-      mine = w == wave ? c : mine;
-      c = scan_apply(lds[((w * 2) * VEC + v) * CG + cg], c, lds[((w * 2 + 1) * VEC + v) * CG + cg]);
+    in[v] = VEC == 1 && CG == 64 ? own : __shfl(own, c0 + v);
+    if (CG < 64) {
+      const float ke = REV ? __shfl_down(k[v], CG & 63) : __shfl_up(k[v], CG & 63);
+      const float be = REV ? __shfl_down(b[v], CG & 63) : __shfl_up(b[v], CG & 63);
+      const float j = scan_apply(ke, in[v], be);
+      in[v] = first ? in[v] : j;
     }
-    carry[v] = c;
-    in[v] = scan_apply(ke, mine, be);
   }
+}
+
+// What a thread of the tile kernels is: VEC channels from d0 on, L steps of every tile; a wave's steps are 64 / CG * L rows.
+template <int VEC, int CG, int L>
+struct ScanSpot {
+  static constexpr int ROWS = 64 / CG * L;
+  int wave, lane, first, d0, seg, b, tb, te, len;      // first: the thread's first step within its wave's
+  int ch;                                              // the one channel of the lane (states, maps of pieces), in range
+  bool dok, chok;                                      // chok: wave 0 writes channel ch
+  __device__ __forceinline__ explicit ScanSpot(const ScanArgs& a) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    first = lane / CG * L;
+    const int db = blockIdx.x % a.ndb, q = blockIdx.x / a.ndb, want = (db * CG + lane % CG) * VEC;
+    seg = q % a.nseg;
+    b = q / a.nseg;
+    dok = want < a.D;
+    d0 = dok ? want : 0;
+    const int cw = db * CG * VEC + lane % (CG * VEC);
+    ch = min(cw, a.D - 1);
+    chok = wave == 0 && lane < CG * VEC && cw < a.D;
+    tb = seg * a.seg_len;
+    te = min(a.T, tb + a.seg_len);
+    len = min(te, scan_len(a, b));
+  }
+};
+
+// One (B, T, D) tensor as a wave sees it: `base` is its sequence (uniform), `off` the thread's byte offset from its wave's
+// first row, or behind everything for channels that do not exist.
+template <typename T, int VEC, int L, typename Spot>
+struct ScanRows {
+  const char* base;
+  long long ts;          // bytes from step to step
+  uint32_t off;
+  __device__ __forceinline__ ScanRows(const Spot& me, const void* p, long long bs, long long step) {
+    constexpr int E = sizeof(typename T::bits);
+    base = (const char*)p + me.b * bs * E;
+    ts = step * E;
+    off = me.dok ? (uint32_t)(me.first * ts) + (uint32_t)(me.d0 * E) : SQ_NOWHERE;
+  }
+  // the wave's rows from step t on, as far as they are before `te` (a row is D wide)
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int t, int te, int D) const {
+    const int rows = min(te - t, Spot::ROWS);
+    return sq_buffer(base + t * ts, rows > 0 ? (rows - 1) * (int)ts + D * (int)sizeof(typename T::bits) : 0);
+  }
+  __device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[L], int t, int te, int D) const {
+    const __amdgpu_buffer_rsrc_t b = at(t, te, D);
+#pragma unroll
+    for (int l = 0; l < L; ++l) sq_load(r[l], b, off + l * (uint32_t)ts);
+  }
+};
+
+// The starts of a thread's steps, one byte per lane: every thread of a time chunk loads one, scan_cuts collects them.
+template <int CG, int L>
+__device__ __forceinline__ unsigned char scan_start(const unsigned char* starts, int t, int te, int lane) {
+  static_assert(L <= CG, "a chunk's starts fit its lanes");
+  return starts ? starts[min(t + (lane & (CG - 1) & (L - 1)), te - 1)] : 0;
+}
+template <int CG, int L>
+__device__ __forceinline__ unsigned scan_cuts(unsigned char start, int t, int len, int lane) {
+  const unsigned long long all = __ballot(start != 0);
+  const unsigned bits = (unsigned)(all >> (lane & ~(CG - 1))) & (L == 32 ? ~0u : (1u << (L & 31)) - 1u);
+  const int live = len - t;            // steps at and behind the length start nothing
+  return live >= L ? bits : live <= 0 ? 0u : bits & ((1u << live) - 1u);
+}
+// v = value where a step starts an episode (its k is 0, but k v + b would carry on a NaN of v)
+// (the empty asm keeps the compiler from running these rare blocks always, as selects)
+template <int VEC> __device__ __forceinline__ void scan_cut(float (&v)[VEC], bool cut, float value) {
+  asm volatile("");
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = cut ? value : v[i];
+}
+template <int VEC> __device__ __forceinline__ void scan_cut(float (&v)[VEC], bool cut, const float (&value)[VEC]) {
+  asm volatile("");
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = cut ? value[i] : v[i];
+}
+// value `keep ? r : fill` of every element (fill: the bits of a pair of 16-bit or of one 32-bit element)
+template <typename T, int VEC>
+__device__ __forceinline__ void scan_mask(Raw<T, VEC>& r, bool keep, uint32_t fill) {
+  asm volatile("");
+  if constexpr (VEC == 1) {
+    r.w = keep ? r.w : (typename T::bits)fill;
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<T, VEC>::W; ++i) r.w[i] = keep ? r.w[i] : fill;
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t scan_inf() {       // a gate of +inf: f = 1, the state is held
+  return T::code == SERL_F32 ? 0x7f800000u : T::code == SERL_BF16 ? 0x7f807f80u : 0x7c007c00u;
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
 // SUMMARY: write the piece's map instead of the outputs (first of two launches when the time axis is split).
-template <typename T, int VEC, int CG, int L, bool SUMMARY>
-__global__ __launch_bounds__(SCAN_THREADS, 2) void scan_fwd_kernel(const ScanArgs a) {
-  constexpr int TC = SCAN_THREADS / CG, TILE = TC * L;
+template <typename T, int VEC, int CG, int L, int THREADS, bool SUMMARY>
+__global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
+  constexpr int TC = THREADS / CG, TILE = TC * L, WAVES = THREADS / 64;
   static_assert(SCAN_CKPT % L == 0, "kept states lie between the chunks of two threads");
-  __shared__ float lds[2][4 * 2 * VEC * CG];
-  typedef typename T::bits bits;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, cg = tid % CG, tc = tid / CG;
-  const int db = blockIdx.x % a.ndb, q = blockIdx.x / a.ndb, seg = q % a.nseg, b = q / a.nseg;
-  const int dwant = (db * CG + cg) * VEC;
-  const bool dok = dwant < a.D;
-  const int d0 = dok ? dwant : 0;
-  const int tb = seg * a.seg_len, te = min(a.T, tb + a.seg_len), len = min(te, scan_len(a, b));
-  const bits* gate = (const bits*)a.gate + b * a.gate_bs + d0;
-  const bits* x = (const bits*)a.x + b * a.x_bs + d0;
-  const unsigned char* starts = a.starts ? a.starts + b * a.starts_bs : nullptr;
+  __shared__ __attribute__((aligned(16))) float lds[2][WAVES * 2 * VEC * CG];
+  typedef ScanSpot<VEC, CG, L> Spot;
+  const Spot me(a);
+  typedef ScanRows<T, VEC, L, Spot> Rows;
+  const Rows gate(me, a.gate, a.gate_bs, a.gate_ts), x(me, a.x, a.x_bs, a.x_ts), y(me, a.y, a.y_bs, a.y_ts);
+  const unsigned char* starts = a.starts ? a.starts + me.b * a.starts_bs : nullptr;
 
-  float carry[VEC], all[VEC];        // all: product of the piece's k (SUMMARY)
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    carry[v] = !SUMMARY && a.h0 ? a.h0[(long long)b * a.D + d0 + v] : 0.f;
-    all[v] = 1.f;
-  }
-  if (!SUMMARY && a.nseg > 1) scan_join_fwd<VEC>(a, b, seg, d0, carry);
+  const long long state = (long long)me.b * a.D + me.ch;
+  float all = 1.f, carry = !SUMMARY && a.h0 ? a.h0[state] : 0.f;      // all: product of the piece's k (SUMMARY)
+  if (!SUMMARY && a.nseg > 1) carry = scan_join_fwd(a, me.b, me.seg, me.ch, carry);
 
   Raw<T, VEC> rg[L], rx[L];
-  unsigned char rs[L];
-  const auto fetch = [&](int t0) {
+  int tw = me.tb + me.wave * me.ROWS, buf = 0;          // the wave's first step of the tile
+  gate.fetch(rg, tw, me.te, a.D);
+  x.fetch(rx, tw, me.te, a.D);
+  unsigned char rs = scan_start<CG, L>(starts, tw + me.first, me.te, me.lane);
+  for (int t0 = me.tb; t0 < me.te; t0 += TILE, tw += TILE, buf ^= 1) {
+    const int t = tw + me.first;
+    const bool whole = t0 + TILE <= me.len;               // every step is before the sequence's length
+    const unsigned cut = scan_cuts<CG, L>(rs, t, me.len, me.lane);
+    const bool cuts = __any(cut != 0);                    // rare: an episode starts in the wave's steps
+    float k[L][VEC], add[L][VEC], kk[VEC], bb[VEC], c[VEC];
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-      const int t = min(t0 + tc * L + l, te - 1);       // rows behind the piece: its last one again, not used
-      rg[l].load(gate + t * a.gate_ts);
-      rx[l].load(x + t * a.x_ts);
-      rs[l] = starts ? starts[t] : 0;
-    }
-  };
-  fetch(tb);
-  int buf = 0;
-  for (int t0 = tb; t0 < te; t0 += TILE, buf ^= 1) {
-    float k[L][VEC], add[L][VEC];
-    const int tt = t0 + tc * L;
-    unsigned cut = 0;                    // bit l: an episode starts at the step
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
+      if (!whole) {
+        scan_mask(rg[l], t + l < me.len, scan_inf<T>());
+        scan_mask(rx[l], t + l < me.len, 0);
+      }
       float g[VEC], xv[VEC];
       rg[l].get(g);
       rx[l].get(xv);
-      const bool live = tt + l < len;
-      cut |= live && rs[l] ? 1u << l : 0u;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        float f, rest;
-        scan_gate(g[v], f, rest);
-        k[l][v] = live ? f : 1.f;
-        add[l][v] = live ? rest * xv[v] : 0.f;
+        float rest;
+        scan_gate(g[v], k[l][v], rest);
+        add[l][v] = rest * xv[v];
       }
+      if (cuts) scan_cut<VEC>(k[l], cut >> l & 1, 0.f);
     }
-    if (t0 + TILE < te) fetch(t0 + TILE);
-    float kk[VEC], bb[VEC], c[VEC];
+    gate.fetch(rg, tw + TILE, me.te, a.D);
+    x.fetch(rx, tw + TILE, me.te, a.D);
+    rs = scan_start<CG, L>(starts, t + TILE, me.te, me.lane);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { kk[v] = 1.f; bb[v] = 0.f; }
+    for (int v = 0; v < VEC; ++v) { kk[v] = k[0][v]; bb[v] = add[0][v]; }
 #pragma unroll
-    for (int l = 0; l < L; ++l)
+    for (int l = 1; l < L; ++l) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        bb[v] = cut >> l & 1 ? add[l][v] : fmaf(k[l][v], bb[v], add[l][v]);
+        bb[v] = fmaf(k[l][v], bb[v], add[l][v]);
         kk[v] *= k[l][v];
       }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) kk[v] = cut ? 0.f : kk[v];
-    scan_join_tile<VEC, CG, false>(kk, bb, carry, c, lds[buf], wave, lane);
-    if constexpr (SUMMARY) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) all[v] = scan_times(lds[buf][((w * 2) * VEC + v) * CG + cg], all[v]);
-    } else {
-      if (a.ckpt && dok && tt < te && tt % SCAN_CKPT == 0) {
-        float* p = a.ckpt + ((long long)b * ((a.T + SCAN_CKPT - 1) / SCAN_CKPT) + tt / SCAN_CKPT) * a.D + d0;
+      if (cuts) scan_cut<VEC>(bb, cut >> l & 1, add[l]);
+    }
+    if (cuts) scan_cut<VEC>(kk, cut != 0, 0.f);
+    scan_join_tile<VEC, CG, WAVES, false>(kk, bb, carry, all, c, lds[buf], me.wave, me.lane);
+    if constexpr (!SUMMARY) {
+      if (a.ckpt && me.dok && t < me.te && t % SCAN_CKPT == 0) {
+        float* p = a.ckpt + ((long long)me.b * ((a.T + SCAN_CKPT - 1) / SCAN_CKPT) + t / SCAN_CKPT) * a.D + me.d0;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) p[v] = c[v];
       }
-      bits* y = (bits*)a.y + b * a.y_bs + d0;
+      const __amdgpu_buffer_rsrc_t out = y.at(tw, me.te, a.D);
 #pragma unroll
       for (int l = 0; l < L; ++l) {
-        float o[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          c[v] = cut >> l & 1 ? add[l][v] : fmaf(k[l][v], c[v], add[l][v]);
-          o[v] = tt + l < len ? c[v] : 0.f;
-        }
+        for (int v = 0; v < VEC; ++v) c[v] = fmaf(k[l][v], c[v], add[l][v]);
+        if (cuts) scan_cut<VEC>(c, cut >> l & 1, add[l]);
         Raw<T, VEC> r;
-        r.put(o);
-        if (dok && tt + l < te) r.store(y + (tt + l) * a.y_ts);
+        r.put(c);
+        if (!whole) scan_mask(r, t + l < me.len, 0);
+        sq_store(r, out, y.off + l * (uint32_t)y.ts);
       }
     }
   }
-  if (tc == 0 && dok) {
+  if (me.chok) {
     if constexpr (SUMMARY) {
-      float* p = a.seg + ((long long)b * a.nseg + seg) * 2 * a.D + d0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) { p[v] = all[v]; p[a.D + v] = carry[v]; }
-    } else if (te == a.T) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) a.h_last[(long long)b * a.D + d0 + v] = carry[v];
+      float* p = a.seg + ((long long)me.b * a.nseg + me.seg) * 2 * a.D + me.ch;
+      p[0] = all;
+      p[a.D] = carry;
+    } else if (me.te == a.T) {
+      a.h_last[state] = carry;
     }
   }
 }
@@ -230,199 +304,186 @@ __global__ __launch_bounds__(SCAN_THREADS, 2) void scan_fwd_kernel(const ScanArg
 // With C_t = k_t G_t the gradient that leaves step t backwards in time: G_t = dy_t + C_{t+1}, C_t = k_t (dy_t + C_{t+1}),
 // C_T = dh_last, dh0 = C_0; dx = G (1 - f), dgate = G (k_t/f_t h_{t-1} - x) f (1 - f).  h is recomputed from the state that
 // the forward pass kept at the tile's first step (in 32 bits, where y was rounded), so y is not read.
-template <typename T, int VEC, int CG, int L>
-__global__ __launch_bounds__(SCAN_THREADS, 2) void scan_bwd_kernel(const ScanArgs a) {
-  constexpr int TC = SCAN_THREADS / CG, TILE = TC * L;
-  static_assert(TILE == SCAN_CKPT, "one kept state per tile");
-  __shared__ float lds[2][2][4 * 2 * VEC * CG];
-  typedef typename T::bits bits;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, cg = tid % CG, tc = tid / CG;
-  const int db = blockIdx.x % a.ndb, q = blockIdx.x / a.ndb, seg = q % a.nseg, b = q / a.nseg;
-  const int dwant = (db * CG + cg) * VEC;
-  const bool dok = dwant < a.D;
-  const int d0 = dok ? dwant : 0;
-  const int tb = seg * a.seg_len, te = min(a.T, tb + a.seg_len), len = min(te, scan_len(a, b));
-  const bits* gate = (const bits*)a.gate + b * a.gate_bs + d0;
-  const bits* x = (const bits*)a.x + b * a.x_bs + d0;
-  const bits* dy = (const bits*)a.dy + b * a.dy_bs + d0;
-  const unsigned char* starts = a.starts ? a.starts + b * a.starts_bs : nullptr;
-  const float* ckpt = a.ckpt + (long long)b * ((a.T + SCAN_CKPT - 1) / SCAN_CKPT) * a.D + d0;
-
-  float carry[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) carry[v] = a.dh_last ? a.dh_last[(long long)b * a.D + d0 + v] : 0.f;
-  if (a.nseg > 1) scan_join_bwd<VEC>(a, b, seg, d0, carry);
+template <typename T, int VEC, int CG, int L, int THREADS>
+__global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
+  constexpr int TC = THREADS / CG, TILE = TC * L, WAVES = THREADS / 64;
+  __shared__ __attribute__((aligned(16))) float lds[2][2][WAVES * 2 * VEC * CG];
+  typedef ScanSpot<VEC, CG, L> Spot;
+  const Spot me(a);
+  typedef ScanRows<T, VEC, L, Spot> Rows;
+  const Rows gate(me, a.gate, a.gate_bs, a.gate_ts), x(me, a.x, a.x_bs, a.x_ts), dy(me, a.dy, a.dy_bs, a.dy_ts);
+  const Rows dgate(me, a.dgate, a.dgate_bs, a.dgate_ts), dx(me, a.dx, a.dx_bs, a.dx_ts);
+  const unsigned char* starts = a.starts ? a.starts + me.b * a.starts_bs : nullptr;
+  const float* ckpt = a.ckpt + (long long)me.b * ((a.T + SCAN_CKPT - 1) / SCAN_CKPT) * a.D + me.ch;
+  const long long state = (long long)me.b * a.D + me.ch;
+  const int last = me.tb + (me.te - 1 - me.tb) / TILE * TILE;
+  float carry = a.dh_last ? a.dh_last[state] : 0.f, kept = ckpt[(long long)(last / SCAN_CKPT) * a.D], all = 1.f;
+  if (a.nseg > 1) carry = scan_join_bwd(a, me.b, me.seg, me.ch, carry);
 
   Raw<T, VEC> rg[L], rx[L], rd[L];
-  unsigned char rs[L];
-  float kept[VEC];
-  const auto fetch = [&](int t0) {
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      const int t = min(t0 + tc * L + l, te - 1);
-      rg[l].load(gate + t * a.gate_ts);
-      rx[l].load(x + t * a.x_ts);
-      rd[l].load(dy + t * a.dy_ts);
-      rs[l] = starts ? starts[t] : 0;
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) kept[v] = ckpt[(long long)(t0 / SCAN_CKPT) * a.D + v];
-  };
-  const int last = tb + (te - 1 - tb) / TILE * TILE;
-  fetch(last);
-  int buf = 0;
-  for (int t0 = last; t0 >= tb; t0 -= TILE, buf ^= 1) {
-    float k[L][VEC], rest[L][VEC], w[L][VEC], d[L][VEC];
-    const int tt = t0 + tc * L;
-    float kk[VEC], hh[VEC], cc[VEC], h[VEC];
+  int tw = last + me.wave * me.ROWS, buf = 0;
+  gate.fetch(rg, tw, me.te, a.D);
+  x.fetch(rx, tw, me.te, a.D);
+  dy.fetch(rd, tw, me.te, a.D);
+  unsigned char rs = scan_start<CG, L>(starts, tw + me.first, me.te, me.lane);
+  for (int t0 = last; t0 >= me.tb; t0 -= TILE, tw -= TILE, buf ^= 1) {
+    const int t = tw + me.first;
+    const bool whole = t0 + TILE <= me.len;
+    const unsigned cut = scan_cuts<CG, L>(rs, t, me.len, me.lane);
+    const bool cuts = __any(cut != 0);
+    float k[L][VEC], rest[L][VEC], w[L][VEC];
+    Raw<T, VEC> rc[L];                   // dy as it lies in memory: half the registers
 #pragma unroll
     for (int l = 0; l < L; ++l) {        // w: x for now
+      if (!whole) {
+        scan_mask(rg[l], t + l < me.len, scan_inf<T>());
+        scan_mask(rx[l], t + l < me.len, 0);
+        scan_mask(rd[l], t + l < me.len, 0);
+      }
       float g[VEC];
       rg[l].get(g);
       rx[l].get(w[l]);
-      rd[l].get(d[l]);
-      const bool live = tt + l < len;
+      rc[l] = rd[l];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) scan_gate(g[v], k[l][v], rest[l][v]);
+      if (cuts) scan_cut<VEC>(k[l], cut >> l & 1, 0.f);
+    }
+    float h = kept;
+    {                                    // the tile before (none: nothing is read)
+      const int before = t0 - TILE >= me.tb ? me.te : 0, tp = max(tw - TILE, 0);
+      gate.fetch(rg, tp, before, a.D);
+      x.fetch(rx, tp, before, a.D);
+      dy.fetch(rd, tp, before, a.D);
+      rs = scan_start<CG, L>(starts, max(t - TILE, 0), me.te, me.lane);
+      kept = ckpt[(long long)(max(t0 - TILE, 0) / SCAN_CKPT) * a.D];
+    }
+    // the chunk's maps in both directions
+    float kk[VEC], k2[VEC], hh[VEC], cc[VEC], hin[VEC], cin[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { kk[v] = k[0][v]; hh[v] = rest[0][v] * w[0][v]; cc[v] = 0.f; }
+#pragma unroll
+    for (int l = 1; l < L; ++l) {
+      float add[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        float f, r;
-        scan_gate(g[v], f, r);
-        k[l][v] = live ? f : 1.f;
-        rest[l][v] = live ? r : 0.f;
-        w[l][v] = live ? w[l][v] : 0.f;
-        d[l][v] = live ? d[l][v] : 0.f;
-      }
-    }
-    unsigned cut = 0;                    // bit l: an episode starts at the step (and the step is live)
-#pragma unroll
-    for (int l = 0; l < L; ++l) cut |= (rs[l] && tt + l < len) ? 1u << l : 0u;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      kk[v] = 1.f; hh[v] = 0.f; cc[v] = 0.f; h[v] = kept[v];
-    }
-    if (t0 - TILE >= tb) fetch(t0 - TILE);
-#pragma unroll
-    for (int l = 0; l < L; ++l)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float add = rest[l][v] * w[l][v];
-        hh[v] = cut >> l & 1 ? add : fmaf(k[l][v], hh[v], add);
+        add[v] = rest[l][v] * w[l][v];
+        hh[v] = fmaf(k[l][v], hh[v], add[v]);
         kk[v] *= k[l][v];
       }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) kk[v] = cut ? 0.f : kk[v];
-#pragma unroll
-    for (int l = L - 1; l >= 0; --l)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) cc[v] = cut >> l & 1 ? 0.f : k[l][v] * (d[l][v] + cc[v]);
-    float hin[VEC], cin[VEC], k2[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) k2[v] = kk[v];
-    scan_join_tile<VEC, CG, false>(kk, hh, h, hin, lds[buf][0], wave, lane);
-    scan_join_tile<VEC, CG, true>(k2, cc, carry, cin, lds[buf][1], wave, lane);
-    // forwards: h_{t-1} of every step, folded at once into w = (h_{t-1} - x) f (1 - f)
-#pragma unroll
-    for (int l = 0; l < L; ++l)
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float hp = cut >> l & 1 ? 0.f : hin[v], xv = w[l][v], r = rest[l][v], f = k[l][v];
-        w[l][v] = (hp - xv) * (f * r);
-        hin[v] = fmaf(f, hp, r * xv);
-      }
-    // backwards
-    bits* dgate = (bits*)a.dgate + b * a.dgate_bs + d0;
-    bits* dx = (bits*)a.dx + b * a.dx_bs + d0;
+      if (cuts) scan_cut<VEC>(hh, cut >> l & 1, add);
+    }
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-      float og[VEC], ox[VEC];
+      float d[VEC];
+      rc[l].get(d);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) cc[v] = k[l][v] * (d[v] + cc[v]);
+      if (cuts) scan_cut<VEC>(cc, cut >> l & 1, 0.f);
+    }
+    if (cuts) scan_cut<VEC>(kk, cut != 0, 0.f);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) k2[v] = kk[v];
+    scan_join_tile<VEC, CG, WAVES, false>(kk, hh, h, all, hin, lds[buf][0], me.wave, me.lane);
+    scan_join_tile<VEC, CG, WAVES, true>(k2, cc, carry, all, cin, lds[buf][1], me.wave, me.lane);
+    // forwards: h_{t-1} of every step, folded at once into w = (h_{t-1} - x) f (1 - f); where an episode starts h_{t-1} is 0
+    // and f, which k no longer holds, is 1 - rest
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      float add[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        const float G = d[l][v] + cin[v];
-        og[v] = tt + l < len ? G * w[l][v] : 0.f;
-        ox[v] = tt + l < len ? G * rest[l][v] : 0.f;
-        cin[v] = cut >> l & 1 ? 0.f : k[l][v] * G;
+        const float xv = w[l][v];
+        add[v] = rest[l][v] * xv;
+        w[l][v] = (hin[v] - xv) * (k[l][v] * rest[l][v]);
+        hin[v] = fmaf(k[l][v], hin[v], add[v]);
       }
-      Raw<T, VEC> r;
-      if (dok && tt + l < te) {
-        r.put(og);
-        r.store(dgate + (tt + l) * a.dgate_ts);
-        r.put(ox);
-        r.store(dx + (tt + l) * a.dx_ts);
+      if (cuts) {
+        asm volatile("");
+        float old[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) old[v] = -add[v] * (1.f - rest[l][v]);
+        scan_cut<VEC>(w[l], cut >> l & 1, old);
+        scan_cut<VEC>(hin, cut >> l & 1, add);
       }
     }
-  }
-  if (seg == 0 && tc == 0 && dok) {
+    // backwards
+    const __amdgpu_buffer_rsrc_t og = dgate.at(tw, me.te, a.D), ox = dx.at(tw, me.te, a.D);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) a.dh0[(long long)b * a.D + d0 + v] = carry[v];
+    for (int l = L - 1; l >= 0; --l) {
+      float d[VEC], g[VEC];
+      sq_again(rc[l]);
+      rc[l].get(d);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float G = d[v] + cin[v];
+        g[v] = G * w[l][v];
+        d[v] = G * rest[l][v];
+        cin[v] = k[l][v] * G;
+      }
+      if (cuts) scan_cut<VEC>(cin, cut >> l & 1, 0.f);
+      Raw<T, VEC> r1, r2;
+      r1.put(g);
+      r2.put(d);
+      if (!whole) {
+        scan_mask(r1, t + l < me.len, 0);
+        scan_mask(r2, t + l < me.len, 0);
+      }
+      sq_store(r1, og, dgate.off + l * (uint32_t)dgate.ts);
+      sq_store(r2, ox, dx.off + l * (uint32_t)dx.ts);
+    }
   }
+  if (me.seg == 0 && me.chok) a.dh0[state] = carry;
 }
 
 // The map of a piece for the backward direction: C entering from the right -> C leaving to the left (reads gate and dy).
-template <typename T, int VEC, int CG, int L>
-__global__ __launch_bounds__(SCAN_THREADS, 2) void scan_bwd_summary_kernel(const ScanArgs a) {
-  constexpr int TC = SCAN_THREADS / CG, TILE = TC * L;
-  __shared__ float lds[2][4 * 2 * VEC * CG];
-  typedef typename T::bits bits;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, cg = tid % CG, tc = tid / CG;
-  const int db = blockIdx.x % a.ndb, q = blockIdx.x / a.ndb, seg = q % a.nseg, b = q / a.nseg;
-  const int dwant = (db * CG + cg) * VEC;
-  const bool dok = dwant < a.D;
-  const int d0 = dok ? dwant : 0;
-  const int tb = seg * a.seg_len, te = min(a.T, tb + a.seg_len), len = min(te, scan_len(a, b));
-  const bits* gate = (const bits*)a.gate + b * a.gate_bs + d0;
-  const bits* dy = (const bits*)a.dy + b * a.dy_bs + d0;
-  const unsigned char* starts = a.starts ? a.starts + b * a.starts_bs : nullptr;
-  float carry[VEC], all[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) { carry[v] = 0.f; all[v] = 1.f; }
+template <typename T, int VEC, int CG, int L, int THREADS>
+__global__ __launch_bounds__(THREADS) void scan_bwd_summary_kernel(const ScanArgs a) {
+  constexpr int TC = THREADS / CG, TILE = TC * L, WAVES = THREADS / 64;
+  __shared__ __attribute__((aligned(16))) float lds[2][WAVES * 2 * VEC * CG];
+  typedef ScanSpot<VEC, CG, L> Spot;
+  const Spot me(a);
+  typedef ScanRows<T, VEC, L, Spot> Rows;
+  const Rows gate(me, a.gate, a.gate_bs, a.gate_ts), dy(me, a.dy, a.dy_bs, a.dy_ts);
+  const unsigned char* starts = a.starts ? a.starts + me.b * a.starts_bs : nullptr;
+  float carry = 0.f, all = 1.f;
   Raw<T, VEC> rg[L], rd[L];
-  unsigned char rs[L];
-  const auto fetch = [&](int t0) {
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      const int t = min(t0 + tc * L + l, te - 1);
-      rg[l].load(gate + t * a.gate_ts);
-      rd[l].load(dy + t * a.dy_ts);
-      rs[l] = starts ? starts[t] : 0;
-    }
-  };
-  const int last = tb + (te - 1 - tb) / TILE * TILE;
-  fetch(last);
-  int buf = 0;
-  for (int t0 = last; t0 >= tb; t0 -= TILE, buf ^= 1) {
-    const int tt = t0 + tc * L;
+  const int last = me.tb + (me.te - 1 - me.tb) / TILE * TILE;
+  int tw = last + me.wave * me.ROWS, buf = 0;
+  gate.fetch(rg, tw, me.te, a.D);
+  dy.fetch(rd, tw, me.te, a.D);
+  unsigned char rs = scan_start<CG, L>(starts, tw + me.first, me.te, me.lane);
+  for (int t0 = last; t0 >= me.tb; t0 -= TILE, tw -= TILE, buf ^= 1) {
+    const int t = tw + me.first;
     float kk[VEC], cc[VEC], in[VEC];
-    bool cuts = false;
+    const unsigned cut = scan_cuts<CG, L>(rs, t, me.len, me.lane);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { kk[v] = 1.f; cc[v] = 0.f; }
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
+      scan_mask(rg[l], t + l < me.len, scan_inf<T>());
+      scan_mask(rd[l], t + l < me.len, 0);
       float g[VEC], d[VEC];
       rg[l].get(g);
       rd[l].get(d);
-      const bool live = tt + l < len, cut = live && rs[l];
-      cuts |= cut;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         float f, r;
         scan_gate(g[v], f, r);
-        f = live ? f : 1.f;
-        cc[v] = cut ? 0.f : f * ((live ? d[v] : 0.f) + cc[v]);
-        kk[v] *= f;
+        f = cut >> l & 1 ? 0.f : f;
+        cc[v] = scan_times(f, d[v] + cc[v]);
+        kk[v] = scan_times(kk[v], f);
       }
     }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) kk[v] = cuts ? 0.f : kk[v];
-    if (t0 - TILE >= tb) fetch(t0 - TILE);
-    scan_join_tile<VEC, CG, true>(kk, cc, carry, in, lds[buf], wave, lane);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) all[v] = scan_times(lds[buf][((w * 2) * VEC + v) * CG + cg], all[v]);
+    const int before = t0 - TILE >= me.tb ? me.te : 0;
+    gate.fetch(rg, max(tw - TILE, 0), before, a.D);
+    dy.fetch(rd, max(tw - TILE, 0), before, a.D);
+    rs = scan_start<CG, L>(starts, max(t - TILE, 0), me.te, me.lane);
+    scan_join_tile<VEC, CG, WAVES, true>(kk, cc, carry, all, in, lds[buf], me.wave, me.lane);
   }
-  if (tc == 0 && dok) {
-    float* p = a.seg + ((long long)b * a.nseg + seg) * 2 * a.D + d0;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { p[v] = all[v]; p[a.D + v] = carry[v]; }
+  if (me.chok) {
+    float* p = a.seg + ((long long)me.b * a.nseg + me.seg) * 2 * a.D + me.ch;
+    p[0] = all;
+    p[a.D] = carry;
   }
 }
 
@@ -468,19 +529,19 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_short_kernel(const ScanArgs
 
 // ---------------------------------------------------------------------------------------------------------- host side
 struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
-// wide: rows of whole 16-byte pieces.  The time axis is split (two launches, gate and x read twice) only when sequences
+// wide: rows of whole pieces of 4 elements.  The time axis is split (two launches, gate and x read twice) only when sequences
 // and channels alone give fewer workgroups than there are CUs.
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
-  p.vec = !wide ? 1 : type == SERL_F32 ? 4 : 8;
-  p.cg = wide ? 8 : 64;
+  p.vec = wide ? 4 : 1;
+  p.cg = !wide ? 64 : type == SERL_F32 ? 8 : 16;
   p.ndb = cdiv(D, p.vec * p.cg);
   p.nseg = 1;
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
-  if (blocks < 256 && T > 1024) {
+  if (blocks <= 144 && T > 2 * SCAN_CKPT) {
     const int want = (int)cdivll(512, blocks);
-    p.seg_len = cdiv(cdiv(T, want < SCAN_MAXSEG ? want : SCAN_MAXSEG), 512) * 512;
+    p.seg_len = cdiv(cdiv(T, want < SCAN_MAXSEG ? want : SCAN_MAXSEG), SCAN_CKPT) * SCAN_CKPT;
     p.nseg = cdiv(T, p.seg_len);
   }
   return p;
@@ -506,34 +567,43 @@ extern "C" long long serl_gated_scan_states_floats(int B, int T, int D) {
   return (long long)B * cdivll(T, SCAN_CKPT) * D;
 }
 
-static bool scan_wide(int type, int D, const void* p, long long bs, long long ts) {
-  const int vec = type == SERL_F32 ? 4 : 8;
-  return D % vec == 0 && bs % vec == 0 && ts % vec == 0 && sq_aligned(p, 16);
+// A wave addresses its rows of a tile (at most 32; narrow: 16) with 31-bit byte offsets from the first.
+static bool scan_reach(int type, bool wide, int D, long long ts) {
+  return ts < (1ll << 40) && ((wide ? 31 : 15) * ts + D) * sq_size(type) < (1ll << 31);
+}
+// whether every row of (B, T, D) starts at a multiple of `vec` elements and holds whole pieces of them
+static bool scan_wide(int type, int vec, int D, const void* p, long long bs, long long ts) {
+  return D % vec == 0 && bs % vec == 0 && ts % vec == 0 && sq_aligned(p, vec * sq_size(type)) && scan_reach(type, true, D, ts);
 }
 
+// Tiles of 128 steps (a kept state in front of each), of 64 where no sequence is longer: 16 elements per thread.  Wide: 128
+// bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32 elements per thread 10 to
+// 20 %: registers).
+#define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
+#define SCAN_PICK(KERNEL, ...)                                                          \
+  do {                                                                                  \
+    if (p.vec == 1) {                                                                   \
+      if (a.T <= 64) SCAN_GO(KERNEL, 1, 64, 8, 512, ##__VA_ARGS__);                     \
+      else SCAN_GO(KERNEL, 1, 64, 8, 1024, ##__VA_ARGS__);                               \
+    } else if constexpr (T::code == SERL_F32) {                                         \
+      if (a.T <= 64) SCAN_GO(KERNEL, 4, 8, 2, 256, ##__VA_ARGS__);                      \
+      else SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);                                \
+    } else {                                                                            \
+      if (a.T <= 64) SCAN_GO(KERNEL, 4, 16, 4, 256, ##__VA_ARGS__);                     \
+      else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                               \
+    }                                                                                   \
+  } while (0)
 template <typename T>
 static void scan_launch_fwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
-  constexpr int W = T::code == SERL_F32 ? 4 : 8;
-  const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb)), blk(SCAN_THREADS);
-  if (p.vec == 1) {
-    if (a.nseg > 1) hipLaunchKernelGGL((scan_fwd_kernel<T, 1, 64, 32, true>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((scan_fwd_kernel<T, 1, 64, 32, false>), grid, blk, 0, st, a);
-  } else {
-    if (a.nseg > 1) hipLaunchKernelGGL((scan_fwd_kernel<T, W, 8, 4, true>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((scan_fwd_kernel<T, W, 8, 4, false>), grid, blk, 0, st, a);
-  }
+  const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
+  if (a.nseg > 1) SCAN_PICK(scan_fwd_kernel, true);
+  SCAN_PICK(scan_fwd_kernel, false);
 }
 template <typename T>
 static void scan_launch_bwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
-  constexpr int W = T::code == SERL_F32 ? 4 : 8;
-  const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb)), blk(SCAN_THREADS);
-  if (p.vec == 1) {
-    if (a.nseg > 1) hipLaunchKernelGGL((scan_bwd_summary_kernel<T, 1, 64, 32>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((scan_bwd_kernel<T, 1, 64, 32>), grid, blk, 0, st, a);
-  } else {
-    if (a.nseg > 1) hipLaunchKernelGGL((scan_bwd_summary_kernel<T, W, 8, 4>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((scan_bwd_kernel<T, W, 8, 4>), grid, blk, 0, st, a);
-  }
+  const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
+  if (a.nseg > 1) SCAN_PICK(scan_bwd_summary_kernel);
+  SCAN_PICK(scan_bwd_kernel);
 }
 template <typename T>
 static void scan_launch_short(ScanArgs a, bool wide, hipStream_t st) {
@@ -559,8 +629,9 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
                  "gated_scan_fwd: negative stride");
   SERL_CHECK_ARG((T <= 1 || y_ts >= D) && (T == 0 || B <= 1 || y_bs >= D), "gated_scan_fwd: rows of y overlap");
   SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_fwd: T too large");
-  const bool wide = scan_wide(type, D, gate, gate_bs, gate_ts) && scan_wide(type, D, x, x_bs, x_ts) &&
-                    scan_wide(type, D, y, y_bs, y_ts);
+  const int vec = T <= SCAN_SHORT && type != SERL_F32 ? 8 : 4;
+  const bool wide = scan_wide(type, vec, D, gate, gate_bs, gate_ts) && scan_wide(type, vec, D, x, x_bs, x_ts) &&
+                    scan_wide(type, vec, D, y, y_bs, y_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll && (long long)B * D <= 0x7fffffffll * SCAN_THREADS,
                  "gated_scan_fwd: B * D too large");
@@ -575,6 +646,8 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
     else if (type == SERL_BF16) scan_launch_short<BF16>(a, wide, st);
     else scan_launch_short<F16>(a, wide, st);
   } else {
+    SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, y_ts),
+                   "gated_scan_fwd: 15 steps of a tensor must span less than 2^31 bytes");
     const long long need = scan_ws(p, B, D);
     SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                    "gated_scan_fwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
@@ -601,11 +674,14 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG((T <= 1 || (dgate_ts >= D && dx_ts >= D)) && (B <= 1 || (dgate_bs >= D && dx_bs >= D)),
                  "gated_scan_bwd: rows of dgate or dx overlap");
   SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_bwd: T too large");
-  const bool wide = scan_wide(type, D, gate, gate_bs, gate_ts) && scan_wide(type, D, x, x_bs, x_ts) &&
-                    scan_wide(type, D, dy, dy_bs, dy_ts) && scan_wide(type, D, dgate, dgate_bs, dgate_ts) &&
-                    scan_wide(type, D, dx, dx_bs, dx_ts);
+  const bool wide = scan_wide(type, 4, D, gate, gate_bs, gate_ts) && scan_wide(type, 4, D, x, x_bs, x_ts) &&
+                    scan_wide(type, 4, D, dy, dy_bs, dy_ts) && scan_wide(type, 4, D, dgate, dgate_bs, dgate_ts) &&
+                    scan_wide(type, 4, D, dx, dx_bs, dx_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll, "gated_scan_bwd: B * D too large");
+  SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
+                 scan_reach(type, false, D, dgate_ts) && scan_reach(type, false, D, dx_ts),
+                 "gated_scan_bwd: 15 steps of a tensor must span less than 2^31 bytes");
   const long long need = scan_ws(p, B, D);
   SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                  "gated_scan_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);

@@ -256,8 +256,10 @@ def test_gated_scan_offsets_beyond_32_bits(dev):
     b = s.gated_scan(gate, x, i["h0"], save=True)
     ga = s.gated_scan_backward(i["gate"], i["x"], a[2], i["dy"], i["dh_last"])
     gb = s.gated_scan_backward(gate, x, b[2], i["dy"], i["dh_last"])
+    # rows this far apart run the kernel of narrow loads, whose threads join in another order: both results are within
+    # check_scan's tolerance of the recurrence, with |G| <= 57 max |dy| <= 57 * 5 and |h| + |x| <= 10
     for u, v in zip(a + ga, b + gb):
-        assert torch.equal(u, v)
+        within(v, u, 2 * (2 * SCAN_STATE * 57 * 5 * 10 / 4 + HALF[torch.bfloat16] * u.double().abs().cpu()), "far rows")
 
 
 def replayed(dev, fn, outputs_of):
