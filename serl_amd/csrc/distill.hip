@@ -450,8 +450,13 @@ static DistPlan dist_plan(int type, int R, int V, bool wide) {
 
 template <typename T, int VEC, int THREADS, int NV>
 static void dist_go(const DistArgs& a, hipStream_t st) {
-  // persistent: as many workgroups as fit the 256 CUs at once
-  const int fit = THREADS == 1024 ? 256 : THREADS == 256 ? 256 * 4 : 256 * 16;
+  // persistent: as many workgroups as 256 CUs hold at once (asked for once; 128 slots' tables in LDS)
+  static const int fit = [] {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV>, THREADS,
+                                                     3 * 3 * 128 * sizeof(float)) != hipSuccess || n < 1) n = 1;
+    return 256 * n;
+  }();
   hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
                      3 * 3 * a.K * sizeof(float), st, a);
 }
@@ -470,9 +475,10 @@ static void dist_launch(const DistArgs& a, hipStream_t st) {
   } else {
     if (n <= 64) dist_go<T, VEC, 64, 1>(a, st);
     else if (n <= 256) dist_go<T, VEC, 64, 4>(a, st);
-    else if (n <= 1024) dist_go<T, VEC, 256, 4>(a, st);
+    else if (n <= 512) dist_go<T, VEC, 64, 8>(a, st);
+    else if (n <= 1024) dist_go<T, VEC, 128, 8>(a, st);
     else if (n <= 2048) dist_go<T, VEC, 256, 8>(a, st);
-    else if (n <= 4096) dist_go<T, VEC, 1024, 4>(a, st);
+    else if (n <= 4096) dist_go<T, VEC, 512, 8>(a, st);
     else if (n <= 8192) dist_go<T, VEC, 1024, 8>(a, st);
     else if (n <= 16384) dist_go<T, VEC, 1024, 16>(a, st);
     else dist_go<T, VEC, 1024, 20>(a, st);
