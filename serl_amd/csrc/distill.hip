@@ -156,6 +156,8 @@ __device__ __forceinline__ float dist_loss(const DistArgs& a, const DistTeacher&
   }
   return sq_wave_sum(s);
 }
+// All the wave's stores have been taken: behind the barrier that follows, another wave's store to the same place comes later.
+__device__ __forceinline__ void dist_drain() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // the teacher's columns [lo, hi): scale (p - q summed over the slots of the column), slots in order
 template <typename T>
 __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistTeacher& d, float m, float inv_sum, float scale,
@@ -167,6 +169,7 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
     const int id = d.idx[k];
     if (id < lo || id >= hi) continue;
     float q = 0.f;
+#pragma unroll 8
     for (int j = 0; j < a.K; ++j) q += d.idx[j] == id ? d.q[j] : 0.f;
     out[id] = sq_bits(T(), scale * (dist_exp(d.lg[k], m, k2) * inv_sum - q));
   }
@@ -229,6 +232,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     s += dist_exp(xe[0], wref, k2);
     s = sq_wave_sum(s);
     if (lane == 0) { red[buf][wave][0] = m; red[buf][wave][1] = s; }
+    dist_drain();          // the last row's gradient; its loads are behind those of this row, which have arrived
     __syncthreads();
     if (last >= 0) dist_fix<T>(a, last, dist_tables(tables, a.K, tab == 0 ? 2 : tab - 1), last_m, last_inv, last_scale, 0, a.V, t, THREADS);
     if constexpr (WAVES > 1) {              // lane 0's join for everybody: the order of the parts, and so the bits, are its own
@@ -286,6 +290,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     }
     w = wn;
   }
+  dist_drain();
   __syncthreads();
   if (last >= 0) dist_fix<T>(a, last, dist_tables(tables, a.K, tab == 0 ? 2 : tab - 1), last_m, last_inv, last_scale, 0, a.V, t, THREADS);
 }
@@ -363,6 +368,18 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
   const int j0 = piece * a.piece_vecs, j1 = min(w.nvec, j0 + a.piece_vecs);
   const float k2 = DIST_LOG2E / a.tau;
   const DistTeacher d = dist_tables(tables, a.K, 0);
+  constexpr int U = 4;
+  Raw<T, VEC> raw[U];
+  const auto fetch = [&](int jb) {
+    if (jb < j1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * DIST_CUT + t;
+        dist_load(raw[u], p + w.nh, j < j1 ? j : j1 - 1);
+      }
+    }
+  };
+  if (a.dlogits) fetch(j0);             // under way while the statistics and the teacher are read
   // every wave joins the row's statistics; wave 0 takes the teacher
   float m = -INFINITY, s = 0.f;
   for (int q = lane; q < a.pieces; q += 64) {
@@ -388,14 +405,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
   const bool dead = !alive || c == 0.f;
   const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
   bits* out = (bits*)a.dlogits + row * a.ldd;
-  constexpr int U = 4;
   for (int jb = j0; jb < j1; jb += DIST_CUT * U) {
-    Raw<T, VEC> raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * DIST_CUT + t;
-      dist_load(raw[u], p + w.nh, j < j1 ? j : j1 - 1);
-    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = jb + u * DIST_CUT + t;
@@ -406,6 +416,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
       raw[u].put(x);
       if (j < j1) dist_store(raw[u], out + w.nh, j);
     }
+    fetch(jb + DIST_CUT * U);
   }
   const int ex = piece == 0 ? dist_extra<VEC>(w, t) : -1;
   if (ex >= 0) {
@@ -417,6 +428,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
     e.put(x);
     e.store(out + ex);
   }
+  dist_drain();
   __syncthreads();
   if (dead) return;
   dist_fix<T>(a, row, d, m, inv, scale, w.nh + j0 * VEC, w.nh + j1 * VEC, t, DIST_CUT);
@@ -454,7 +466,10 @@ static void dist_go(const DistArgs& a, hipStream_t st) {
   static const int fit = [] {
     int n = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV>, THREADS,
-                                                     3 * 3 * 128 * sizeof(float)) != hipSuccess || n < 1) n = 1;
+                                                     3 * 3 * 128 * sizeof(float)) != hipSuccess || n < 1) {
+      (void)hipGetLastError();
+      n = 1;
+    }
     return 256 * n;
   }();
   hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
