@@ -118,7 +118,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
   const float inv = 1.f / a.tau;
   float top = -INFINITY;
   bool any = false;
-#pragma unroll 1
+#pragma unroll(TAKEN ? 4 : 1)      // the kernel that holds rows has no registers to spare
   for (int k = lane; k < a.K; k += 64) {
     const long long id = dist_column(a, row, k);
     const float tv = a.teacher_f32 ? ((const float*)a.teacher)[row * a.ldt + k]
@@ -169,8 +169,16 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
     const int id = d.idx[k];
     if (id < lo || id >= hi) continue;
     float q = 0.f;
-#pragma unroll 8
-    for (int j = 0; j < a.K; ++j) q += d.idx[j] == id ? d.q[j] : 0.f;
+    int j = 0;
+    for (; j + 8 <= a.K; j += 8) {       // both read whatever they are: the reads of eight slots are under way together
+      int ij[8];
+      float qj[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { ij[i] = d.idx[j + i]; qj[i] = d.q[j + i]; }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q += ij[i] == id ? qj[i] : 0.f;
+    }
+    for (; j < a.K; ++j) q += d.idx[j] == id ? d.q[j] : 0.f;
     out[id] = sq_bits(T(), scale * (dist_exp(d.lg[k], m, k2) * inv_sum - q));
   }
 }
@@ -357,8 +365,9 @@ __global__ __launch_bounds__(DIST_CUT) void dist_stats_kernel(const DistArgs a) 
   }
 }
 
+// Four waves write the gradient of a piece, a fifth takes the teacher meanwhile; only then the teacher's columns are put right.
 template <typename T, int VEC>
-__global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
+__global__ __launch_bounds__(DIST_CUT + 64) void dist_grad_kernel(const DistArgs a) {
   extern __shared__ float tables[];
   __shared__ int alive;
   typedef typename T::bits bits;
@@ -368,6 +377,7 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
   const int j0 = piece * a.piece_vecs, j1 = min(w.nvec, j0 + a.piece_vecs);
   const float k2 = DIST_LOG2E / a.tau;
   const DistTeacher d = dist_tables(tables, a.K, 0);
+  const bool dense = t < DIST_CUT;
   constexpr int U = 4;
   Raw<T, VEC> raw[U];
   const auto fetch = [&](int jb) {
@@ -379,9 +389,10 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
       }
     }
   };
-  if (a.dlogits) fetch(j0);             // under way while the statistics and the teacher are read
-  // every wave joins the row's statistics; wave 0 takes the teacher
-  float m = -INFINITY, s = 0.f;
+  if (dense && a.dlogits) fetch(j0);    // under way while the statistics are read
+  bool any = false;
+  if (!dense) any = dist_stage<T, true>(a, row, d, lane);
+  float m = -INFINITY, s = 0.f;         // every wave joins the row's statistics
   for (int q = lane; q < a.pieces; q += 64) {
     const float* o = a.part + ((long long)row * a.pieces + q) * 2;
     dist_join(m, s, o[0], o[1], k2);
@@ -391,50 +402,59 @@ __global__ __launch_bounds__(DIST_CUT) void dist_grad_kernel(const DistArgs a) {
     const float m2 = __shfl_xor(m, o), s2 = __shfl_xor(s, o);
     dist_join(m, s, m2, s2, k2);
   }
+  m = dist_uniform(m);
+  s = dist_uniform(s);
   const float c = a.coef ? a.coef[row] : 1.f;
-  if (t < 64) {
-    const bool any = dist_stage<T, true>(a, row, d, lane);
+  const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
+  bits* out = (bits*)a.dlogits + row * a.ldd;
+  const int ex = piece == 0 && dense ? dist_extra<VEC>(w, t) : -1;
+  if (!dense) {
     if (lane == 0) alive = any;
     if (piece == 0) {
       const float l = dist_loss(a, d, m, s, lane);
       if (lane == 0) a.loss[row] = any && c != 0.f ? c * a.tau * a.tau * l : 0.f;
     }
-  }
-  __syncthreads();
-  if (!a.dlogits) return;
-  const bool dead = !alive || c == 0.f;
-  const float inv = 1.f / s, scale = c * a.tau, mul = scale * inv;
-  bits* out = (bits*)a.dlogits + row * a.ldd;
-  for (int jb = j0; jb < j1; jb += DIST_CUT * U) {
+  } else if (a.dlogits && c != 0.f) {
+    for (int jb = j0; jb < j1; jb += DIST_CUT * U) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = jb + u * DIST_CUT + t;
-      float x[VEC];
-      raw[u].get(x);
+      for (int u = 0; u < U; ++u) {
+        const int j = jb + u * DIST_CUT + t;
+        float x[VEC];
+        raw[u].get(x);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
-      raw[u].put(x);
-      if (j < j1) dist_store(raw[u], out + w.nh, j);
+        for (int v = 0; v < VEC; ++v) x[v] = dist_exp(x[v], m, k2) * mul;
+        raw[u].put(x);
+        if (j < j1) dist_store(raw[u], out + w.nh, j);
+      }
+      fetch(jb + DIST_CUT * U);
     }
-    fetch(jb + DIST_CUT * U);
+    if (ex >= 0) {
+      Raw<T, 1> e;
+      e.load(p + ex);
+      float x[1];
+      e.get(x);
+      x[0] = dist_exp(x[0], m, k2) * mul;
+      e.put(x);
+      e.store(out + ex);
+    }
   }
-  const int ex = piece == 0 ? dist_extra<VEC>(w, t) : -1;
-  if (ex >= 0) {
-    Raw<T, 1> e;
-    e.load(p + ex);
-    float x[1];
-    e.get(x);
-    x[0] = dead ? 0.f : dist_exp(x[0], m, k2) * mul;
-    e.put(x);
-    e.store(out + ex);
-  }
+  if (!a.dlogits) return;
   dist_drain();
   __syncthreads();
-  if (dead) return;
-  dist_fix<T>(a, row, d, m, inv, scale, w.nh + j0 * VEC, w.nh + j1 * VEC, t, DIST_CUT);
-  if (piece == 0) {
-    dist_fix<T>(a, row, d, m, inv, scale, 0, w.nh, t, DIST_CUT);
-    dist_fix<T>(a, row, d, m, inv, scale, w.nh + w.nvec * VEC, a.V, t, DIST_CUT);
+  if (alive && c != 0.f) {
+    dist_fix<T>(a, row, d, m, inv, scale, w.nh + j0 * VEC, w.nh + j1 * VEC, t, DIST_CUT + 64);
+    if (piece == 0) {
+      dist_fix<T>(a, row, d, m, inv, scale, 0, w.nh, t, DIST_CUT + 64);
+      dist_fix<T>(a, row, d, m, inv, scale, w.nh + w.nvec * VEC, a.V, t, DIST_CUT + 64);
+    }
+  } else if (dense) {                   // a row that is left out: zeros, whatever was written above
+    Raw<T, VEC> zero;
+    float x[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) x[v] = 0.f;
+    zero.put(x);
+    for (int j = j0 + t; j < j1; j += DIST_CUT) dist_store(zero, out + w.nh, j);
+    if (ex >= 0) out[ex] = 0;
   }
 }
 
@@ -478,9 +498,9 @@ static void dist_go(const DistArgs& a, hipStream_t st) {
 template <typename T, int VEC>
 static void dist_launch(const DistArgs& a, hipStream_t st) {
   if (a.pieces > 1) {
-    const dim3 grid((unsigned)(a.R * a.pieces)), blk(DIST_CUT);
-    hipLaunchKernelGGL((dist_stats_kernel<T, VEC>), grid, blk, 0, st, a);
-    hipLaunchKernelGGL((dist_grad_kernel<T, VEC>), grid, blk, 3 * a.K * sizeof(float), st, a);
+    const dim3 grid((unsigned)(a.R * a.pieces));
+    hipLaunchKernelGGL((dist_stats_kernel<T, VEC>), grid, dim3(DIST_CUT), 0, st, a);
+    hipLaunchKernelGGL((dist_grad_kernel<T, VEC>), grid, dim3(DIST_CUT + 64), 3 * a.K * sizeof(float), st, a);
     return;
   }
   const int n = cdiv(a.V, VEC);
