@@ -8,7 +8,7 @@ Tensors are float32, bfloat16 or float16 on one GPU, channels contiguous (others
 sums are float32 and a value is rounded once, when it is stored.  Calls are enqueued on the current stream of the tensors'
 device, wait for nothing, and may be captured into a graph; results and scratch memory come from torch's allocator, call by
 call, so nothing is shared between calls or graphs.  As in the learners, gradients are explicit calls: autograd records
-nothing here.  Wrong types raise TypeError, wrong shapes ValueError, before anything is enqueued.  Results are the same
+nothing here, and the gradient of an expanded (broadcast) input comes full size, for the caller to sum.  Wrong types raise TypeError, wrong shapes ValueError, before anything is enqueued.  Results are the same
 bits on every call with the same arguments."""
 from __future__ import annotations
 
@@ -30,7 +30,7 @@ except AttributeError:
 def _shape(t, name, shape):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
@@ -39,19 +39,20 @@ def _type(t, name, *dtypes):
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
 
 
-def _place(*named):
+def _place(names, *tensors):
     """The tensors' common GPU: the context that makes it the current one."""
-    dev = None
-    for name, t in named:
+    at = None
+    for i, t in enumerate(tensors):
         if t is None:
             continue
-        if not t.is_cuda:
-            raise TypeError(f"{name} must be a CUDA tensor")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the others on {dev}")
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        d = t.get_device()              # -1: not on a GPU
+        if d < 0:
+            raise TypeError(f"{names[i]} must be a CUDA tensor")
+        if at is None:
+            at = d
+        elif d != at:
+            raise ValueError(f"{names[i]} is on {t.device}, the others on cuda:{at}")
+    return _NO_GUARD if at == torch.cuda.current_device() else torch.cuda.device(at)
 
 
 def _channels(t):
@@ -120,7 +121,7 @@ def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
     gated_scan_backward needs."""
     B, T, D = _scan_args(gate, x, starts, lengths)
     _state(h0, "h0", B, D)
-    with _place(("gate", gate), ("x", x), ("h0", h0), ("starts", starts), ("lengths", lengths)):
+    with _place(("gate", "x", "h0", "starts", "lengths"), gate, x, h0, starts, lengths):
         gate, x = _channels(gate), _channels(x)
         starts, lengths = _masks(starts, lengths, T)
         if h0 is not None:
@@ -150,8 +151,8 @@ def gated_scan_backward(gate, x, saved, dy, dh_last=None, starts=None, lengths=N
         dgate, dx = _out(out[0], "out[0]", (B, T, D), gate.dtype), _out(out[1], "out[1]", (B, T, D), gate.dtype)
     else:
         dgate = dx = None
-    with _place(("gate", gate), ("x", x), ("saved", saved), ("dy", dy), ("dh_last", dh_last), ("starts", starts),
-                ("lengths", lengths), ("out[0]", dgate), ("out[1]", dx)):
+    with _place(("gate", "x", "saved", "dy", "dh_last", "starts", "lengths", "out[0]", "out[1]"), gate, x, saved, dy, dh_last,
+                starts, lengths, dgate, dx):
         gate, x, dy, saved = _channels(gate), _channels(x), _channels(dy), saved.contiguous()
         starts, lengths = _masks(starts, lengths, T)
         if dh_last is not None:
@@ -192,7 +193,7 @@ def gated_scan_step(gate, x, h, starts=None, h_out=None):
         _state(h_out, "h_out", B, D)
         if not h_out.is_contiguous():
             raise ValueError("h_out must be contiguous")
-    with _place(("gate", gate), ("x", x), ("h", h), ("starts", starts), ("h_out", h_out)):
+    with _place(("gate", "x", "h", "starts", "h_out"), gate, x, h, starts, h_out):
         gate, x, h = _channels(gate), _channels(x), h.contiguous()
         y = torch.empty((B, D), dtype=gate.dtype, device=gate.device)
         if h_out is None:
@@ -230,7 +231,7 @@ def _norm_args(x, weight, residual):
 
 def _norm(x, weight, residual, eps, fp8, save):
     _norm_args(x, weight, residual)
-    with _place(("x", x), ("weight", weight), ("residual", residual)):
+    with _place(("x", "weight", "residual"), x, weight, residual):
         shape, N = x.shape, x.shape[-1]
         rows, res, weight = _rows(x), None if residual is None else _rows(residual), weight.contiguous()
         R, dev = rows.shape[0], x.device
@@ -279,7 +280,7 @@ def rms_norm_backward(dy, s, rstd, weight, ds=None):
     if ds is not None:
         _shape(ds, "ds", s.shape)
         _type(ds, "ds", s.dtype)
-    with _place(("s", s), ("dy", dy), ("rstd", rstd), ("weight", weight), ("ds", ds)):
+    with _place(("s", "dy", "rstd", "weight", "ds"), s, dy, rstd, weight, ds):
         shape, N = s.shape, s.shape[-1]
         sr, yr, dr = _rows(s), _rows(dy), None if ds is None else _rows(ds)
         weight, rstd = weight.contiguous(), rstd.contiguous()
@@ -331,7 +332,7 @@ def topk_distill(logits, teacher, index, temperature=1.0, coef=None, grad=True, 
         if not grad:
             raise ValueError("out is given, but no gradient is asked for")
         _out(out, "out", (R, V), logits.dtype)
-    with _place(("logits", logits), ("teacher", teacher), ("index", index), ("coef", coef), ("out", out)):
+    with _place(("logits", "teacher", "index", "coef", "out"), logits, teacher, index, coef, out):
         logits = _channels(logits)
         teacher, index = _channels(teacher), _channels(index)
         if coef is not None:

@@ -668,6 +668,60 @@ def test_topk_distill_in_graphs(dev):
         replayed(dev, lambda: s.topk_distill(i["logits"], i["teacher"], i["index"], 1.0, i["coef"]), list)
 
 
+# ------------------------------------------------------------------------------------------------ all of them
+def test_rows_of_any_stride(dev):
+    """Broadcast steps (stride 0), windows that overlap (a stride below the width), single channels of wider rows."""
+    s = seq()
+    for dtype in (torch.float32, torch.bfloat16):
+        for T in (3, 40, 300):
+            for D in (1, 16, 50):
+                i = scan_inputs(dev, dtype, 2, T, D, T + D)
+                base = torch.randn((2, T + D), device=dev).to(dtype)
+                windows = torch.as_strided(base, (2, T, D), (T + D, 1, 1))
+                fixed = i["gate"][:, :1].expand(2, T, D)
+                one = torch.randn((2, T, D, 3), device=dev).to(dtype)[..., 1]
+                for gate, x in ((fixed, windows), (i["gate"], windows), (windows, i["x"]), (one, one)):
+                    a = s.gated_scan(gate, x, i["h0"], save=True)
+                    b = s.gated_scan(gate.contiguous(), x.contiguous(), i["h0"], save=True)
+                    ga = s.gated_scan_backward(gate, x, a[2], i["dy"], i["dh_last"])
+                    gb = s.gated_scan_backward(gate.contiguous(), x.contiguous(), b[2], i["dy"], i["dh_last"])
+                    # narrow and wide loads join in another order: both within check_scan's tolerance, |G| <= 57 * 5, |h| + |x| <= 10
+                    for u, v in zip(a + ga, b + gb):
+                        within(u, v, 2 * (2 * SCAN_STATE * 57 * 5 * 10 / 4 + HALF[dtype] * v.double().abs().cpu()), "strides")
+    x = torch.randn((1, 96), device=dev).bfloat16().expand(5, 96)
+    w = torch.ones(96, device=dev)
+    y, total, rstd = s.rms_norm(x, w, residual=x, save=True)
+    assert torch.equal(y, y[:1].expand(5, 96)) and torch.equal(total, (x.float() * 2).bfloat16())
+    dx, dw = s.rms_norm_backward(x, total, rstd, w, ds=x)
+    assert torch.equal(dx, dx[:1].expand(5, 96))
+
+
+def test_two_streams_at_once(dev):
+    """The same calls on two streams together, those with scratch memory among them, give what one call alone gives."""
+    s = seq()
+    i = scan_inputs(dev, torch.bfloat16, 2, 3000, 64, 1, starts=True)
+    n = norm_inputs(dev, torch.bfloat16, torch.bfloat16, 900, 520, 1)
+    k = distill_inputs(dev, torch.bfloat16, 4, 30000, 20, 1)
+
+    def work():
+        y, h, saved = s.gated_scan(i["gate"], i["x"], i["h0"], i["starts"], save=True)
+        out = [y, h, *s.gated_scan_backward(i["gate"], i["x"], saved, i["dy"], i["dh_last"], i["starts"])]
+        y, total, rstd = s.rms_norm(n["x"], n["weight"], n["residual"], save=True)
+        out += [y, *s.rms_norm_backward(n["dy"], total, rstd, n["weight"], n["ds"])]
+        return out + list(s.topk_distill(k["logits"], k["teacher"], k["index"], 1.0, k["coef"]))
+    want = work()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(dev) for _ in range(2)], []
+    for _ in range(6):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(work())
+    torch.cuda.synchronize()
+    for out in got:
+        for u, v in zip(out, want):
+            assert torch.equal(u, v)
+
+
 # --------------------------------------------------------------------------------------------------- used together
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
 def test_a_recurrent_policy_learns_a_step_from_its_teacher(dev, dtype):
@@ -718,4 +772,4 @@ def test_a_recurrent_policy_learns_a_step_from_its_teacher(dev, dtype):
     tol = 40 * max(HALF[dtype], 16 * U)
     for got, want in ((dx, gx), (dw1, gw1), (dw2, gw2)):
         within(got, want, tol * want.abs().max(), "gradient")
-    assert abs(float(loss.sum()) - float(total)) <= tol * float(total)
+    assert abs(float(loss.sum()) - total.item()) <= tol * total.item()
