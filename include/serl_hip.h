@@ -476,7 +476,7 @@ int serl_learner_timing_reset(serl_learner* h);
 /* ---- operators of sequence policies (serl_amd/sequence.py): no counterpart in the reference, whose policies see history
  * through frame stacks and whose only discrete head is the gripper's.  type: 0 fp32, 1 bf16, 2 fp16 of the tensors named
  * `const void*` / `void*`; strides in elements; all sums, states and statistics are fp32, a value is rounded once, when it
- * is stored.  Any alignment and stride is taken: rows of whole 16-byte pieces at 16-byte addresses run wide loads.
+ * is stored.  Any alignment and stride is taken; rows at 16-byte (recurrence: 4-byte) addresses run wide loads.
  *
  * Gated linear recurrence: f = sigmoid(gate), h_t = f_t (start_t ? 0 : h_{t-1}) + (1 - f_t) x_t, y_t = h_t over (B, T, D)
  * (_bs, _ts: strides of a sequence and of a step; channels are contiguous).  h0 (B, D) or NULL = 0; starts: bytes (B, T),

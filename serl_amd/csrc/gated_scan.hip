@@ -120,6 +120,8 @@ __device__ __forceinline__ void scan_join_tile(float (&k)[VEC], float (&b)[VEC],
 }
 
 // What a thread of the tile kernels is: VEC channels from d0 on, L steps of every tile; a wave's steps are 64 / CG * L rows.
+// Where D is no multiple of VEC the last thread's channels are the row's last VEC: some it has in common with the thread
+// before, and both compute and store the same bits for those.
 template <int VEC, int CG, int L>
 struct ScanSpot {
   static constexpr int ROWS = 64 / CG * L;
@@ -134,10 +136,10 @@ struct ScanSpot {
     seg = q % a.nseg;
     b = q / a.nseg;
     dok = want < a.D;
-    d0 = dok ? want : 0;
-    const int cw = db * CG * VEC + lane % (CG * VEC);
-    ch = min(cw, a.D - 1);
-    chok = wave == 0 && lane < CG * VEC && cw < a.D;
+    d0 = dok ? min(want, a.D - VEC) : 0;
+    const int slot = lane % (CG * VEC), group = (db * CG + slot / VEC) * VEC;
+    ch = min(group, a.D - VEC) + slot % VEC;
+    chok = wave == 0 && lane < CG * VEC && group < a.D;
     tb = seg * a.seg_len;
     te = min(a.T, tb + a.seg_len);
     len = min(te, scan_len(a, b));
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_short_kernel(const ScanArgs
 
 // ---------------------------------------------------------------------------------------------------------- host side
 struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
-// wide: rows of whole pieces of 4 elements.  The time axis is split (two launches, gate and x read twice) only when sequences
+// wide: 4 elements per access.  The time axis is split (two launches, gate and x read twice) only when sequences
 // and channels alone give fewer workgroups than there are CUs.
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
@@ -571,9 +573,13 @@ extern "C" long long serl_gated_scan_states_floats(int B, int T, int D) {
 static bool scan_reach(int type, bool wide, int D, long long ts) {
   return ts < (1ll << 40) && ((wide ? 31 : 15) * ts + D) * sq_size(type) < (1ll << 31);
 }
-// whether every row of (B, T, D) starts at a multiple of `vec` elements and holds whole pieces of them
-static bool scan_wide(int type, int vec, int D, const void* p, long long bs, long long ts) {
-  return D % vec == 0 && bs % vec == 0 && ts % vec == 0 && sq_aligned(p, vec * sq_size(type)) && scan_reach(type, true, D, ts);
+// whether every row of (B, T, D) starts at a multiple of `bytes` (the tile kernels' accesses of 4 elements want whole dwords)
+static bool scan_rows(int type, int bytes, const void* p, long long bs, long long ts) {
+  const int e = sq_size(type);
+  return bs * e % bytes == 0 && ts * e % bytes == 0 && sq_aligned(p, bytes);
+}
+static bool scan_wide(int type, int D, const void* p, long long bs, long long ts) {
+  return D >= 4 && D * sq_size(type) % 4 == 0 && scan_rows(type, 4, p, bs, ts) && scan_reach(type, true, D, ts);
 }
 
 // Tiles of 128 steps (a kept state in front of each), of 64 where no sequence is longer: 16 elements per thread.  Wide: 128
@@ -629,9 +635,11 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
                  "gated_scan_fwd: negative stride");
   SERL_CHECK_ARG((T <= 1 || y_ts >= D) && (T == 0 || B <= 1 || y_bs >= D), "gated_scan_fwd: rows of y overlap");
   SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_fwd: T too large");
-  const int vec = T <= SCAN_SHORT && type != SERL_F32 ? 8 : 4;
-  const bool wide = scan_wide(type, vec, D, gate, gate_bs, gate_ts) && scan_wide(type, vec, D, x, x_bs, x_ts) &&
-                    scan_wide(type, vec, D, y, y_bs, y_ts);
+  const bool few = T <= SCAN_SHORT;
+  const bool wide = few ? D * sq_size(type) % 16 == 0 && scan_rows(type, 16, gate, gate_bs, gate_ts) &&
+                              scan_rows(type, 16, x, x_bs, x_ts) && scan_rows(type, 16, y, y_bs, y_ts)
+                        : scan_wide(type, D, gate, gate_bs, gate_ts) && scan_wide(type, D, x, x_bs, x_ts) &&
+                              scan_wide(type, D, y, y_bs, y_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll && (long long)B * D <= 0x7fffffffll * SCAN_THREADS,
                  "gated_scan_fwd: B * D too large");
@@ -641,7 +649,7 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
   a.lengths = lengths; a.ckpt = states; a.B = B; a.T = T; a.D = D;
   a.ndb = p.ndb; a.nseg = p.nseg; a.seg_len = p.seg_len; a.seg = workspace;
   hipStream_t st = (hipStream_t)stream;
-  if (T <= SCAN_SHORT) {
+  if (few) {
     if (type == SERL_F32) scan_launch_short<F32>(a, wide, st);
     else if (type == SERL_BF16) scan_launch_short<BF16>(a, wide, st);
     else scan_launch_short<F16>(a, wide, st);
@@ -674,9 +682,9 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG((T <= 1 || (dgate_ts >= D && dx_ts >= D)) && (B <= 1 || (dgate_bs >= D && dx_bs >= D)),
                  "gated_scan_bwd: rows of dgate or dx overlap");
   SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_bwd: T too large");
-  const bool wide = scan_wide(type, 4, D, gate, gate_bs, gate_ts) && scan_wide(type, 4, D, x, x_bs, x_ts) &&
-                    scan_wide(type, 4, D, dy, dy_bs, dy_ts) && scan_wide(type, 4, D, dgate, dgate_bs, dgate_ts) &&
-                    scan_wide(type, 4, D, dx, dx_bs, dx_ts);
+  const bool wide = scan_wide(type, D, gate, gate_bs, gate_ts) && scan_wide(type, D, x, x_bs, x_ts) &&
+                    scan_wide(type, D, dy, dy_bs, dy_ts) && scan_wide(type, D, dgate, dgate_bs, dgate_ts) &&
+                    scan_wide(type, D, dx, dx_bs, dx_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll, "gated_scan_bwd: B * D too large");
   SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
