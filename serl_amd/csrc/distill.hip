@@ -10,6 +10,9 @@
 // stores overlap.  Few long rows, and rows too long for registers, are cut into pieces of their own workgroups: one launch
 // for the statistics, one that joins them and writes the gradient (it reads the row again, from the caches where they hold it).
 //
+// 2048 x 131072 bf16, 128 slots: 242 us (4.45 TB/s where a large copy reaches 5.2; the first load and the last store of a
+// workgroup's eight rows overlap nothing, and the vector ALU is half busy with two exponentials per column).
+//
 // Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
 // single threads (`head` and `tail`).  The teacher's columns are stored a second time, behind a barrier that all dense
 // stores of the row have passed.

@@ -6,6 +6,8 @@
 // Bound by memory: a row is read once into registers, reduced, and written; a wave takes a row of up to 1024 16-bit
 // elements (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
 // STORED (rounded to the residual's type): later layers and the backward pass see the values that were normed.
+// 16384 x 4096 bf16: forward 82 us (6.5 TB/s: part of it from the caches), backward 110 us (4.9 TB/s) and 5 us for the shares
+// of the weight's gradient; 64 rows to e4m3 4 us.
 #include "seqtypes.h"
 
 #define RMS_MAXN 32768
