@@ -484,7 +484,7 @@ int serl_learner_timing_reset(serl_learner* h);
  * give y = 0 and zero gradients, whatever the inputs hold there.  h_last (B, D) = the state behind the last step; it may be
  * h0 itself for T <= 8 (acting: T = 1).  states: NULL, or serl_gated_scan_states_floats floats that the backward pass
  * reads.  workspace: serl_gated_scan_workspace_bytes (0 for most shapes), for either direction, contents undefined.  For
- * T > 8 fifteen steps of a tensor must span less than 2^31 bytes. */
+ * T > 8 fifteen steps of a tensor must span less than 2^31 bytes; D <= 2^26. */
 long long serl_gated_scan_workspace_bytes(int type, int B, int T, int D);
 long long serl_gated_scan_states_floats(int B, int T, int D);
 int serl_gated_scan_fwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,

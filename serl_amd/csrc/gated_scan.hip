@@ -17,6 +17,7 @@
 
 #define SCAN_CKPT 128       // steps between the states that the forward pass keeps for the backward pass
 #define SCAN_THREADS 256    // of the kernel for a few steps
+#define SCAN_MAXD (1 << 26)  // channels
 #define SCAN_MAXSEG 32      // most pieces the time axis is split into
 
 struct ScanArgs {
@@ -562,7 +563,7 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
 static long long scan_ws(const ScanPlan& p, int B, int D) { return p.nseg > 1 ? (long long)B * p.nseg * 2 * D * 4 : 0; }
 
 extern "C" long long serl_gated_scan_workspace_bytes(int type, int B, int T, int D) {
-  if (type < 0 || type > 2 || B < 0 || T < 0 || D < 0) {
+  if (type < 0 || type > 2 || B < 0 || T < 0 || D < 0 || D > SCAN_MAXD) {
     serl_set_error("gated_scan: bad type or sizes");
     return -1;
   }
@@ -639,6 +640,7 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
                                    long long workspace_bytes, void* stream) {
   SERL_CHECK_ARG(type >= 0 && type <= 2, "gated_scan_fwd: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   SERL_CHECK_ARG(B >= 0 && T >= 0 && D >= 0, "gated_scan_fwd: negative size");
+  SERL_CHECK_ARG(D <= SCAN_MAXD, "gated_scan_fwd: D must be at most %d", SCAN_MAXD);
   if (B == 0 || D == 0) return SERL_OK;
   SERL_CHECK_ARG(h_last && (T == 0 || (gate && x && y)), "gated_scan_fwd: null pointer");
   SERL_CHECK_ARG(gate_bs >= 0 && gate_ts >= 0 && x_bs >= 0 && x_ts >= 0 && (!starts || starts_bs >= 0),
@@ -686,6 +688,7 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
                                    float* dh0, float* workspace, long long workspace_bytes, void* stream) {
   SERL_CHECK_ARG(type >= 0 && type <= 2, "gated_scan_bwd: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   SERL_CHECK_ARG(B >= 0 && T >= 1 && D >= 0, "gated_scan_bwd: bad size (T must be >= 1)");
+  SERL_CHECK_ARG(D <= SCAN_MAXD, "gated_scan_bwd: D must be at most %d", SCAN_MAXD);
   if (B == 0 || D == 0) return SERL_OK;
   SERL_CHECK_ARG(gate && x && states && dy && dgate && dx && dh0, "gated_scan_bwd: null pointer");
   SERL_CHECK_ARG(gate_bs >= 0 && gate_ts >= 0 && x_bs >= 0 && x_ts >= 0 && dy_bs >= 0 && dy_ts >= 0 &&

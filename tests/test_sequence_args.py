@@ -63,6 +63,10 @@ def test_gated_scan_entry_point_refusals():
         scan(gate_ts=-8)
     with pytest.raises(ValueError, match="rows of y overlap"):
         scan(y_ts=4)
+    with pytest.raises(ValueError, match="D must be at most 67108864"):
+        scan(D=(1 << 26) + 1)
+    with pytest.raises(ValueError, match="15 steps of a tensor must span less than"):
+        scan(T=9, gate_ts=1 << 26)
     with pytest.raises(ValueError, match=r"workspace of \d+ bytes needed, 0 available"):
         scan(T=5000, gate_bs=40000, x_bs=40000, y_bs=40000)
     with pytest.raises(ValueError, match="bad type or sizes"):
