@@ -578,7 +578,7 @@ def test_topk_distill_views_and_misaligned_rows(dev):
     assert torch.equal(t[1], s.topk_distill(i["logits"], i["teacher"], i["index"])[1])
 
 
-@pytest.mark.parametrize("R,V", [(8, 64), (8, 1500), (8, 9001), (200, 9001), (8, 70000), (200, 70000)])
+@pytest.mark.parametrize("R,V", [(8, 64), (8, 1500), (8, 9001), (200, 9001), (8, 70000), (200, 70000), (8, 170000)])
 def test_topk_distill_masks_infinities_and_nan(dev, R, V):
     s = seq()
     for dtype in DTYPES:
@@ -663,7 +663,7 @@ def test_topk_distill_no_rows_and_offsets_beyond_32_bits(dev):
 
 def test_topk_distill_in_graphs(dev):
     s = seq()
-    for R, V in ((64, 256), (3, 50000), (300, 5001)):
+    for R, V in ((64, 256), (3, 50000), (300, 5001), (3, 140001)):
         i = distill_inputs(dev, torch.bfloat16, R, V, 10, V)
         replayed(dev, lambda: s.topk_distill(i["logits"], i["teacher"], i["index"], 1.0, i["coef"]), list)
 
@@ -701,7 +701,7 @@ def test_two_streams_at_once(dev):
     s = seq()
     i = scan_inputs(dev, torch.bfloat16, 2, 3000, 64, 1, starts=True)
     n = norm_inputs(dev, torch.bfloat16, torch.bfloat16, 900, 520, 1)
-    k = distill_inputs(dev, torch.bfloat16, 4, 30000, 20, 1)
+    k = distill_inputs(dev, torch.bfloat16, 4, 140000, 20, 1)
 
     def work():
         y, h, saved = s.gated_scan(i["gate"], i["x"], i["h0"], i["starts"], save=True)
