@@ -20,6 +20,7 @@ from . import ops
 
 _CODES = {torch.float32: ops.F32, torch.bfloat16: ops.BF16, torch.float16: ops.F16}
 _NO_GUARD = contextlib.nullcontext()
+_ROWS = torch.contiguous_format
 try:                                    # the handle alone: a tenth of the time of torch.cuda.current_stream(), which makes an object
     _raw_stream = torch._C._cuda_getCurrentRawStream
 except AttributeError:
@@ -127,9 +128,9 @@ def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
         if h0 is not None:
             h0 = h0.contiguous()
         code, dev = _CODES[gate.dtype], gate.device
-        y = torch.empty((B, T, D), dtype=gate.dtype, device=dev)
-        h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
-        saved = torch.empty((B, -(-T // 128), D), dtype=torch.float32, device=dev) if save else None
+        y = torch.empty_like(gate, memory_format=_ROWS)
+        h_last = gate.new_empty((B, D), dtype=torch.float32)
+        saved = gate.new_empty((B, -(-T // 128), D), dtype=torch.float32) if save else None
         ws, nws = _scan_scratch(code, B, T, D, dev)
         ops.gated_scan_fwd(code, B, T, D, gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
                            x.stride(1), _ptr(h0), _ptr(starts), 0 if starts is None else starts.stride(0), _ptr(lengths),
@@ -159,11 +160,11 @@ def gated_scan_backward(gate, x, saved, dy, dh_last=None, starts=None, lengths=N
             dh_last = dh_last.contiguous()
         code, dev = _CODES[gate.dtype], gate.device
         if out is None:
-            dgate, dx = (torch.empty((B, T, D), dtype=gate.dtype, device=dev) for _ in range(2))
+            dgate, dx = torch.empty_like(gate, memory_format=_ROWS), torch.empty_like(gate, memory_format=_ROWS)
         if T == 0:
             dh0 = torch.zeros((B, D), dtype=torch.float32, device=dev) if dh_last is None else dh_last.clone()
             return dgate, dx, dh0
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev)
+        dh0 = gate.new_empty((B, D), dtype=torch.float32)
         ws, nws = _scan_scratch(code, B, T, D, dev)
         ops.gated_scan_bwd(code, B, T, D, gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
                            x.stride(1), _ptr(starts), 0 if starts is None else starts.stride(0), _ptr(lengths),
@@ -195,9 +196,9 @@ def gated_scan_step(gate, x, h, starts=None, h_out=None):
             raise ValueError("h_out must be contiguous")
     with _place(("gate", "x", "h", "starts", "h_out"), gate, x, h, starts, h_out):
         gate, x, h = _channels(gate), _channels(x), h.contiguous()
-        y = torch.empty((B, D), dtype=gate.dtype, device=gate.device)
+        y = torch.empty_like(gate, memory_format=_ROWS)
         if h_out is None:
-            h_out = torch.empty((B, D), dtype=torch.float32, device=gate.device)
+            h_out = torch.empty_like(h, memory_format=_ROWS)
         ops.gated_scan_fwd(_CODES[gate.dtype], B, 1, D, gate.data_ptr(), gate.stride(0), 0, x.data_ptr(), x.stride(0), 0,
                            h.data_ptr(), _ptr(starts), 0 if starts is None else starts.stride(0), None, y.data_ptr(), D, D,
                            h_out.data_ptr(), None, None, 0, _raw_stream(gate.device.index))
@@ -235,10 +236,10 @@ def _norm(x, weight, residual, eps, fp8, save):
         shape, N = x.shape, x.shape[-1]
         rows, res, weight = _rows(x), None if residual is None else _rows(residual), weight.contiguous()
         R, dev = rows.shape[0], x.device
-        y = torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=dev)
-        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if fp8 else None
-        total = x if res is None else torch.empty(shape, dtype=residual.dtype, device=dev)
-        rstd = torch.empty(shape[:-1], dtype=torch.float32, device=dev) if save else None
+        y = torch.empty_like(x, dtype=torch.float8_e4m3fn if fp8 else x.dtype, memory_format=_ROWS)
+        scale = x.new_empty(shape[:-1], dtype=torch.float32) if fp8 else None
+        total = x if res is None else torch.empty_like(residual, memory_format=_ROWS)
+        rstd = x.new_empty(shape[:-1], dtype=torch.float32) if save else None
         code = _CODES[x.dtype]
         ops.rms_norm_fwd(code, code if res is None else _CODES[residual.dtype], _CODES[weight.dtype], R, N, rows.data_ptr(),
                          rows.stride(0), _ptr(res), 0 if res is None else res.stride(0), weight.data_ptr(), eps, y.data_ptr(),
@@ -281,12 +282,12 @@ def rms_norm_backward(dy, s, rstd, weight, ds=None):
         _shape(ds, "ds", s.shape)
         _type(ds, "ds", s.dtype)
     with _place(("s", "dy", "rstd", "weight", "ds"), s, dy, rstd, weight, ds):
-        shape, N = s.shape, s.shape[-1]
+        N = s.shape[-1]
         sr, yr, dr = _rows(s), _rows(dy), None if ds is None else _rows(ds)
         weight, rstd = weight.contiguous(), rstd.contiguous()
         R, dev = sr.shape[0], s.device
-        dx = torch.empty(shape, dtype=s.dtype, device=dev)
-        dw = torch.empty((N,), dtype=torch.float32, device=dev)
+        dx = torch.empty_like(s, memory_format=_ROWS)
+        dw = s.new_empty(N, dtype=torch.float32)
         n = ops.rms_norm_bwd_workspace_bytes(R, N)
         ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
         ops.rms_norm_bwd(_CODES[dy.dtype], _CODES[s.dtype], _CODES[weight.dtype], R, N, yr.data_ptr(), yr.stride(0),
@@ -338,9 +339,9 @@ def topk_distill(logits, teacher, index, temperature=1.0, coef=None, grad=True, 
         if coef is not None:
             coef = coef.contiguous()
         dev, code = logits.device, _CODES[logits.dtype]
-        loss = torch.empty((R,), dtype=torch.float32, device=dev)
+        loss = logits.new_empty(R, dtype=torch.float32)
         if grad and out is None:
-            out = torch.empty((R, V), dtype=logits.dtype, device=dev)
+            out = torch.empty_like(logits, memory_format=_ROWS)
         n = ops.topk_distill_workspace_bytes(code, R, V, K)
         ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
         ops.topk_distill(code, _CODES[teacher.dtype], index.dtype == torch.int64, R, V, K, logits.data_ptr(), logits.stride(0),
