@@ -541,9 +541,10 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_short_kernel(const ScanArgs
 
 // ---------------------------------------------------------------------------------------------------------- host side
 struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
-// wide: 4 elements per access.  The time axis is split (two launches, gate and x read twice) only when sequences and
-// channels alone leave half of the CUs idle: 8 x 4000 x 1024 bf16 forward (128 workgroups) 86 -> 68 us, but 12 x 4000 x 1024
-// (192) 88 -> 132 us.
+// wide: 4 elements per access.  The time axis is split (two launches, gate and x read twice) only where sequences and
+// channels alone leave half of the CUs idle and there are more than 5 tiles.  bf16 forward: 8 x 4000 x 1024 (128 workgroups) 85 ->
+// 68 us; but 12 x 4000 x 1024 (192) 89 -> 132 us, 4 x 512 x 1024 (4 tiles) 11.9 -> 16 us; both ways: 9 x 2000 x 1024 (144) 117 ->
+// 128 us, 12 x 777 x 333 fp32 (132) 52 -> 44 us.
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
   p.vec = wide ? 4 : 1;
@@ -552,7 +553,7 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   p.nseg = 1;
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
-  if (blocks <= 144 && T > 2 * SCAN_CKPT) {
+  if (blocks <= 136 && T > 5 * SCAN_CKPT) {
     const int want = (int)cdivll(512, blocks);
     p.seg_len = cdiv(cdiv(T, want < SCAN_MAXSEG ? want : SCAN_MAXSEG), SCAN_CKPT) * SCAN_CKPT;
     p.nseg = cdiv(T, p.seg_len);
