@@ -57,10 +57,10 @@ def scan_reference(gate, x, h0, starts, lengths, dy=None, dh_last=None):
     first = torch.zeros((B, D), dtype=torch.float64) if h0 is None else h0.double().cpu()
     first.requires_grad_()
     h, ys = first, []
-    f = torch.sigmoid(gate)
+    f, xs = torch.sigmoid(gate).unbind(1), x.unbind(1)
     for t in range(T):
         prev = h if starts is None else torch.where(starts[:, t, None].cpu(), torch.zeros_like(h), h)
-        new = f[:, t] * prev + (1 - f[:, t]) * x[:, t]
+        new = f[t] * prev + (1 - f[t]) * xs[t]
         live = torch.ones((B, 1), dtype=torch.bool) if lengths is None else (t < lengths.cpu().long())[:, None]
         h = torch.where(live, new, h)
         ys.append(torch.where(live, new, torch.zeros_like(new)))
@@ -100,7 +100,8 @@ def check_scan(i, dtype, with_backward=True):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("B,T,D", [(1, 1, 1), (3, 1, 64), (2, 5, 7), (4, 8, 64), (2, 9, 16), (1, 31, 24), (2, 127, 40), (1, 128, 136),
-                                   (2, 129, 33), (3, 257, 96), (2, 385, 65), (1, 1100, 8), (2, 1537, 19), (1, 4700, 72)])
+                                   (2, 129, 33), (3, 257, 96), (2, 385, 65), (1, 640, 12), (2, 641, 10), (34, 645, 256), (35, 643, 256),
+                                   (1, 1100, 8), (2, 1537, 19), (1, 4700, 72)])
 def test_gated_scan_matches_the_recurrence(dev, dtype, B, T, D):
     for k, opt in enumerate(({}, {"starts": True}, {"lengths": True, "h0": False}, {"starts": True, "lengths": True})):
         check_scan(scan_inputs(dev, dtype, B, T, D, 100 * k + T + D, **opt), dtype)
