@@ -2,14 +2,15 @@
 the residual's addition, and the distillation of a teacher's top logits -- each with its gradient, all arithmetic in HIP
 kernels (csrc/gated_scan.hip, rms_norm.hip, distill.hip).  No counterpart in the reference: its policies see history
 through frame stacks (serl/networks/pixel_multiplexer.py:27) and its only discrete head is the gripper's
-(serl/agents/bc/pixel_hybrid_bc_learner.py:99-107).
+(serl/agents/bc/pixel_hybrid_bc_learner.py).
 
 Tensors are float32, bfloat16 or float16 on one GPU, channels contiguous (others are copied first); states, statistics and
 sums are float32 and a value is rounded once, when it is stored.  Calls are enqueued on the current stream of the tensors'
 device, wait for nothing, and may be captured into a graph; results and scratch memory come from torch's allocator, call by
 call, so nothing is shared between calls or graphs.  As in the learners, gradients are explicit calls: autograd records
-nothing here, and the gradient of an expanded (broadcast) input comes full size, for the caller to sum.  Wrong types raise TypeError, wrong shapes ValueError, before anything is enqueued.  Results are the same
-bits on every call with the same arguments."""
+nothing here, and the gradient of an expanded (broadcast) input comes full size, for the caller to sum.  Wrong types raise
+TypeError, wrong shapes ValueError, before anything is enqueued.  The same arguments, laid out the same, give the same bits
+on every call."""
 from __future__ import annotations
 
 import contextlib
