@@ -11,7 +11,8 @@
 #include "seqtypes.h"
 
 #define RMS_MAXN 32768
-#define RMS_PARTS 512        // rows of partial weight gradients: at most this many workgroups in the backward pass
+#define RMS_PARTS 512        // rows of partial weight gradients: at most this many workgroups in the backward pass,
+#define RMS_MOSTPARTS 8192   // more for short rows
 
 struct RmsArgs {
   const void *x, *res, *w, *ds;      // backward: x = dy, res = s
@@ -290,12 +291,19 @@ static void rms_pick_fwd(const RmsArgs& a, bool wide, hipStream_t st) {
   else rms_go_fwd<TX, TR, FP8, 1024, 8, V>(a, st);      // fp32 only: RMS_MAXN elements
 }
 
-// rows of the partial weight gradients: one per row of the input up to RMS_PARTS workgroups
-static int rms_parts(int R) { return R < RMS_PARTS ? (R + 3) / 4 * 4 : RMS_PARTS; }
+// Rows of the partial weight gradients: one per row of the input, at most RMS_PARTS (one per workgroup).  Short rows get more, as
+// many as keep the partial sums at 8 MB: 131072 x 512 bf16 355 -> 207 us both ways, 20000 x 1536 99 -> 88 us; longer ones, or
+// narrow loads, lose by it (32768 x 2048 with 2048 parts 193 -> 210 us, 5000 x 1001 fp32 39 -> 42 us).  vec: elements per access.
+static int rms_parts(int R, int N, int vec) {
+  const int n = cdiv(N, vec);
+  int most = vec > 1 && n <= 128 ? (1 << 21) / N : vec > 1 && n <= 256 ? (3 << 19) / N : RMS_PARTS;
+  most = (most < RMS_PARTS ? RMS_PARTS : most > RMS_MOSTPARTS ? RMS_MOSTPARTS : most) / 4 * 4;
+  return R < most ? (R + 3) / 4 * 4 : most;
+}
 
 template <typename TY, typename TS, int THREADS, int NV, int VEC>
 static void rms_go_bwd(const RmsArgs& a, hipStream_t st) {
-  const int parts = rms_parts(a.R);
+  const int parts = rms_parts(a.R, a.N, VEC);
   hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC>), dim3(THREADS == 64 ? parts / 4 : parts),
                      dim3(THREADS == 64 ? 256 : THREADS), 0, st, a);
 }
@@ -366,7 +374,8 @@ extern "C" long long serl_rms_norm_bwd_workspace_bytes(int R, int N) {
     serl_set_error("rms_norm_bwd: N must be in [1, %d], R >= 0", RMS_MAXN);
     return -1;
   }
-  return (long long)rms_parts(R) * N * 4;
+  const int most = rms_parts(R, N, 8);
+  return (long long)(most > rms_parts(R, N, 4) ? most : rms_parts(R, N, 4)) * N * 4;
 }
 
 extern "C" int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int R, int N, const void* dy, long long lddy,
@@ -378,13 +387,13 @@ extern "C" int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int
   SERL_CHECK_ARG(dweight && (R == 0 || (dy && sum && rstd && weight && dx)), "rms_norm_bwd: null pointer");
   SERL_CHECK_ARG(lddy >= 0 && ldsum >= 0 && ldds >= 0 && (R <= 1 || lddx >= N),
                  "rms_norm_bwd: negative row stride, or output rows overlap");
-  const int parts = rms_parts(R);
-  const long long need = (long long)parts * N * 4;
-  SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
-                 "rms_norm_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
   const int V = type == SERL_F32 ? 4 : 8;
   const bool wide = N % V == 0 && rms_wide(type, V, dy, lddy) && rms_wide(stream_type, V, sum, ldsum) &&
                     rms_wide(stream_type, V, ds, ldds) && rms_wide(stream_type, V, dx, lddx) && sq_aligned(weight, 16);
+  const int parts = rms_parts(R, N, wide ? V : 1);
+  const long long need = (long long)parts * N * 4;
+  SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
+                 "rms_norm_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
   RmsArgs a{};
   a.x = dy; a.ldx = lddy; a.res = sum; a.ldres = ldsum; a.rstd_in = rstd; a.w = weight; a.w_f32 = weight_type == SERL_F32;
   a.ds = ds; a.ldds = ldds; a.y = dx; a.ldy = lddx; a.part = workspace; a.R = R; a.N = N;
