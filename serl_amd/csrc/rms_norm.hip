@@ -3,8 +3,9 @@
 // its backward pass, and the form whose output is 8 bits (OCP e4m3) with one scale per row.  No counterpart in the
 // reference (its networks use LayerNorm, rowops.hip).
 //
-// Bound by memory: a row is read once into registers, reduced, and written; a wave takes a row of up to 1024 16-bit
-// elements (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
+// Bound by memory: a row is read once into registers, reduced, and written; 16 or 32 lanes take a row of up to
+// 16 or 32 vectors of 16 bytes (16: 262144 x 128 bf16 83 -> 42 us, 500000 x 33 both ways 360 -> 128 us against a wave per row), a
+// wave one of up to 128 (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
 // STORED (rounded to the residual's type): later layers and the backward pass see the values that were normed.
 // 16384 x 4096 bf16: forward 82 us (6.5 TB/s: part of it from the caches), backward 110 us (4.9 TB/s) and 5 us for the shares
 // of the weight's gradient; 64 rows to e4m3 4 us.
@@ -23,22 +24,46 @@ struct RmsArgs {
   int R, N, w_f32; float eps;
 };
 
+// Where round i of thread t lies in a row of N columns, VEC apiece.  LOOSE: the row's length is no multiple of VEC, or its rows start
+// at any element; the last vector then moves left to end with the row (N >= VEC), and its first `skip` columns are the left
+// neighbour's, computed twice and counted once.  A column behind the row reads some of its last (or first) ones, not used.
+// Against single elements: 5840 x 4295 fp16 with an fp32 residual 694 -> 57 us, 20000 x 1001
+// bf16 both ways 98 -> 71 us.
+template <int THREADS, int NV, int VEC, bool LOOSE> struct RmsAt {
+  int n, skip;
+  bool in;
+  __device__ __forceinline__ RmsAt(int i, int t, int N) {
+    const int c = (i * THREADS + t) * VEC;
+    const bool whole = i < NV / 2;      // the row has more than NV / 2 rounds: see the choice of the shape
+    in = whole || c < N;
+    n = whole ? c : LOOSE ? min(c, N - VEC) : in ? c : 0;
+    skip = LOOSE ? c - n : 0;
+  }
+  __device__ __forceinline__ bool counts(int v) const { return LOOSE ? v >= skip : in; }
+};
+
 // VEC weights from column n on, in the tensors' own 16-bit type or fp32
-template <typename T, int VEC>
+template <typename T, int VEC, bool LOOSE>
 __device__ __forceinline__ void rms_weight(const RmsArgs& a, int n, float (&w)[VEC]) {
   if (T::code == SERL_F32 || a.w_f32) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) w[v] = ((const float*)a.w)[n + v];
   } else {
     Raw<T, VEC> r;
-    r.load((const typename T::bits*)a.w + n);
+    r.template load<LOOSE>((const typename T::bits*)a.w + n);
     r.get(w);
   }
 }
 
-__device__ __forceinline__ unsigned rms_wave_max(unsigned v) {
+// over a row's lanes of a wave: all of them, or the THREADS of a short row
+template <int THREADS> __device__ __forceinline__ float rms_sum(float v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = (THREADS < 64 ? THREADS : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+template <int THREADS> __device__ __forceinline__ unsigned rms_max(unsigned v) {
+#pragma unroll
+  for (int o = (THREADS < 64 ? THREADS : 64) / 2; o > 0; o >>= 1) {
     const unsigned p = (unsigned)__shfl_xor((int)v, o);
     v = v > p ? v : p;
   }
@@ -53,34 +78,34 @@ __device__ __forceinline__ uint32_t rms_e4m3x4(float a, float b, float c, float 
   return (uint32_t)r;
 }
 
-template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC>
-__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(const RmsArgs a) {
-  constexpr int WAVES = THREADS / 64;
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE>
+__global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_fwd_kernel(const RmsArgs a) {
+  constexpr int WAVES = THREADS <= 64 ? 1 : THREADS / 64;
   __shared__ float red[WAVES];
   __shared__ unsigned redm[WAVES];
   const int t = threadIdx.x % THREADS, wave = t >> 6, lane = t & 63;
-  const int row = THREADS == 64 ? (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) : (int)blockIdx.x;
-  if (THREADS == 64 && row >= a.R) return;
+  const int row = THREADS <= 64 ? (int)(blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS) : (int)blockIdx.x;
+  if (THREADS <= 64 && row >= a.R) return;
   const typename TX::bits* x = (const typename TX::bits*)a.x + row * a.ldx;
   Raw<TX, VEC> rx[NV];
   Raw<TR, VEC> rr[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {        // unconditional: a column behind the row reads the row's first ones, not used
-    const int n = (i * THREADS + t) * VEC;
-    rx[i].load(x + (n < a.N ? n : 0));
+  for (int i = 0; i < NV; ++i) {
+    const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+    rx[i].template load<LOOSE>(x + at.n);
   }
   if (a.res) {
     const typename TR::bits* res = (const typename TR::bits*)a.res + row * a.ldres;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int n = (i * THREADS + t) * VEC;
-      rr[i].load(res + (n < a.N ? n : 0));
+      const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+      rr[i].template load<LOOSE>(res + at.n);
     }
   }
   float s[NV][VEC], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const bool in = (i * THREADS + t) * VEC < a.N;
+    const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
     rx[i].get(s[i]);
     if (a.res) {
       float r[VEC];
@@ -91,17 +116,20 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(
       rr[i].get(s[i]);
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) ss = in ? fmaf(s[i][v], s[i][v], ss) : ss;
+    for (int v = 0; v < VEC; ++v) ss = at.counts(v) ? fmaf(s[i][v], s[i][v], ss) : ss;
   }
-  if (a.sum) {
-    typename TR::bits* sum = (typename TR::bits*)a.sum + row * a.ldsum;
+  const auto put_sum = [&]() {
+    if (a.sum) {
+      typename TR::bits* sum = (typename TR::bits*)a.sum + row * a.ldsum;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int n = (i * THREADS + t) * VEC;
-      if (n < a.N) rr[i].store(sum + n);
+      for (int i = 0; i < NV; ++i) {
+        const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+        if (at.in) rr[i].template store<LOOSE>(sum + at.n);
+      }
     }
-  }
-  ss = sq_wave_sum(ss);
+  };
+  if constexpr (!LOOSE) put_sum();
+  ss = rms_sum<THREADS>(ss);
   if constexpr (WAVES > 1) {
     if (lane == 0) red[wave] = ss;
     __syncthreads();
@@ -109,29 +137,30 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) ss += red[w];
   }
+  if constexpr (LOOSE) put_sum();       // when all have read: sum may be the residual, and two threads read some columns
   const float rstd = rsqrtf(ss / (float)a.N + a.eps);
   if (a.rstd_out && t == 0) a.rstd_out[row] = rstd;
   unsigned top = 0;                     // |y| as bits: ordered like the values, NaN above infinity
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int n = (i * THREADS + t) * VEC;
+    const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
     float w[VEC];
-    rms_weight<TX, VEC>(a, n < a.N ? n : 0, w);
+    rms_weight<TX, VEC, LOOSE>(a, at.n, w);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       s[i][v] = s[i][v] * rstd * w[v];
       if (FP8) {
         const unsigned m = __float_as_uint(s[i][v]) & 0x7fffffffu;
-        top = n < a.N && m > top ? m : top;
+        top = at.in && m > top ? m : top;
       }
     }
-    if (!FP8 && n < a.N) {
+    if (!FP8 && at.in) {
       rx[i].put(s[i]);
-      rx[i].store((typename TX::bits*)a.y + row * a.ldy + n);
+      rx[i].template store<LOOSE>((typename TX::bits*)a.y + row * a.ldy + at.n);
     }
   }
   if constexpr (FP8) {
-    top = rms_wave_max(top);
+    top = rms_max<THREADS>(top);
     if constexpr (WAVES > 1) {
       if (lane == 0) redm[wave] = top;
       __syncthreads();
@@ -145,14 +174,18 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(
     const float inv = 1.f / scale;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int n = (i * THREADS + t) * VEC;
-      unsigned char* q = (unsigned char*)a.y + row * a.ldy + n;
-      if (n < a.N) {
+      const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+      unsigned char* q = (unsigned char*)a.y + row * a.ldy + at.n;
+      if (at.in) {
         if constexpr (VEC == 8) {
-          *(sq_u32x2*)q = (sq_u32x2){rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv),
-                                     rms_e4m3x4(s[i][4] * inv, s[i][5] * inv, s[i][6] * inv, s[i][7] * inv)};
+          const sq_u32x2 c = {rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv),
+                              rms_e4m3x4(s[i][4] * inv, s[i][5] * inv, s[i][6] * inv, s[i][7] * inv)};
+          if constexpr (LOOSE) __builtin_memcpy(q, &c, 8);
+          else *(sq_u32x2*)q = c;
         } else if constexpr (VEC == 4) {
-          *(uint32_t*)q = rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv);
+          const uint32_t c = rms_e4m3x4(s[i][0] * inv, s[i][1] * inv, s[i][2] * inv, s[i][3] * inv);
+          if constexpr (LOOSE) __builtin_memcpy(q, &c, 4);
+          else *(uint32_t*)q = c;
         } else {
           *q = (unsigned char)(rms_e4m3x4(s[i][0] * inv, 0.f, 0.f, 0.f) & 0xffu);
         }
@@ -162,20 +195,23 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_fwd_kernel(
 }
 
 // dx = rstd (w dy - xh mean(w dy xh)) + ds with xh = s rstd; dw = sum over rows of dy xh.  A workgroup (THREADS = 64: a
-// wave) takes every gridDim-th row and keeps its share of dw in registers; the shares are added in a fixed order by
+// wave, less: that many lanes) takes every gridDim-th row and keeps its share of dw in registers; the shares are added in a fixed order by
 // rms_dw_kernel, so the result does not depend on timing.
-template <typename TY, typename TS, int THREADS, int NV, int VEC>
-__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_bwd_kernel(const RmsArgs a) {
-  constexpr int WAVES = THREADS / 64;
+template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE>
+__global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_bwd_kernel(const RmsArgs a) {
+  constexpr int WAVES = THREADS <= 64 ? 1 : THREADS / 64;
   __shared__ float red[2][WAVES];
   const int t = threadIdx.x % THREADS, wave = t >> 6, lane = t & 63;
-  const int first = THREADS == 64 ? (int)(blockIdx.x * 4 + (threadIdx.x >> 6)) : (int)blockIdx.x;
-  const int step = THREADS == 64 ? (int)gridDim.x * 4 : (int)gridDim.x;
-  float w[NV][VEC], dw[NV][VEC];
+  const int first = THREADS <= 64 ? (int)(blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS) : (int)blockIdx.x;
+  const int step = THREADS <= 64 ? (int)gridDim.x * (256 / THREADS) : (int)gridDim.x;
+  // The weights stay in registers, and ds is fetched with the rest; with 32 columns per thread they would not fit the 128
+  // registers, so both are read where they are used, the weights twice a row (from the L2).  2048 x 32768 bf16 383 -> 356 us.
+  constexpr bool HOLD = THREADS < 1024 || NV * VEC <= 16;
+  float w[HOLD ? NV : 1][VEC], dw[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int n = (i * THREADS + t) * VEC;
-    rms_weight<TY, VEC>(a, n < a.N ? n : 0, w[i]);
+    const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+    if (HOLD) rms_weight<TY, VEC, LOOSE>(a, at.n, w[HOLD ? i : 0]);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) dw[i][v] = 0.f;
   }
@@ -186,35 +222,36 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_bwd_kernel(
     const typename TS::bits* ds = (const typename TS::bits*)a.ds + row * a.ldds;
     const float rstd = a.rstd_in[row];
     Raw<TY, VEC> ry[NV];
-    Raw<TS, VEC> rs[NV], rd[NV];
+    Raw<TS, VEC> rs[NV], rd[HOLD ? NV : 1];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int n = (i * THREADS + t) * VEC, m = n < a.N ? n : 0;
-      ry[i].load(dy + m);
-      rs[i].load(s + m);
+      const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+      ry[i].template load<LOOSE>(dy + at.n);
+      rs[i].template load<LOOSE>(s + at.n);
     }
-    if (a.ds) {
+    if (HOLD && a.ds) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int n = (i * THREADS + t) * VEC;
-        rd[i].load(ds + (n < a.N ? n : 0));
+        const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+        rd[HOLD ? i : 0].template load<LOOSE>(ds + at.n);
       }
     }
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const bool in = (i * THREADS + t) * VEC < a.N;
+      const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
       float y[VEC], x[VEC];
+      if (!HOLD) rms_weight<TY, VEC, LOOSE>(a, at.n, w[0]);
       ry[i].get(y);
       rs[i].get(x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
         const float d = y[v] * (x[v] * rstd);
         dw[i][v] += d;
-        dot = in ? fmaf(w[i][v], d, dot) : dot;
+        dot = at.counts(v) ? fmaf(w[HOLD ? i : 0][v], d, dot) : dot;
       }
     }
-    dot = sq_wave_sum(dot);
+    dot = rms_sum<THREADS>(dot);
     if constexpr (WAVES > 1) {
       if (lane == 0) red[buf][wave] = dot;
       __syncthreads();
@@ -225,26 +262,39 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void rms_bwd_kernel(
     dot /= (float)a.N;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int n = (i * THREADS + t) * VEC;
+      const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
       float y[VEC], x[VEC], d[VEC];
+      if (!HOLD) rms_weight<TY, VEC, LOOSE>(a, at.n, w[0]);
+      if (!HOLD && a.ds) rd[0].template load<LOOSE>(ds + at.n);
+      sq_again(ry[i]);
+      sq_again(rs[i]);
       ry[i].get(y);
       rs[i].get(x);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) d[v] = 0.f;
-      if (a.ds) rd[i].get(d);
+      if (a.ds) rd[HOLD ? i : 0].get(d);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) d[v] = fmaf(rstd, fmaf(-(x[v] * rstd), dot, y[v] * w[i][v]), d[v]);
+      for (int v = 0; v < VEC; ++v) d[v] = fmaf(rstd, fmaf(-(x[v] * rstd), dot, y[v] * w[HOLD ? i : 0][v]), d[v]);
       rs[i].put(d);
-      if (n < a.N) rs[i].store((typename TS::bits*)a.y + row * a.ldy + n);
+      if (at.in) rs[i].template store<LOOSE>((typename TS::bits*)a.y + row * a.ldy + at.n);
     }
   }
-  float* part = a.part + (long long)first * a.N;
+  if constexpr (THREADS < 64) {          // the wave's rows side by side
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+#pragma unroll
+        for (int o = THREADS; o < 64; o <<= 1) dw[i][v] += __shfl_xor(dw[i][v], o);
+    if (lane >= THREADS) return;
+  }
+  float* part = a.part + (long long)(THREADS < 64 ? blockIdx.x * 4 + (threadIdx.x >> 6) : first) * a.N;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int n = (i * THREADS + t) * VEC;
-    if (n < a.N)
+    const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
+    if (at.in)
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) part[n + v] = dw[i][v];
+      for (int v = 0; v < VEC; ++v) part[at.n + v] = dw[i][v];
   }
 }
 
@@ -268,61 +318,75 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(const float* part, int par
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
-template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC>
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE>
 static void rms_go_fwd(const RmsArgs& a, hipStream_t st) {
-  const unsigned grid = THREADS == 64 ? (unsigned)cdiv(a.R, 4) : (unsigned)a.R;
-  hipLaunchKernelGGL((rms_fwd_kernel<TX, TR, FP8, THREADS, NV, VEC>), dim3(grid), dim3(THREADS == 64 ? 256 : THREADS), 0, st, a);
+  const unsigned grid = THREADS <= 64 ? (unsigned)cdiv(a.R, 256 / THREADS) : (unsigned)a.R;
+  hipLaunchKernelGGL((rms_fwd_kernel<TX, TR, FP8, THREADS, NV, VEC, LOOSE>), dim3(grid), dim3(THREADS <= 64 ? 256 : THREADS), 0, st, a);
+}
+template <typename TX, typename TR, bool FP8, bool LOOSE>
+static void rms_shape_fwd(const RmsArgs& a, hipStream_t st) {
+  constexpr int V = TX::code == SERL_F32 ? 4 : 8;
+  const int n = cdiv(a.N, V);          // vectors of a row; more than half of those of a shape with several rounds (RmsAt)
+  if (n <= 16) rms_go_fwd<TX, TR, FP8, 16, 1, V, LOOSE>(a, st);
+  else if (n <= 32) rms_go_fwd<TX, TR, FP8, 32, 1, V, LOOSE>(a, st);
+  else if (n <= 64) rms_go_fwd<TX, TR, FP8, 64, 1, V, LOOSE>(a, st);
+  else if (n <= 128) rms_go_fwd<TX, TR, FP8, 64, 2, V, LOOSE>(a, st);
+  else if (n <= 256) rms_go_fwd<TX, TR, FP8, 256, 1, V, LOOSE>(a, st);
+  else if (n <= 512) rms_go_fwd<TX, TR, FP8, 256, 2, V, LOOSE>(a, st);
+  else if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, V, LOOSE>(a, st);
+  else if (n <= 2048) rms_go_fwd<TX, TR, FP8, 1024, 2, V, LOOSE>(a, st);
+  else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 1024, 4, V, LOOSE>(a, st);
+  else if constexpr (TX::code == SERL_F32) rms_go_fwd<TX, TR, FP8, 1024, 8, V, LOOSE>(a, st);      // RMS_MAXN elements
 }
 template <typename TX, typename TR, bool FP8>
 static void rms_pick_fwd(const RmsArgs& a, bool wide, hipStream_t st) {
-  constexpr int V = TX::code == SERL_F32 ? 4 : 8;
-  const int n = cdiv(a.N, wide ? V : 1);          // vectors of a row
-  if (!wide) {
-    if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, 1>(a, st);
-    else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 256, 16, 1>(a, st);
-    else rms_go_fwd<TX, TR, FP8, 1024, 32, 1>(a, st);
-  } else if (n <= 64) rms_go_fwd<TX, TR, FP8, 64, 1, V>(a, st);
-  else if (n <= 128) rms_go_fwd<TX, TR, FP8, 64, 2, V>(a, st);
-  else if (n <= 256) rms_go_fwd<TX, TR, FP8, 256, 1, V>(a, st);
-  else if (n <= 512) rms_go_fwd<TX, TR, FP8, 256, 2, V>(a, st);
-  else if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, V>(a, st);
-  else if (n <= 2048) rms_go_fwd<TX, TR, FP8, 1024, 2, V>(a, st);
-  else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 1024, 4, V>(a, st);
-  else rms_go_fwd<TX, TR, FP8, 1024, 8, V>(a, st);      // fp32 only: RMS_MAXN elements
+  if (wide) rms_shape_fwd<TX, TR, FP8, false>(a, st);
+  else if (a.N >= (TX::code == SERL_F32 ? 4 : 8)) rms_shape_fwd<TX, TR, FP8, true>(a, st);
+  else rms_go_fwd<TX, TR, FP8, 16, 1, 1, false>(a, st);      // a row of less than a vector
 }
 
-// Rows of the partial weight gradients: one per row of the input, at most RMS_PARTS (one per workgroup).  Short rows get more, as
-// many as keep the partial sums at 8 MB: 131072 x 512 bf16 355 -> 207 us both ways, 20000 x 1536 99 -> 88 us; longer ones, or
-// narrow loads, lose by it (32768 x 2048 with 2048 parts 193 -> 210 us, 5000 x 1001 fp32 39 -> 42 us).  vec: elements per access.
+// Rows of the partial weight gradients: one per row of the input (rounded up to 4), at most RMS_PARTS, one per workgroup or, for
+// short rows, per wave.  Short rows get more, as many as keep the partial sums at 8 MB and 8 rows to each: 131072 x 512 bf16
+// 355 -> 207 us both ways, 20000 x 1536 99 -> 84 us; but without the 8 rows 5000 x 1001 fp32 36 -> 39 us, and longer rows lose by
+// it (32768 x 2048 with 2048 parts 193 -> 210 us).  A workgroup of 1024 threads has a CU to itself, so 256 parts: 2048 x 32768
+// bf16 356 -> 324 us.  vec: elements per access.
 static int rms_parts(int R, int N, int vec) {
   const int n = cdiv(N, vec);
-  int most = vec > 1 && n <= 128 ? (1 << 21) / N : vec > 1 && n <= 256 ? (3 << 19) / N : RMS_PARTS;
-  most = (most < RMS_PARTS ? RMS_PARTS : most > RMS_MOSTPARTS ? RMS_MOSTPARTS : most) / 4 * 4;
+  int most = n <= 128 ? (1 << 21) / N : n <= 256 ? (3 << 19) / N : n <= 1024 ? RMS_PARTS : RMS_PARTS / 2;
+  if (n <= 256) {
+    most = most > RMS_MOSTPARTS ? RMS_MOSTPARTS : most;
+    most = most > R / 8 ? R / 8 : most;
+    most = most < RMS_PARTS ? RMS_PARTS : most / 4 * 4;
+  }
   return R < most ? (R + 3) / 4 * 4 : most;
 }
 
-template <typename TY, typename TS, int THREADS, int NV, int VEC>
+template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE>
 static void rms_go_bwd(const RmsArgs& a, hipStream_t st) {
-  const int parts = rms_parts(a.R, a.N, VEC);
-  hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC>), dim3(THREADS == 64 ? parts / 4 : parts),
-                     dim3(THREADS == 64 ? 256 : THREADS), 0, st, a);
+  const int parts = rms_parts(a.R, a.N, TY::code == SERL_F32 ? 4 : 8);
+  hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC, LOOSE>), dim3(THREADS <= 64 ? parts / 4 : parts),
+                     dim3(THREADS <= 64 ? 256 : THREADS), 0, st, a);
+}
+template <typename TY, typename TS, bool LOOSE>
+static void rms_shape_bwd(const RmsArgs& a, hipStream_t st) {
+  constexpr int V = TY::code == SERL_F32 ? 4 : 8;
+  const int n = cdiv(a.N, V);          // as in rms_shape_fwd
+  if (n <= 16) rms_go_bwd<TY, TS, 16, 1, V, LOOSE>(a, st);
+  else if (n <= 32) rms_go_bwd<TY, TS, 32, 1, V, LOOSE>(a, st);
+  else if (n <= 64) rms_go_bwd<TY, TS, 64, 1, V, LOOSE>(a, st);
+  else if (n <= 128) rms_go_bwd<TY, TS, 64, 2, V, LOOSE>(a, st);
+  else if (n <= 256) rms_go_bwd<TY, TS, 256, 1, V, LOOSE>(a, st);
+  else if (n <= 512) rms_go_bwd<TY, TS, 256, 2, V, LOOSE>(a, st);
+  else if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, V, LOOSE>(a, st);
+  else if (n <= 2048) rms_go_bwd<TY, TS, 1024, 2, V, LOOSE>(a, st);
+  else if (n <= 4096) rms_go_bwd<TY, TS, 1024, 4, V, LOOSE>(a, st);
+  else if constexpr (TY::code == SERL_F32) rms_go_bwd<TY, TS, 1024, 8, V, LOOSE>(a, st);
 }
 template <typename TY, typename TS>
 static void rms_pick_bwd(const RmsArgs& a, bool wide, hipStream_t st) {
-  constexpr int V = TY::code == SERL_F32 ? 4 : 8;
-  const int n = cdiv(a.N, wide ? V : 1);
-  if (!wide) {
-    if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, 1>(a, st);
-    else if (n <= 4096) rms_go_bwd<TY, TS, 256, 16, 1>(a, st);
-    else rms_go_bwd<TY, TS, 1024, 32, 1>(a, st);
-  } else if (n <= 64) rms_go_bwd<TY, TS, 64, 1, V>(a, st);
-  else if (n <= 128) rms_go_bwd<TY, TS, 64, 2, V>(a, st);
-  else if (n <= 256) rms_go_bwd<TY, TS, 256, 1, V>(a, st);
-  else if (n <= 512) rms_go_bwd<TY, TS, 256, 2, V>(a, st);
-  else if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, V>(a, st);
-  else if (n <= 2048) rms_go_bwd<TY, TS, 1024, 2, V>(a, st);
-  else if (n <= 4096) rms_go_bwd<TY, TS, 1024, 4, V>(a, st);
-  else rms_go_bwd<TY, TS, 1024, 8, V>(a, st);
+  if (wide) rms_shape_bwd<TY, TS, false>(a, st);
+  else if (a.N >= (TY::code == SERL_F32 ? 4 : 8)) rms_shape_bwd<TY, TS, true>(a, st);
+  else rms_go_bwd<TY, TS, 16, 1, 1, false>(a, st);
 }
 
 static bool rms_wide(int type, int elems, const void* p, long long ld) {
@@ -390,7 +454,7 @@ extern "C" int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int
   const int V = type == SERL_F32 ? 4 : 8;
   const bool wide = N % V == 0 && rms_wide(type, V, dy, lddy) && rms_wide(stream_type, V, sum, ldsum) &&
                     rms_wide(stream_type, V, ds, ldds) && rms_wide(stream_type, V, dx, lddx) && sq_aligned(weight, 16);
-  const int parts = rms_parts(R, N, wide ? V : 1);
+  const int parts = rms_parts(R, N, V);
   const long long need = (long long)parts * N * 4;
   SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                  "rms_norm_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);

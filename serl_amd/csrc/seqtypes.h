@@ -43,14 +43,23 @@ template <> __device__ __forceinline__ uint32_t sq_pack2<F16>(float a, float b) 
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((sq_f32x2){a, b}, sq_f16x2));
 }
 
-// VEC consecutive elements of type T as they lie in memory (VEC * size = a power of two of bytes, naturally aligned; VEC = 1: one element)
+// VEC consecutive elements of type T as they lie in memory (VEC * size = a power of two of bytes, naturally aligned; LOOSE: at any
+// element, the same instructions, which the hardware takes at any address; VEC = 1: one element)
 template <typename T, int VEC> struct Raw {
   static constexpr int BYTES = VEC * (int)sizeof(typename T::bits);
   static constexpr int W = BYTES / 4;
   static_assert(BYTES % 4 == 0, "whole dwords");
   uint32_t w[W];
-  __device__ __forceinline__ void load(const typename T::bits* p) {
-    if constexpr (W % 4 == 0) {
+  template <bool LOOSE = false> __device__ __forceinline__ void load(const typename T::bits* p) {
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        sq_u32x4 v = {};
+        __builtin_memcpy(&v, (const char*)p + 4 * i, W < 4 ? BYTES : 16);
+#pragma unroll
+        for (int j = 0; j < 4 && i + j < W; ++j) w[i + j] = v[j];
+      }
+    } else if constexpr (W % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
         const sq_u32x4 v = reinterpret_cast<const sq_u32x4*>(p)[i];
@@ -64,8 +73,16 @@ template <typename T, int VEC> struct Raw {
       w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
   }
-  __device__ __forceinline__ void store(typename T::bits* p) const {
-    if constexpr (W % 4 == 0) {
+  template <bool LOOSE = false> __device__ __forceinline__ void store(typename T::bits* p) const {
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        sq_u32x4 v = {};
+#pragma unroll
+        for (int j = 0; j < 4 && i + j < W; ++j) v[j] = w[i + j];
+        __builtin_memcpy((char*)p + 4 * i, &v, W < 4 ? BYTES : 16);
+      }
+    } else if constexpr (W % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < W / 4; ++i)
         reinterpret_cast<sq_u32x4*>(p)[i] = (sq_u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
@@ -96,8 +113,8 @@ template <typename T, int VEC> struct Raw {
 };
 template <typename T> struct Raw<T, 1> {
   typename T::bits w;
-  __device__ __forceinline__ void load(const typename T::bits* p) { w = *p; }
-  __device__ __forceinline__ void store(typename T::bits* p) const { *p = w; }
+  template <bool LOOSE = false> __device__ __forceinline__ void load(const typename T::bits* p) { w = *p; }
+  template <bool LOOSE = false> __device__ __forceinline__ void store(typename T::bits* p) const { *p = w; }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = sq_val(T(), w); }
   __device__ __forceinline__ void put(const float (&v)[1]) { w = sq_bits(T(), v[0]); }
 };

@@ -351,24 +351,44 @@ def check_norm(i, dtype, eps=1e-6):
         dyw, xh = i["dy"].double().cpu() * w, v * r
         size = r * (dyw.abs() + xh.abs() * (dyw * xh).abs().mean(1, keepdim=True)) + (0 if ds is None else add.abs())
         within(dx, rx + add, 2 * (NORM_Y + 54 * U) * size + HALF[dx.dtype] * (rx + add).abs() + SMALL, "dx")
-        # a share adds R / 512 rows, a lane of the last step 16 shares, then 32 lanes
-        within(dw, rw, (R / 512 + 52 + NORM_Y / U) * U * (i["dy"].double().cpu() * xh).abs().sum(0) + 1e-30, "dweight")
+        # at least 512 shares (256 for R < 512), or one per row: a share adds up to R / 256 rows and four lanes; the last step's lanes
+        # up to 16 shares, with more than 512 shares no more than R / 8 / 32; then 32 lanes
+        within(dw, rw, (R / 128 + 52 + NORM_Y / U) * U * (i["dy"].double().cpu() * xh).abs().sum(0) + 1e-30, "dweight")
 
 
 @pytest.mark.parametrize("dtype,stream", [(torch.float32, None), (torch.float32, torch.float32), (torch.bfloat16, None),
                                           (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
                                           (torch.float16, torch.float16), (torch.float16, torch.float32)], ids=str)
 def test_rms_norm_matches_its_formulas(dev, dtype, stream):
-    for R, N in ((1, 1), (3, 7), (5, 64), (1, 512), (6, 520), (2, 1000), (3, 1001), (2, 1024), (3, 2048), (2, 2056), (5, 4096),
+    for R, N in ((1, 1), (3, 7), (70, 3), (3, 8), (4, 9), (5, 64), (1, 512), (6, 520), (2, 1000), (3, 1001), (2, 1024), (3, 2048),
+                 (2, 2056), (5, 4096),
                  (2, 4097), (3, 8192), (1, 12288), (2, 16384), (1, 20000), (2, 32767), (1, 32768)):
         check_norm(norm_inputs(dev, dtype, stream, R, N, R + N), dtype)
     check_norm(norm_inputs(dev, dtype, stream, 3, 264, 1, wtype=torch.float32), dtype, eps=0.5)
 
 
-@pytest.mark.parametrize("R,N", [(513, 40), (2051, 33), (700, 1100), (1030, 2064)])
+@pytest.mark.parametrize("R,N", [(513, 40), (2051, 33), (700, 1100), (1030, 2064), (70001, 5), (33000, 128), (5001, 249), (9000, 333),
+                                 (300, 9001)])
 def test_rms_norm_many_rows(dev, R, N):
     for dtype in (torch.float32, torch.bfloat16):
         check_norm(norm_inputs(dev, dtype, dtype, R, N, R), dtype)
+
+
+# rows that start at any element, NaN around them: each shape of the kernel with its last vector moved left
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)],
+                         ids=str)
+def test_rms_norm_rows_at_any_element(dev, dtype, stream):
+    for R, N in ((9, 8), (7, 61), (5, 130), (6, 257), (3, 777), (2, 1030), (3, 2047), (2, 4101), (3, 8193), (2, 16390), (2, 32761)):
+        i = norm_inputs(dev, dtype, stream, R, N, R * N)
+        for off, pad in ((1, 2), (4, 4)):
+            for k in ("x", "residual", "dy", "ds"):
+                big = torch.full((R, off + N + pad), float("nan"), dtype=i[k].dtype, device=dev)
+                big[:, off:off + N] = i[k]
+                i[k] = big[:, off:off + N]
+            w = torch.full((N + off,), float("nan"), dtype=i["weight"].dtype, device=dev)
+            w[off:] = i["weight"]
+            i["weight"] = w[off:]
+            check_norm(i, dtype)
 
 
 def test_rms_norm_views_shapes_and_empty_rows(dev):
