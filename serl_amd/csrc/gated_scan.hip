@@ -545,6 +545,9 @@ struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
 // channels alone leave half of the CUs idle and there are more than 5 tiles.  bf16 forward: 8 x 4000 x 1024 (128 workgroups) 85 ->
 // 68 us; but 12 x 4000 x 1024 (192) 89 -> 132 us, 4 x 512 x 1024 (4 tiles) 11.9 -> 16 us; both ways: 9 x 2000 x 1024 (144) 117 ->
 // 128 us, 12 x 777 x 333 fp32 (132) 52 -> 44 us.
+// How many pieces: a CU holds two workgroups of the forward kernels, one of the backward, so what counts is the rounds of 512 and
+// 256 workgroups, times the tiles of a piece and three quarters of one for its start and end.  Against 512 workgroups or more
+// whatever the rounds, both ways bf16: 1 x 24576 x 2424 468 -> 357 us, 6 x 4000 x 1024 179 -> 150, 6 x 10127 x 83 76 -> 61.
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
   p.vec = wide ? 4 : 1;
@@ -554,8 +557,16 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
   if (blocks <= 136 && T > 5 * SCAN_CKPT) {
-    const int want = (int)cdivll(512, blocks);
-    p.seg_len = cdiv(cdiv(T, want < SCAN_MAXSEG ? want : SCAN_MAXSEG), SCAN_CKPT) * SCAN_CKPT;
+    const int tiles = cdiv(T, SCAN_CKPT);
+    long long best = 0;
+    for (int want = SCAN_MAXSEG; want > 1; --want) {
+      const int n = cdiv(tiles, want);      // tiles of a piece
+      const long long w = blocks * cdiv(tiles, n), cost = (4ll * n + 3) * (2 * cdivll(w, 512) + cdivll(w, 256));
+      if (!best || cost <= best) {
+        best = cost;
+        p.seg_len = n * SCAN_CKPT;
+      }
+    }
     p.nseg = cdiv(T, p.seg_len);
   }
   return p;
