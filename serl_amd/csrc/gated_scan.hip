@@ -605,33 +605,35 @@ static bool scan_rows(int type, int bytes, const void* p, long long bs, long lon
 // elements), so it only takes 4 channels.
 static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_reach(type, true, D, ts); }
 
-// Tiles of 128 steps (a kept state in front of each), of 64 where no sequence is longer: 16 elements per thread.  Wide: 128
-// bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32 elements per thread 10 to
-// 20 %: registers).
+// Tiles of 128 steps (a kept state in front of each), of 16, 32 or 64 where no sequence is longer: 16 (fp32: up to 64 steps 8)
+// elements per thread.  Wide: 128 bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32
+// elements per thread 10 to 20 %: registers).  Both ways bf16, tile of 64 -> smaller:
+// 256 x 16 x 1024 57 -> 28 us, 181 x 24 x 1536 61 -> 36, 1024 x 10 x 512 106 -> 31.
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
+#define SCAN_LONG(KERNEL, ...)                                                          \
+  do {                                                                                  \
+    if (p.vec == 1) SCAN_GO(KERNEL, 1, 64, 8, 1024, ##__VA_ARGS__);                     \
+    else if constexpr (T::code == SERL_F32) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__); \
+    else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                                 \
+  } while (0)
 #define SCAN_PICK(KERNEL, ...)                                                          \
   do {                                                                                  \
-    if (p.vec == 1) {                                                                   \
-      if (a.T <= 64) SCAN_GO(KERNEL, 1, 64, 8, 512, ##__VA_ARGS__);                     \
-      else SCAN_GO(KERNEL, 1, 64, 8, 1024, ##__VA_ARGS__);                               \
-    } else if constexpr (T::code == SERL_F32) {                                         \
-      if (a.T <= 64) SCAN_GO(KERNEL, 4, 8, 2, 256, ##__VA_ARGS__);                      \
-      else SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);                                \
-    } else {                                                                            \
-      if (a.T <= 64) SCAN_GO(KERNEL, 4, 16, 4, 256, ##__VA_ARGS__);                     \
-      else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                               \
-    }                                                                                   \
+    constexpr int C = T::code == SERL_F32 ? 8 : 16, L = T::code == SERL_F32 ? 2 : 4;    \
+    if (p.vec == 1 || a.T > 64) SCAN_LONG(KERNEL, ##__VA_ARGS__);                       \
+    else if (a.T > 32) SCAN_GO(KERNEL, 4, C, L, 256, ##__VA_ARGS__);                    \
+    else if (a.T > 16) SCAN_GO(KERNEL, 4, C, L, 128, ##__VA_ARGS__);                    \
+    else SCAN_GO(KERNEL, 4, C, L, 64, ##__VA_ARGS__);                                   \
   } while (0)
 template <typename T>
 static void scan_launch_fwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
-  if (a.nseg > 1) SCAN_PICK(scan_fwd_kernel, true);
+  if (a.nseg > 1) SCAN_LONG(scan_fwd_kernel, true);
   SCAN_PICK(scan_fwd_kernel, false);
 }
 template <typename T>
 static void scan_launch_bwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
-  if (a.nseg > 1) SCAN_PICK(scan_bwd_summary_kernel);
+  if (a.nseg > 1) SCAN_LONG(scan_bwd_summary_kernel);
   SCAN_PICK(scan_bwd_kernel);
 }
 template <typename T>
