@@ -5,7 +5,7 @@
 //
 // The recurrence is an affine map h -> k h + b per step (k = f, or 0 at the start of an episode, or the identity behind
 // a sequence's length), and maps compose: (k2, b2) o (k1, b1) = (k1 k2, k2 b1 + b2).  A workgroup takes one sequence and 128
-// bytes of channels (a cache line per row; 64 bytes were 10 % slower) and walks through time in tiles of 128 steps: a thread
+// bytes of channels (a cache line per row; 64 bytes were 10 % slower) and walks through time in tiles of up to 128 steps: a thread
 // reads 4 channels of 4 consecutive steps, composes them, the maps of the threads of a channel are joined by wave shuffles and,
 // between the waves, through LDS (one barrier per direction and tile), and each thread then runs its steps from the state that
 // reaches it.  Every input is read once and every output written once; the next tile's loads are issued before the current tile
@@ -15,7 +15,8 @@
 // forward 94 us (4.3 TB/s where a large copy reaches 5.2), backward 163 us (4.1 TB/s).
 #include "seqtypes.h"
 
-#define SCAN_CKPT 128       // steps between the states that the forward pass keeps for the backward pass
+#define SCAN_CKPT 64        // steps between the states that the forward pass keeps for the backward pass
+#define SCAN_TILE 128       // steps of a tile where the time axis may be split
 #define SCAN_THREADS 256    // of the kernel for a few steps
 #define SCAN_MAXD (1 << 26)  // channels
 #define SCAN_MAXSEG 32      // most pieces the time axis is split into
@@ -29,7 +30,7 @@ struct ScanArgs {
   float *h_last, *dh0;                                       // (B, D)
   const unsigned char* starts; long long starts_bs;          // (B, T) bytes or null
   const int* lengths;                                        // (B) or null
-  float *ckpt;                                               // (B, ceil(T / 128), D) or null
+  float *ckpt;                                               // (B, ceil(T / 64), D) or null
   float *seg;                                                // (B, nseg, 2, D): the maps of the pieces, nseg > 1 only
   int B, T, D, ndb, nseg, seg_len;                           // channel blocks; pieces of the time axis and their length
   int share;                                                 // rows start inside cache lines
@@ -556,15 +557,15 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   p.nseg = 1;
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
-  if (blocks <= 136 && T > 5 * SCAN_CKPT) {
-    const int tiles = cdiv(T, SCAN_CKPT);
+  if (blocks <= 136 && T > 5 * SCAN_TILE) {
+    const int tiles = cdiv(T, SCAN_TILE);
     long long best = 0;
     for (int want = SCAN_MAXSEG; want > 1; --want) {
       const int n = cdiv(tiles, want);      // tiles of a piece
       const long long w = blocks * cdiv(tiles, n), cost = (4ll * n + 3) * (2 * cdivll(w, 512) + cdivll(w, 256));
       if (!best || cost <= best) {
         best = cost;
-        p.seg_len = n * SCAN_CKPT;
+        p.seg_len = n * SCAN_TILE;
       }
     }
     p.nseg = cdiv(T, p.seg_len);
@@ -605,10 +606,11 @@ static bool scan_rows(int type, int bytes, const void* p, long long bs, long lon
 // elements), so it only takes 4 channels.
 static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_reach(type, true, D, ts); }
 
-// Tiles of 128 steps (a kept state in front of each), of 16, 32 or 64 where no sequence is longer: 16 (fp32: up to 64 steps 8)
-// elements per thread.  Wide: 128 bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32
-// elements per thread 10 to 20 %: registers).  Both ways bf16, tile of 64 -> smaller:
-// 256 x 16 x 1024 57 -> 28 us, 181 x 24 x 1536 61 -> 36, 1024 x 10 x 512 106 -> 31.
+// Tiles of 128 steps, of 16, 32 or 64 where no sequence is longer: 16 (fp32: up to 64 steps 8) elements per thread.  Wide: 128
+// bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32 elements per thread 10 to 20 %:
+// registers).  Both ways bf16, tile of 64 -> smaller: 256 x 16 x 1024 57 -> 28 us, 181 x 24 x 1536 61 -> 36, 1024 x 10 x 512
+// 106 -> 31.  16-bit types with two workgroups per CU to spare stay with 64 steps, half of which wait while the others work: both
+// ways 256 x 130 x 1024 229 -> 164 us, 64 x 400 x 1024 124 -> 110; with fewer the larger tile is needed to keep enough loads in flight (8 x 4096 x 2048 264 against 344 us).
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
 #define SCAN_LONG(KERNEL, ...)                                                          \
   do {                                                                                  \
@@ -618,8 +620,9 @@ static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_rea
   } while (0)
 #define SCAN_PICK(KERNEL, ...)                                                          \
   do {                                                                                  \
+    const bool half = T::code != SERL_F32 && (long long)a.B * a.ndb >= 512;           \
     constexpr int C = T::code == SERL_F32 ? 8 : 16, L = T::code == SERL_F32 ? 2 : 4;    \
-    if (p.vec == 1 || a.T > 64) SCAN_LONG(KERNEL, ##__VA_ARGS__);                       \
+    if (p.vec == 1 || (a.T > 64 && !half)) SCAN_LONG(KERNEL, ##__VA_ARGS__);            \
     else if (a.T > 32) SCAN_GO(KERNEL, 4, C, L, 256, ##__VA_ARGS__);                    \
     else if (a.T > 16) SCAN_GO(KERNEL, 4, C, L, 128, ##__VA_ARGS__);                    \
     else SCAN_GO(KERNEL, 4, C, L, 64, ##__VA_ARGS__);                                   \

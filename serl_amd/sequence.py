@@ -131,7 +131,7 @@ def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
         code, dev = _CODES[gate.dtype], gate.device
         y = torch.empty_like(gate, memory_format=_ROWS)
         h_last = gate.new_empty((B, D), dtype=torch.float32)
-        saved = gate.new_empty((B, -(-T // 128), D), dtype=torch.float32) if save else None
+        saved = gate.new_empty((B, -(-T // 64), D), dtype=torch.float32) if save else None
         ws, nws = _scan_scratch(code, B, T, D, dev)
         ops.gated_scan_fwd(code, B, T, D, gate.data_ptr(), gate.stride(0), gate.stride(1), x.data_ptr(), x.stride(0),
                            x.stride(1), _ptr(h0), _ptr(starts), 0 if starts is None else starts.stride(0), _ptr(lengths),
@@ -144,7 +144,7 @@ def gated_scan_backward(gate, x, saved, dy, dh_last=None, starts=None, lengths=N
     forward call; dy (B, T, D), dh_last (B, D) float32 or None.  out: (dgate, dx) tensors to write, for instance the two
     halves of one projection's gradient; they share no memory with the inputs."""
     B, T, D = _scan_args(gate, x, starts, lengths)
-    _shape(saved, "saved", (B, -(-T // 128), D))
+    _shape(saved, "saved", (B, -(-T // 64), D))
     _type(saved, "saved", torch.float32)
     _shape(dy, "dy", (B, T, D))
     _type(dy, "dy", gate.dtype)

@@ -74,7 +74,7 @@ def test_gated_scan_entry_point_refusals():
     with pytest.raises(ValueError, match="bad sizes"):
         ops.gated_scan_states_floats(1, -1, 1)
     assert ops.gated_scan_workspace_bytes(1, 8, 4096, 2048) == 0
-    assert ops.gated_scan_states_floats(2, 129, 8) == 2 * 2 * 8
+    assert ops.gated_scan_states_floats(2, 129, 8) == 2 * 3 * 8
     bwd = lambda **k: ops.gated_scan_bwd(*{**dict(  # noqa: E731
         dtype=0, B=2, T=5, D=8, gate=16, gate_bs=40, gate_ts=8, x=16, x_bs=40, x_ts=8, starts=None, starts_bs=0, lengths=None,
         states=16, dy=16, dy_bs=40, dy_ts=8, dh_last=None, dgate=16, dgate_bs=40, dgate_ts=8, dx=16, dx_bs=40, dx_ts=8, dh0=16,
