@@ -10,11 +10,12 @@
 // stores overlap.  Few long rows, and rows too long for registers, are cut into pieces of their own workgroups: one launch
 // for the statistics, one that joins them and writes the gradient (it reads the row again, from the caches where they hold it).
 //
-// 2048 x 131072 bf16, 128 slots: 242 us (4.45 TB/s where a large copy reaches 5.2; the first load and the last store of a
+// 2048 x 131072 bf16, 128 slots: 225 us (4.8 TB/s where a large copy reaches 5.2; the first load and the last store of a
 // workgroup's eight rows overlap nothing, and the vector ALU is half busy with two exponentials per column).
 //
 // Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
-// single threads (`head` and `tail`).  The teacher's columns are stored a second time, behind a barrier that all dense
+// single threads (`head` and `tail`); the gradient is stored in the logits' pieces, which may lie at any element of its rows
+// (against single elements where the two differ, 1500 x 50021 165 -> 75 us).  The teacher's columns are stored a second time, behind a barrier that all dense
 // stores of the row have passed.
 #include "seqtypes.h"
 
@@ -66,13 +67,14 @@ template <int VEC> __device__ __forceinline__ float dist_max(float m, const floa
 }
 
 // piece j of a row's whole pieces (`base`: the first one): a uniform address and a 32-bit offset per thread
-template <typename T, int VEC>
+template <bool STREAM = false, typename T, int VEC>
 __device__ __forceinline__ void dist_load(Raw<T, VEC>& r, const typename T::bits* base, int j) {
-  r.load((const typename T::bits*)((const char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
+  r.template load<false, STREAM>((const typename T::bits*)((const char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
 }
-template <typename T, int VEC>
+// (the gradient's rows may lie otherwise than the logits': at any element)
+template <bool STREAM = false, typename T, int VEC>
 __device__ __forceinline__ void dist_store(const Raw<T, VEC>& r, typename T::bits* base, int j) {
-  r.store((typename T::bits*)((char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
+  r.template store<!STREAM, STREAM>((typename T::bits*)((char*)base + (uint32_t)j * (uint32_t)(VEC * sizeof(typename T::bits))));
 }
 
 template <typename T> __device__ __forceinline__ uint32_t dist_minus_inf() {
@@ -187,7 +189,7 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
 }
 
 // -------------------------------------------------------------------------------------------- rows held in registers
-template <typename T, int VEC, int THREADS, int NV>
+template <typename T, int VEC, int THREADS, int NV, bool STREAM>
 __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
   constexpr int WAVES = THREADS / 64;
   extern __shared__ float tables[];           // 3 x K x {column, q, logit}: of the last, this and the next row
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = i * THREADS + t;
-    dist_load(raw[i], p + w.nh, j < w.nvec ? j : 0);
+    dist_load<STREAM>(raw[i], p + w.nh, j < w.nvec ? j : 0);
   }
   extra.load(p + max(0, dist_extra<VEC>(w, t)));
   if (wave == 0) {
@@ -281,9 +283,9 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
         for (int v = 0; v < VEC; ++v) x[v] = dead ? 0.f : dist_exp(x[v], m, k2) * mul;
         Raw<T, VEC> g;
         g.put(x);
-        if (j < w.nvec) dist_store(g, out + w.nh, j);
+        if (j < w.nvec) dist_store<STREAM>(g, out + w.nh, j);
       }
-      dist_load(raw[i], pn + wn.nh, j < nn ? j : 0);      // no next row (nn = 0): one cached line
+      dist_load<STREAM>(raw[i], pn + wn.nh, j < nn ? j : 0);      // no next row (nn = 0): one cached line
     }
     if (out && ex >= 0) {
       Raw<T, 1> g;
@@ -465,10 +467,10 @@ __global__ __launch_bounds__(DIST_CUT + 64) void dist_grad_kernel(const DistArgs
 // Pieces a row is cut into (1: a workgroup holds whole rows in registers).  Cutting costs a second launch and pays where few
 // workgroups would hold very long rows: 64 x 131072 bf16 21.7 -> 16.0 us, but 64 x 65536 13.9 -> 16.8 us.
 struct DistPlan { int pieces, piece_vecs; };
-static int dist_vec(int type, bool wide) { return !wide ? 1 : type == SERL_F32 ? 4 : 8; }
-static DistPlan dist_plan(int type, int R, int V, bool wide) {
-  const int vec = dist_vec(type, wide), n = cdiv(V, vec);
-  const int most = wide ? 1024 * 20 : 256 * 16;                    // vectors of a row that fit the registers
+static int dist_vec(int type) { return type == SERL_F32 ? 4 : 8; }
+static DistPlan dist_plan(int type, int R, int V) {
+  const int n = cdiv(V, dist_vec(type));
+  const int most = 1024 * 20;                                      // vectors of a row that fit the registers
   DistPlan p{1, n};
   int want = 1;
   if (n > most) want = cdiv(n, 4096);
@@ -484,43 +486,62 @@ static DistPlan dist_plan(int type, int R, int V, bool wide) {
   return p;
 }
 
-template <typename T, int VEC, int THREADS, int NV>
+template <typename T, int VEC, int THREADS, int NV, bool STREAM>
 static void dist_go(const DistArgs& a, hipStream_t st) {
   // persistent: as many workgroups as 256 CUs hold at once (asked for once; 128 slots' tables in LDS)
   static const int fit = [] {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV>, THREADS,
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV, STREAM>, THREADS,
                                                      3 * 3 * 128 * sizeof(float)) != hipSuccess || n < 1) {
       (void)hipGetLastError();
       n = 1;
     }
     return 256 * n;
   }();
-  hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
+  hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV, STREAM>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
                      3 * 3 * a.K * sizeof(float), st, a);
 }
+// Threads and vectors per thread.  Half the vectors for rows of 65 to 128 halve the exponentials: 20000 x 1000 bf16 30 -> 28 us; fp32
+// has fewer per vector and lost by it (50000 x 512 61 -> 71 us).
+template <typename T, int VEC, bool STREAM>
+static void dist_shape(const DistArgs& a, hipStream_t st) {
+  const int n = cdiv(a.V, VEC);
+  if constexpr (!STREAM) {
+    if (n <= 64) return dist_go<T, VEC, 64, 1, false>(a, st);
+    if constexpr (VEC == 8) {
+      if (n <= 128) return dist_go<T, VEC, 64, 2, false>(a, st);
+    }
+    if (n <= 256) return dist_go<T, VEC, 64, 4, false>(a, st);
+    if (n <= 512) return dist_go<T, VEC, 64, 8, false>(a, st);
+  }
+  if (n <= 1024) dist_go<T, VEC, 128, 8, STREAM>(a, st);
+  else if (n <= 2048) dist_go<T, VEC, 256, 8, STREAM>(a, st);
+  else if (n <= 4096) dist_go<T, VEC, 512, 8, STREAM>(a, st);
+  else if (n <= 8192) dist_go<T, VEC, 1024, 8, STREAM>(a, st);
+  else if (n <= 16384) dist_go<T, VEC, 1024, 16, STREAM>(a, st);
+  else dist_go<T, VEC, 1024, 20, STREAM>(a, st);
+}
+// Logits and gradient are streamed past the caches where a call moves more than they hold and rows are whole cache lines, more than
+// 512 vectors: 2048 x 131072 bf16 242 -> 225 us, 16384 x 8192 124 -> 111; below that size 8192 x 8000 53 -> 57, of a wave's rows
+// 65536 x 1024 107 -> 121.
+static bool dist_stream(const DistArgs& a, int type) {
+  const int e = sq_size(type);
+  return a.V > 512 * 16 / e && a.V * (long long)e % 128 == 0 && a.ldl * e % 128 == 0 && a.ldd * e % 128 == 0 && sq_aligned(a.logits, 128) &&
+         sq_aligned(a.dlogits, 128) && (long long)a.R * a.V * e * (a.dlogits ? 2 : 1) > SQ_STREAM;
+}
+
 template <typename T, int VEC>
 static void dist_launch(const DistArgs& a, hipStream_t st) {
-  if (a.pieces > 1) {
+  if constexpr (VEC == 1) {
+    dist_go<T, 1, 64, 1, false>(a, st);      // less than two vectors
+  } else if (a.pieces > 1) {
     const dim3 grid((unsigned)(a.R * a.pieces));
     hipLaunchKernelGGL((dist_stats_kernel<T, VEC>), grid, dim3(DIST_CUT), 0, st, a);
     hipLaunchKernelGGL((dist_grad_kernel<T, VEC>), grid, dim3(DIST_CUT + 64), 3 * a.K * sizeof(float), st, a);
-    return;
-  }
-  const int n = cdiv(a.V, VEC);
-  if constexpr (VEC == 1) {
-    if (n <= 256) dist_go<T, 1, 64, 4>(a, st);
-    else dist_go<T, 1, 256, 16>(a, st);
+  } else if (dist_stream(a, T::code)) {
+    dist_shape<T, VEC, true>(a, st);
   } else {
-    if (n <= 64) dist_go<T, VEC, 64, 1>(a, st);
-    else if (n <= 256) dist_go<T, VEC, 64, 4>(a, st);
-    else if (n <= 512) dist_go<T, VEC, 64, 8>(a, st);
-    else if (n <= 1024) dist_go<T, VEC, 128, 8>(a, st);
-    else if (n <= 2048) dist_go<T, VEC, 256, 8>(a, st);
-    else if (n <= 4096) dist_go<T, VEC, 512, 8>(a, st);
-    else if (n <= 8192) dist_go<T, VEC, 1024, 8>(a, st);
-    else if (n <= 16384) dist_go<T, VEC, 1024, 16>(a, st);
-    else dist_go<T, VEC, 1024, 20>(a, st);
+    dist_shape<T, VEC, false>(a, st);
   }
 }
 
@@ -533,8 +554,7 @@ extern "C" long long serl_topk_distill_workspace_bytes(int type, int R, int V, i
     serl_set_error("topk_distill: bad type or sizes");
     return -1;
   }
-  const long long a = dist_ws(dist_plan(type, R, V, true), R, K), b = dist_ws(dist_plan(type, R, V, false), R, K);
-  return a > b ? a : b;
+  return dist_ws(dist_plan(type, R, V), R, K);
 }
 
 extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R, int V, int K, const void* logits,
@@ -551,11 +571,8 @@ extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R,
   SERL_CHECK_ARG(ldl >= 0 && ldt >= 0 && ldi >= 0 && (!dlogits || R <= 1 || ldd >= V),
                  "topk_distill: negative row stride, or output rows overlap");
   SERL_CHECK_ARG(!dlogits || dlogits != logits || R <= 1 || ldl == ldd, "topk_distill: in place needs the same row stride");
-  const int es = sq_size(type), vec = dist_vec(type, true);
-  // wide: logits and gradient of a row have the same distance to a 16-byte boundary
-  const bool wide = V >= 2 * vec && sq_aligned(logits, es) &&
-                    (!dlogits || (((uintptr_t)logits - (uintptr_t)dlogits) % 16 == 0 && (R <= 1 || (ldl - ldd) % vec == 0)));
-  const DistPlan p = dist_plan(type, R, V, wide);
+  const bool wide = V >= 2 * dist_vec(type);
+  const DistPlan p = dist_plan(type, R, V);
   const long long need = dist_ws(p, R, K);
   SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                  "topk_distill: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);

@@ -78,7 +78,7 @@ __device__ __forceinline__ uint32_t rms_e4m3x4(float a, float b, float c, float 
   return (uint32_t)r;
 }
 
-template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE>
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE, bool STREAM>
 __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_fwd_kernel(const RmsArgs a) {
   constexpr int WAVES = THREADS <= 64 ? 1 : THREADS / 64;
   __shared__ float red[WAVES];
@@ -92,14 +92,14 @@ __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_fwd_kernel(
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
-    rx[i].template load<LOOSE>(x + at.n);
+    rx[i].template load<LOOSE, STREAM>(x + at.n);
   }
   if (a.res) {
     const typename TR::bits* res = (const typename TR::bits*)a.res + row * a.ldres;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
-      rr[i].template load<LOOSE>(res + at.n);
+      rr[i].template load<LOOSE, STREAM>(res + at.n);
     }
   }
   float s[NV][VEC], ss = 0.f;
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_fwd_kernel(
 // dx = rstd (w dy - xh mean(w dy xh)) + ds with xh = s rstd; dw = sum over rows of dy xh.  A workgroup (THREADS = 64: a
 // wave, less: that many lanes) takes every gridDim-th row and keeps its share of dw in registers; the shares are added in a fixed order by
 // rms_dw_kernel, so the result does not depend on timing.
-template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE>
+template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE, bool STREAM>
 __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_bwd_kernel(const RmsArgs a) {
   constexpr int WAVES = THREADS <= 64 ? 1 : THREADS / 64;
   __shared__ float red[2][WAVES];
@@ -226,14 +226,14 @@ __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_bwd_kernel(
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
-      ry[i].template load<LOOSE>(dy + at.n);
-      rs[i].template load<LOOSE>(s + at.n);
+      ry[i].template load<LOOSE, STREAM>(dy + at.n);
+      rs[i].template load<LOOSE, STREAM>(s + at.n);
     }
     if (HOLD && a.ds) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
-        rd[HOLD ? i : 0].template load<LOOSE>(ds + at.n);
+        rd[HOLD ? i : 0].template load<LOOSE, STREAM>(ds + at.n);
       }
     }
     float dot = 0.f;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_bwd_kernel(
       const RmsAt<THREADS, NV, VEC, LOOSE> at(i, t, a.N);
       float y[VEC], x[VEC], d[VEC];
       if (!HOLD) rms_weight<TY, VEC, LOOSE>(a, at.n, w[0]);
-      if (!HOLD && a.ds) rd[0].template load<LOOSE>(ds + at.n);
+      if (!HOLD && a.ds) rd[0].template load<LOOSE, STREAM>(ds + at.n);
       sq_again(ry[i]);
       sq_again(rs[i]);
       ry[i].get(y);
@@ -318,31 +318,43 @@ __global__ __launch_bounds__(1024) void rms_dw_kernel(const float* part, int par
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
-template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE>
+template <typename TX, typename TR, bool FP8, int THREADS, int NV, int VEC, bool LOOSE, bool STREAM>
 static void rms_go_fwd(const RmsArgs& a, hipStream_t st) {
   const unsigned grid = THREADS <= 64 ? (unsigned)cdiv(a.R, 256 / THREADS) : (unsigned)a.R;
-  hipLaunchKernelGGL((rms_fwd_kernel<TX, TR, FP8, THREADS, NV, VEC, LOOSE>), dim3(grid), dim3(THREADS <= 64 ? 256 : THREADS), 0, st, a);
+  hipLaunchKernelGGL((rms_fwd_kernel<TX, TR, FP8, THREADS, NV, VEC, LOOSE, STREAM>), dim3(grid), dim3(THREADS <= 64 ? 256 : THREADS), 0, st, a);
 }
-template <typename TX, typename TR, bool FP8, bool LOOSE>
+template <typename TX, typename TR, bool FP8, bool LOOSE, bool STREAM>
 static void rms_shape_fwd(const RmsArgs& a, hipStream_t st) {
   constexpr int V = TX::code == SERL_F32 ? 4 : 8;
   const int n = cdiv(a.N, V);          // vectors of a row; more than half of those of a shape with several rounds (RmsAt)
-  if (n <= 16) rms_go_fwd<TX, TR, FP8, 16, 1, V, LOOSE>(a, st);
-  else if (n <= 32) rms_go_fwd<TX, TR, FP8, 32, 1, V, LOOSE>(a, st);
-  else if (n <= 64) rms_go_fwd<TX, TR, FP8, 64, 1, V, LOOSE>(a, st);
-  else if (n <= 128) rms_go_fwd<TX, TR, FP8, 64, 2, V, LOOSE>(a, st);
-  else if (n <= 256) rms_go_fwd<TX, TR, FP8, 256, 1, V, LOOSE>(a, st);
-  else if (n <= 512) rms_go_fwd<TX, TR, FP8, 256, 2, V, LOOSE>(a, st);
-  else if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, V, LOOSE>(a, st);
-  else if (n <= 2048) rms_go_fwd<TX, TR, FP8, 1024, 2, V, LOOSE>(a, st);
-  else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 1024, 4, V, LOOSE>(a, st);
-  else if constexpr (TX::code == SERL_F32) rms_go_fwd<TX, TR, FP8, 1024, 8, V, LOOSE>(a, st);      // RMS_MAXN elements
+  if (n <= 16) rms_go_fwd<TX, TR, FP8, 16, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 32) rms_go_fwd<TX, TR, FP8, 32, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 64) rms_go_fwd<TX, TR, FP8, 64, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 128) rms_go_fwd<TX, TR, FP8, 64, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 256) rms_go_fwd<TX, TR, FP8, 256, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 512) rms_go_fwd<TX, TR, FP8, 256, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 1024) rms_go_fwd<TX, TR, FP8, 256, 4, V, LOOSE, STREAM>(a, st);
+  else if constexpr (STREAM) return;                    // not chosen
+  else if (n <= 2048) rms_go_fwd<TX, TR, FP8, 1024, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 4096) rms_go_fwd<TX, TR, FP8, 1024, 4, V, LOOSE, STREAM>(a, st);
+  else if constexpr (TX::code == SERL_F32) rms_go_fwd<TX, TR, FP8, 1024, 8, V, LOOSE, STREAM>(a, st);      // RMS_MAXN elements
 }
+// Inputs are streamed past the caches where a call moves more than they hold and rows are whole cache lines: 16384 x 4096 bf16
+// forward 91 -> 78 us, both ways 197 -> 175; just above the caches' size 16384 x 2048 forward loses, 42.6 -> 44.3.  Not with rows of
+// 1024 threads (2048 x 16384 both ways 111 -> 119 us) or a residual of another type (16384 x 4096 with fp32 317 -> 331 us).
+static bool rms_stream(const RmsArgs& a, int type, int tensors) {
+  const int e = sq_size(type);
+  return a.N * e % 128 == 0 && a.ldx * e % 128 == 0 && a.ldres * e % 128 == 0 && a.N * e <= 1024 * 16 &&
+         sq_aligned(a.x, 128) && sq_aligned(a.res, 128) &&
+         (long long)a.R * a.N * e * tensors > SQ_STREAM;
+}
+
 template <typename TX, typename TR, bool FP8>
 static void rms_pick_fwd(const RmsArgs& a, bool wide, hipStream_t st) {
-  if (wide) rms_shape_fwd<TX, TR, FP8, false>(a, st);
-  else if (a.N >= (TX::code == SERL_F32 ? 4 : 8)) rms_shape_fwd<TX, TR, FP8, true>(a, st);
-  else rms_go_fwd<TX, TR, FP8, 16, 1, 1, false>(a, st);      // a row of less than a vector
+  if (wide && TX::code == TR::code && rms_stream(a, TX::code, a.res ? 4 : 2)) rms_shape_fwd<TX, TR, FP8, false, true>(a, st);
+  else if (wide) rms_shape_fwd<TX, TR, FP8, false, false>(a, st);
+  else if (a.N >= (TX::code == SERL_F32 ? 4 : 8)) rms_shape_fwd<TX, TR, FP8, true, false>(a, st);
+  else rms_go_fwd<TX, TR, FP8, 16, 1, 1, false, false>(a, st);      // a row of less than a vector
 }
 
 // Rows of the partial weight gradients: one per row of the input (rounded up to 4), at most RMS_PARTS, one per workgroup or, for
@@ -361,32 +373,34 @@ static int rms_parts(int R, int N, int vec) {
   return R < most ? (R + 3) / 4 * 4 : most;
 }
 
-template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE>
+template <typename TY, typename TS, int THREADS, int NV, int VEC, bool LOOSE, bool STREAM>
 static void rms_go_bwd(const RmsArgs& a, hipStream_t st) {
   const int parts = rms_parts(a.R, a.N, TY::code == SERL_F32 ? 4 : 8);
-  hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC, LOOSE>), dim3(THREADS <= 64 ? parts / 4 : parts),
+  hipLaunchKernelGGL((rms_bwd_kernel<TY, TS, THREADS, NV, VEC, LOOSE, STREAM>), dim3(THREADS <= 64 ? parts / 4 : parts),
                      dim3(THREADS <= 64 ? 256 : THREADS), 0, st, a);
 }
-template <typename TY, typename TS, bool LOOSE>
+template <typename TY, typename TS, bool LOOSE, bool STREAM>
 static void rms_shape_bwd(const RmsArgs& a, hipStream_t st) {
   constexpr int V = TY::code == SERL_F32 ? 4 : 8;
   const int n = cdiv(a.N, V);          // as in rms_shape_fwd
-  if (n <= 16) rms_go_bwd<TY, TS, 16, 1, V, LOOSE>(a, st);
-  else if (n <= 32) rms_go_bwd<TY, TS, 32, 1, V, LOOSE>(a, st);
-  else if (n <= 64) rms_go_bwd<TY, TS, 64, 1, V, LOOSE>(a, st);
-  else if (n <= 128) rms_go_bwd<TY, TS, 64, 2, V, LOOSE>(a, st);
-  else if (n <= 256) rms_go_bwd<TY, TS, 256, 1, V, LOOSE>(a, st);
-  else if (n <= 512) rms_go_bwd<TY, TS, 256, 2, V, LOOSE>(a, st);
-  else if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, V, LOOSE>(a, st);
-  else if (n <= 2048) rms_go_bwd<TY, TS, 1024, 2, V, LOOSE>(a, st);
-  else if (n <= 4096) rms_go_bwd<TY, TS, 1024, 4, V, LOOSE>(a, st);
-  else if constexpr (TY::code == SERL_F32) rms_go_bwd<TY, TS, 1024, 8, V, LOOSE>(a, st);
+  if (n <= 16) rms_go_bwd<TY, TS, 16, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 32) rms_go_bwd<TY, TS, 32, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 64) rms_go_bwd<TY, TS, 64, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 128) rms_go_bwd<TY, TS, 64, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 256) rms_go_bwd<TY, TS, 256, 1, V, LOOSE, STREAM>(a, st);
+  else if (n <= 512) rms_go_bwd<TY, TS, 256, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 1024) rms_go_bwd<TY, TS, 256, 4, V, LOOSE, STREAM>(a, st);
+  else if constexpr (STREAM) return;                    // not chosen
+  else if (n <= 2048) rms_go_bwd<TY, TS, 1024, 2, V, LOOSE, STREAM>(a, st);
+  else if (n <= 4096) rms_go_bwd<TY, TS, 1024, 4, V, LOOSE, STREAM>(a, st);
+  else if constexpr (TY::code == SERL_F32) rms_go_bwd<TY, TS, 1024, 8, V, LOOSE, STREAM>(a, st);
 }
 template <typename TY, typename TS>
 static void rms_pick_bwd(const RmsArgs& a, bool wide, hipStream_t st) {
-  if (wide) rms_shape_bwd<TY, TS, false>(a, st);
-  else if (a.N >= (TY::code == SERL_F32 ? 4 : 8)) rms_shape_bwd<TY, TS, true>(a, st);
-  else rms_go_bwd<TY, TS, 16, 1, 1, false>(a, st);
+  if (wide && TY::code == TS::code && rms_stream(a, TY::code, a.ds ? 4 : 3)) rms_shape_bwd<TY, TS, false, true>(a, st);
+  else if (wide) rms_shape_bwd<TY, TS, false, false>(a, st);
+  else if (a.N >= (TY::code == SERL_F32 ? 4 : 8)) rms_shape_bwd<TY, TS, true, false>(a, st);
+  else rms_go_bwd<TY, TS, 16, 1, 1, false, false>(a, st);
 }
 
 static bool rms_wide(int type, int elems, const void* p, long long ld) {

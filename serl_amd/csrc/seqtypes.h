@@ -44,13 +44,14 @@ template <> __device__ __forceinline__ uint32_t sq_pack2<F16>(float a, float b) 
 }
 
 // VEC consecutive elements of type T as they lie in memory (VEC * size = a power of two of bytes, naturally aligned; LOOSE: at any
-// element, the same instructions, which the hardware takes at any address; VEC = 1: one element)
+// element, the same instructions, which the hardware takes at any address; STREAM:
+// touched once, in whole cache lines, not to be kept in the caches; VEC = 1: one element)
 template <typename T, int VEC> struct Raw {
   static constexpr int BYTES = VEC * (int)sizeof(typename T::bits);
   static constexpr int W = BYTES / 4;
   static_assert(BYTES % 4 == 0, "whole dwords");
   uint32_t w[W];
-  template <bool LOOSE = false> __device__ __forceinline__ void load(const typename T::bits* p) {
+  template <bool LOOSE = false, bool STREAM = false> __device__ __forceinline__ void load(const typename T::bits* p) {
     if constexpr (LOOSE) {
 #pragma unroll
       for (int i = 0; i < W; i += 4) {
@@ -62,7 +63,8 @@ template <typename T, int VEC> struct Raw {
     } else if constexpr (W % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
-        const sq_u32x4 v = reinterpret_cast<const sq_u32x4*>(p)[i];
+        const sq_u32x4* q = reinterpret_cast<const sq_u32x4*>(p) + i;
+        const sq_u32x4 v = STREAM ? __builtin_nontemporal_load(q) : *q;
         w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
       }
     } else if constexpr (W == 2) {
@@ -73,7 +75,7 @@ template <typename T, int VEC> struct Raw {
       w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
   }
-  template <bool LOOSE = false> __device__ __forceinline__ void store(typename T::bits* p) const {
+  template <bool LOOSE = false, bool STREAM = false> __device__ __forceinline__ void store(typename T::bits* p) const {
     if constexpr (LOOSE) {
 #pragma unroll
       for (int i = 0; i < W; i += 4) {
@@ -84,8 +86,11 @@ template <typename T, int VEC> struct Raw {
       }
     } else if constexpr (W % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i)
-        reinterpret_cast<sq_u32x4*>(p)[i] = (sq_u32x4){w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      for (int i = 0; i < W / 4; ++i) {
+        const sq_u32x4 v = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<sq_u32x4*>(p) + i);
+        else reinterpret_cast<sq_u32x4*>(p)[i] = v;
+      }
     } else if constexpr (W == 2) {
       *reinterpret_cast<sq_u32x2*>(p) = (sq_u32x2){w[0], w[1]};
     } else {
@@ -113,8 +118,8 @@ template <typename T, int VEC> struct Raw {
 };
 template <typename T> struct Raw<T, 1> {
   typename T::bits w;
-  template <bool LOOSE = false> __device__ __forceinline__ void load(const typename T::bits* p) { w = *p; }
-  template <bool LOOSE = false> __device__ __forceinline__ void store(typename T::bits* p) const { *p = w; }
+  template <bool LOOSE = false, bool STREAM = false> __device__ __forceinline__ void load(const typename T::bits* p) { w = *p; }
+  template <bool LOOSE = false, bool STREAM = false> __device__ __forceinline__ void store(typename T::bits* p) const { *p = w; }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = sq_val(T(), w); }
   __device__ __forceinline__ void put(const float (&v)[1]) { w = sq_bits(T(), v[0]); }
 };
@@ -160,6 +165,7 @@ template <typename T, int VEC> __device__ __forceinline__ void sq_store(const Ra
 }
 
 static inline bool sq_aligned(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
+#define SQ_STREAM (5ll << 26)       // a call that moves more bytes gains from streaming accesses (the last cache level has 2^28)
 static inline int sq_size(int code) { return code == SERL_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float sq_wave_sum(float v) {
