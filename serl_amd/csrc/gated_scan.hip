@@ -175,10 +175,10 @@ struct ScanRows {
     const int rows = min(te - t, Spot::ROWS);
     return sq_buffer(base + t * ts, rows > 0 ? (rows - 1) * (int)ts + D * (int)sizeof(typename T::bits) : 0);
   }
-  __device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[L], int t, int te, int D) const {
+  template <bool STREAM = false> __device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[L], int t, int te, int D) const {
     const __amdgpu_buffer_rsrc_t b = at(t, te, D);
 #pragma unroll
-    for (int l = 0; l < L; ++l) sq_load(r[l], b, off + l * (uint32_t)ts);
+    for (int l = 0; l < L; ++l) sq_load<STREAM>(r[l], b, off + l * (uint32_t)ts);
   }
 };
 
@@ -223,8 +223,9 @@ template <typename T> __device__ __forceinline__ uint32_t scan_inf() {       // 
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
-// SUMMARY: write the piece's map instead of the outputs (first of two launches when the time axis is split).
-template <typename T, int VEC, int CG, int L, int THREADS, bool SUMMARY>
+// SUMMARY: write the piece's map instead of the outputs (first of two launches when the time axis is split).  STREAM: 1 the inputs, 2
+// the outputs pass by the caches.
+template <typename T, int VEC, int CG, int L, int THREADS, bool SUMMARY, int STREAM>
 __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
   constexpr int TC = THREADS / CG, TILE = TC * L, WAVES = THREADS / 64;
   static_assert(SCAN_CKPT % L == 0, "kept states lie between the chunks of two threads");
@@ -241,8 +242,8 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
 
   Raw<T, VEC> rg[L], rx[L];
   int tw = me.tb + me.wave * me.ROWS, buf = 0;          // the wave's first step of the tile
-  gate.fetch(rg, tw, me.te, a.D);
-  x.fetch(rx, tw, me.te, a.D);
+  gate.template fetch<STREAM == 1>(rg, tw, me.te, a.D);
+  x.template fetch<STREAM == 1>(rx, tw, me.te, a.D);
   unsigned char rs = scan_start<CG, L>(starts, tw + me.first, me.te, me.lane);
   for (int t0 = me.tb; t0 < me.te; t0 += TILE, tw += TILE, buf ^= 1) {
     const int t = tw + me.first;
@@ -267,8 +268,8 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
       }
       if (cuts) scan_cut<VEC>(k[l], cut >> l & 1, 0.f);
     }
-    gate.fetch(rg, tw + TILE, me.te, a.D);
-    x.fetch(rx, tw + TILE, me.te, a.D);
+    gate.template fetch<STREAM == 1>(rg, tw + TILE, me.te, a.D);
+    x.template fetch<STREAM == 1>(rx, tw + TILE, me.te, a.D);
     rs = scan_start<CG, L>(starts, t + TILE, me.te, me.lane);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { kk[v] = k[0][v]; bb[v] = add[0][v]; }
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
         Raw<T, VEC> r;
         r.put(c);
         if (!whole) scan_mask(r, t + l < me.len, 0);
-        sq_store(r, out, y.off + l * (uint32_t)y.ts);
+        sq_store<STREAM == 2>(r, out, y.off + l * (uint32_t)y.ts);
       }
     }
   }
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
 // With C_t = k_t G_t the gradient that leaves step t backwards in time: G_t = dy_t + C_{t+1}, C_t = k_t (dy_t + C_{t+1}),
 // C_T = dh_last, dh0 = C_0; dx = G (1 - f), dgate = G (k_t/f_t h_{t-1} - x) f (1 - f).  h is recomputed from the state that
 // the forward pass kept at the tile's first step (in 32 bits, where y was rounded), so y is not read.
-template <typename T, int VEC, int CG, int L, int THREADS>
+template <typename T, int VEC, int CG, int L, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
   constexpr int TC = THREADS / CG, TILE = TC * L, WAVES = THREADS / 64;
   __shared__ __attribute__((aligned(16))) float lds[2][2][WAVES * 2 * VEC * CG];
@@ -441,8 +442,8 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
         scan_mask(r1, t + l < me.len, 0);
         scan_mask(r2, t + l < me.len, 0);
       }
-      sq_store(r1, og, dgate.off + l * (uint32_t)dgate.ts);
-      sq_store(r2, ox, dx.off + l * (uint32_t)dx.ts);
+      sq_store<STREAM>(r1, og, dgate.off + l * (uint32_t)dgate.ts);
+      sq_store<STREAM>(r2, ox, dx.off + l * (uint32_t)dx.ts);
     }
   }
   if (me.seg == 0 && me.chok) a.dh0[state] = carry;
@@ -614,30 +615,56 @@ static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_rea
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
 #define SCAN_LONG(KERNEL, ...)                                                          \
   do {                                                                                  \
-    if (p.vec == 1) SCAN_GO(KERNEL, 1, 64, 8, 1024, ##__VA_ARGS__);                     \
-    else if constexpr (T::code == SERL_F32) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__); \
+    if constexpr (T::code == SERL_F32) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);    \
     else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                                 \
   } while (0)
 #define SCAN_PICK(KERNEL, ...)                                                          \
   do {                                                                                  \
-    const bool half = T::code != SERL_F32 && (long long)a.B * a.ndb >= 512;           \
+    const bool half = T::code != SERL_F32 && (long long)a.B * a.ndb >= 512;             \
     constexpr int C = T::code == SERL_F32 ? 8 : 16, L = T::code == SERL_F32 ? 2 : 4;    \
-    if (p.vec == 1 || (a.T > 64 && !half)) SCAN_LONG(KERNEL, ##__VA_ARGS__);            \
+    if (a.T > 64 && !half) SCAN_LONG(KERNEL, ##__VA_ARGS__);                            \
     else if (a.T > 32) SCAN_GO(KERNEL, 4, C, L, 256, ##__VA_ARGS__);                    \
     else if (a.T > 16) SCAN_GO(KERNEL, 4, C, L, 128, ##__VA_ARGS__);                    \
     else SCAN_GO(KERNEL, 4, C, L, 64, ##__VA_ARGS__);                                   \
   } while (0)
+// Streaming where a call moves more than the caches hold and rows are whole cache lines (others lose: 20 x 3000 x 1000 bf16 both ways
+// 347 -> 386 us).  Forward alone the inputs: 64 x 1024 x 1024 bf16 90 -> 80 us, 32 x 2048 x 1024 fp32 185 -> 156; where they are read
+// again, by the second launch of a split axis or the backward pass, the outputs, and so backward: 4 x 8192 x 2048 forward 152 ->
+// 128, both ways 16 x 4096 x 2048 490 -> 470 (with the inputs 501), 64 x 1024 x 1024 254 -> 240.
+template <typename T>
+static bool scan_stream(const ScanArgs& a, int tensors) {
+  return !a.share && (long long)a.B * a.T * a.D * tensors * (long long)sizeof(typename T::bits) > SQ_STREAM;
+}
 template <typename T>
 static void scan_launch_fwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
-  if (a.nseg > 1) SCAN_LONG(scan_fwd_kernel, true);
-  SCAN_PICK(scan_fwd_kernel, false);
+  const bool stream = scan_stream<T>(a, 3);
+  if (p.vec == 1) {
+    if (a.nseg > 1) SCAN_GO(scan_fwd_kernel, 1, 64, 8, 1024, true, 0);
+    SCAN_GO(scan_fwd_kernel, 1, 64, 8, 1024, false, 0);
+  } else if (a.nseg > 1) {
+    SCAN_LONG(scan_fwd_kernel, true, 0);
+    if (stream) SCAN_LONG(scan_fwd_kernel, false, 2);
+    else SCAN_LONG(scan_fwd_kernel, false, 0);
+  } else if (stream && a.ckpt) {
+    SCAN_PICK(scan_fwd_kernel, false, 2);
+  } else if (stream) {
+    SCAN_PICK(scan_fwd_kernel, false, 1);
+  } else {
+    SCAN_PICK(scan_fwd_kernel, false, 0);
+  }
 }
 template <typename T>
 static void scan_launch_bwd(const ScanArgs& a, const ScanPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((long long)a.B * a.nseg * a.ndb));
+  if (p.vec == 1) {
+    if (a.nseg > 1) SCAN_GO(scan_bwd_summary_kernel, 1, 64, 8, 1024);
+    SCAN_GO(scan_bwd_kernel, 1, 64, 8, 1024, false);
+    return;
+  }
   if (a.nseg > 1) SCAN_LONG(scan_bwd_summary_kernel);
-  SCAN_PICK(scan_bwd_kernel);
+  if (scan_stream<T>(a, 5)) SCAN_PICK(scan_bwd_kernel, true);
+  else SCAN_PICK(scan_bwd_kernel, false);
 }
 template <typename T>
 static void scan_launch_short(ScanArgs a, bool wide, hipStream_t st) {

@@ -138,29 +138,30 @@ template <typename T, int VEC> __device__ __forceinline__ void sq_again(Raw<T, V
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t sq_buffer(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
 }
+// STREAM: the non-temporal hint.
 #define SQ_NOWHERE 0x80000000u      // an offset behind every buffer
-template <typename T, int VEC> __device__ __forceinline__ void sq_load(Raw<T, VEC>& r, __amdgpu_buffer_rsrc_t b, uint32_t off) {
+template <bool STREAM = false, typename T, int VEC> __device__ __forceinline__ void sq_load(Raw<T, VEC>& r, __amdgpu_buffer_rsrc_t b, uint32_t off) {
   if constexpr (VEC == 1) {
-    if constexpr (sizeof(typename T::bits) == 2) r.w = __builtin_amdgcn_raw_buffer_load_b16(b, off, 0, 0);
-    else r.w = __builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0);
+    if constexpr (sizeof(typename T::bits) == 2) r.w = __builtin_amdgcn_raw_buffer_load_b16(b, off, 0, STREAM ? 2 : 0);
+    else r.w = __builtin_amdgcn_raw_buffer_load_b32(b, off, 0, STREAM ? 2 : 0);
   } else if constexpr (Raw<T, VEC>::W == 2) {
-    const sq_u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0);
+    const sq_u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, STREAM ? 2 : 0);
     r.w[0] = v.x; r.w[1] = v.y;
   } else {
     static_assert(VEC == 1 || Raw<T, VEC>::W == 4, "one access");
-    const sq_u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0);
+    const sq_u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, STREAM ? 2 : 0);
     r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
   }
 }
-template <typename T, int VEC> __device__ __forceinline__ void sq_store(const Raw<T, VEC>& r, __amdgpu_buffer_rsrc_t b, uint32_t off) {
+template <bool STREAM = false, typename T, int VEC> __device__ __forceinline__ void sq_store(const Raw<T, VEC>& r, __amdgpu_buffer_rsrc_t b, uint32_t off) {
   if constexpr (VEC == 1) {
-    if constexpr (sizeof(typename T::bits) == 2) __builtin_amdgcn_raw_buffer_store_b16(r.w, b, off, 0, 0);
-    else __builtin_amdgcn_raw_buffer_store_b32(r.w, b, off, 0, 0);
+    if constexpr (sizeof(typename T::bits) == 2) __builtin_amdgcn_raw_buffer_store_b16(r.w, b, off, 0, STREAM ? 2 : 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(r.w, b, off, 0, STREAM ? 2 : 0);
   } else if constexpr (Raw<T, VEC>::W == 2) {
-    __builtin_amdgcn_raw_buffer_store_b64((sq_u32x2){r.w[0], r.w[1]}, b, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64((sq_u32x2){r.w[0], r.w[1]}, b, off, 0, STREAM ? 2 : 0);
   } else {
     static_assert(VEC == 1 || Raw<T, VEC>::W == 4, "one access");
-    __builtin_amdgcn_raw_buffer_store_b128((sq_u32x4){r.w[0], r.w[1], r.w[2], r.w[3]}, b, off, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128((sq_u32x4){r.w[0], r.w[1], r.w[2], r.w[3]}, b, off, 0, STREAM ? 2 : 0);
   }
 }
 

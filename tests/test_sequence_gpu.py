@@ -717,6 +717,65 @@ def test_rows_of_any_stride(dev):
     assert torch.equal(dx, dx[:1].expand(5, 96))
 
 
+@pytest.mark.parametrize("dtype,B,T,D", [(torch.bfloat16, 64, 1024, 1024), (torch.bfloat16, 4, 8192, 2048), (torch.float32, 12, 1024, 4096),
+                                         (torch.float16, 8192, 16, 1024)], ids=str)
+def test_gated_scan_larger_than_the_caches(dev, dtype, B, T, D):
+    """The same bits as with rows that lie otherwise in memory, which are not streamed past the caches."""
+    s = seq()
+    g = torch.Generator(dev).manual_seed(B)
+    r = lambda: torch.randn(B, T, D, generator=g, device=dev, dtype=torch.float32).to(dtype)
+    gate, x, dy = r(), r(), r()
+    starts = torch.rand(B, T, generator=g, device=dev) < 0.01
+    lengths = torch.randint(0, T + 1, (B,), generator=g, device=dev)
+
+    def other(t):
+        big = torch.empty(B, T, D + 4, dtype=dtype, device=dev)
+        big[:, :, :D] = t
+        return big[:, :, :D]
+    y, h = s.gated_scan(gate, x, starts=starts, lengths=lengths)
+    y2, h2, saved = s.gated_scan(gate, x, starts=starts, lengths=lengths, save=True)
+    y3, h3, saved3 = s.gated_scan(other(gate), x, starts=starts, lengths=lengths, save=True)
+    assert torch.equal(y, y3) and torch.equal(y2, y3) and torch.equal(h, h3) and torch.equal(h2, h3) and torch.equal(saved, saved3)
+    one = s.gated_scan_backward(gate, x, saved, dy, starts=starts, lengths=lengths)
+    two = s.gated_scan_backward(gate, other(x), saved, dy, starts=starts, lengths=lengths)
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+
+
+@pytest.mark.parametrize("dtype,R,N", [(torch.bfloat16, 12288, 4096), (torch.float32, 12000, 4096), (torch.float16, 700000, 128)], ids=str)
+def test_rms_norm_larger_than_the_caches(dev, dtype, R, N):
+    """The same bits as the calls on some of the rows, which are not streamed past the caches."""
+    s = seq()
+    g = torch.Generator(dev).manual_seed(R)
+    r = lambda *n: torch.randn(*n, generator=g, device=dev).to(dtype)
+    x, res, dy, ds, w = r(R, N), r(R, N), r(R, N), r(R, N), r(N)
+    y, total, rstd = s.rms_norm(x, w, res, save=True)
+    q, scale, total2 = s.rms_norm_fp8(x, w, res)
+    dx, dw = s.rms_norm_backward(dy, total, rstd, w, ds)
+    assert torch.equal(total, total2)
+    step, sums = R // 10, []
+    for a in range(0, R, step):
+        c = slice(a, a + step)
+        y1, t1, r1 = s.rms_norm(x[c], w, res[c], save=True)
+        q1, s1, _ = s.rms_norm_fp8(x[c], w, res[c])
+        d1, w1 = s.rms_norm_backward(dy[c], t1, r1, w, ds[c])
+        sums.append(w1.double())
+        assert torch.equal(y[c], y1) and torch.equal(total[c], t1) and torch.equal(rstd[c], r1) and torch.equal(dx[c], d1)
+        assert torch.equal(q[c].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(scale[c], s1)
+    # |dy xh| of a column sums to less than R at unit variance; both sums as in check_norm, of the same terms
+    within(dw, sum(sums).cpu(), 2 * (R / 128 + 52) * U * R * torch.ones(N, dtype=torch.float64), "dweight")
+
+
+def test_topk_distill_larger_than_the_caches(dev):
+    s = seq()
+    for dtype, R, V in ((torch.bfloat16, 1400, 65536), (torch.float32, 12000, 4096)):
+        i = distill_inputs(dev, dtype, R, V, 20, 3)
+        loss, d = s.topk_distill(i["logits"], i["teacher"], i["index"], 1.5, i["coef"])
+        for a in range(0, R, R // 5):
+            c = slice(a, a + R // 5)
+            l1, d1 = s.topk_distill(i["logits"][c], i["teacher"][c], i["index"][c], 1.5, i["coef"][c])
+            assert torch.equal(loss[c], l1) and torch.equal(d[c], d1)
+
+
 def test_two_streams_at_once(dev):
     """The same calls on two streams together, those with scratch memory among them, give what one call alone gives."""
     s = seq()
