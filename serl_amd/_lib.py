@@ -183,8 +183,9 @@ def check(status: int, what: str = ""):
 
 
 def call(name: str, *args):
-    lib = load()
-    check(getattr(lib, name)(*args), name)
+    status = getattr(_lib or load(), name)(*args)
+    if status != 0:
+        check(status, name)
 
 
 def ptr_table(ptrs):

@@ -14,6 +14,7 @@ on every call."""
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -27,6 +28,14 @@ try:                                    # the handle alone: a tenth of the time 
 except AttributeError:
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
+try:                                    # the tensors at hand have initialised the GPU: without torch.cuda's question whether it is
+    _device = torch._C._cuda_getDevice
+except AttributeError:
+    _device = torch.cuda.current_device
+# scratch sizes depend on the calls' sizes alone
+_scan_bytes = functools.lru_cache(1024)(ops.gated_scan_workspace_bytes)
+_norm_bytes = functools.lru_cache(1024)(ops.rms_norm_bwd_workspace_bytes)
+_distill_bytes = functools.lru_cache(1024)(ops.topk_distill_workspace_bytes)
 
 
 def _shape(t, name, shape):
@@ -54,7 +63,7 @@ def _place(names, *tensors):
             at = d
         elif d != at:
             raise ValueError(f"{names[i]} is on {t.device}, the others on cuda:{at}")
-    return _NO_GUARD if at == torch.cuda.current_device() else torch.cuda.device(at)
+    return _NO_GUARD if at == _device() else torch.cuda.device(at)
 
 
 def _channels(t):
@@ -110,7 +119,7 @@ def _masks(starts, lengths, T):
 
 
 def _scan_scratch(code, B, T, D, device):
-    n = ops.gated_scan_workspace_bytes(code, B, T, D)
+    n = _scan_bytes(code, B, T, D)
     return (torch.empty(n // 4, dtype=torch.float32, device=device) if n else None), n
 
 
@@ -289,7 +298,7 @@ def rms_norm_backward(dy, s, rstd, weight, ds=None):
         R, dev = sr.shape[0], s.device
         dx = torch.empty_like(s, memory_format=_ROWS)
         dw = s.new_empty(N, dtype=torch.float32)
-        n = ops.rms_norm_bwd_workspace_bytes(R, N)
+        n = _norm_bytes(R, N)
         ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
         ops.rms_norm_bwd(_CODES[dy.dtype], _CODES[s.dtype], _CODES[weight.dtype], R, N, yr.data_ptr(), yr.stride(0),
                          sr.data_ptr(), sr.stride(0), rstd.data_ptr(), weight.data_ptr(), _ptr(dr),
@@ -343,7 +352,7 @@ def topk_distill(logits, teacher, index, temperature=1.0, coef=None, grad=True, 
         loss = logits.new_empty(R, dtype=torch.float32)
         if grad and out is None:
             out = torch.empty_like(logits, memory_format=_ROWS)
-        n = ops.topk_distill_workspace_bytes(code, R, V, K)
+        n = _distill_bytes(code, R, V, K)
         ws = torch.empty(n // 4, dtype=torch.float32, device=dev) if n else None
         ops.topk_distill(code, _CODES[teacher.dtype], index.dtype == torch.int64, R, V, K, logits.data_ptr(), logits.stride(0),
                          teacher.data_ptr(), teacher.stride(0), index.data_ptr(), index.stride(0), temperature, _ptr(coef),
