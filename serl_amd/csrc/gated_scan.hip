@@ -739,6 +739,7 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG((T <= 1 || (dgate_ts >= D && dx_ts >= D)) && (B <= 1 || (dgate_bs >= D && dx_bs >= D)),
                  "gated_scan_bwd: rows of dgate or dx overlap");
   SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_bwd: T too large");
+  if (T == 1) gate_ts = x_ts = dy_ts = dgate_ts = dx_ts = D;      // one step: its strides mean nothing, but rows must not overlap
   const bool wide = scan_wide(type, D, gate_ts) && scan_wide(type, D, x_ts) && scan_wide(type, D, dy_ts) &&
                     scan_wide(type, D, dgate_ts) && scan_wide(type, D, dx_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);

@@ -717,6 +717,23 @@ def test_rows_of_any_stride(dev):
     assert torch.equal(dx, dx[:1].expand(5, 96))
 
 
+def test_one_step_whose_time_stride_means_nothing(dev):
+    """(B, 1, D) tensors made by a transpose have a time stride of one element."""
+    s = seq()
+    g = torch.Generator(dev).manual_seed(2)
+    for dtype, D in ((torch.float32, 48), (torch.bfloat16, 130), (torch.bfloat16, 3)):
+        gate, x, dy = (torch.randn(5, 1, D, generator=g, device=dev).to(dtype) for _ in range(3))
+        y, h, saved = s.gated_scan(gate, x, save=True)
+        want = s.gated_scan_backward(gate, x, saved, dy)
+        flat = lambda t: t.reshape(5, D).clone().view(5, D, 1).transpose(1, 2)
+        assert flat(x).stride() == (D, 1, 1)
+        y2, h2, saved2 = s.gated_scan(flat(gate), flat(x), save=True)
+        assert torch.equal(y, y2) and torch.equal(h, h2) and torch.equal(saved, saved2)
+        out = tuple(torch.full((5, D, 1), 9.0, dtype=dtype, device=dev).transpose(1, 2) for _ in range(2))
+        got = s.gated_scan_backward(flat(gate), flat(x), saved, flat(dy), out=out)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 @pytest.mark.parametrize("dtype,B,T,D", [(torch.bfloat16, 64, 1024, 1024), (torch.bfloat16, 4, 8192, 2048), (torch.float32, 12, 1024, 4096),
                                          (torch.float16, 8192, 16, 1024)], ids=str)
 def test_gated_scan_larger_than_the_caches(dev, dtype, B, T, D):
