@@ -15,11 +15,12 @@
 //
 // Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
 // single threads (`head` and `tail`); the gradient is stored in the logits' pieces, which may lie at any element of its rows
-// (against single elements where the two differ, 1500 x 50021 165 -> 75 us).  The teacher's columns are stored a second time, behind a barrier that all dense
-// stores of the row have passed.
+// (against single elements where the two differ, 1500 x 50021 165 -> 75 us).  The teacher's columns are
+// stored a second time, behind a barrier that all dense stores of the row have passed.
 #include "seqtypes.h"
 
 #define DIST_MAXK 512
+#define DIST_MAXR 0x7fff0000  // a row number and the step to the next one fit 31 bits
 #define DIST_LOG2E 1.44269504088896340736f
 #define DIST_LN2 0.69314718055994530942f
 
@@ -550,7 +551,7 @@ static long long dist_ws(const DistPlan& p, int R, int K) {
 }
 
 extern "C" long long serl_topk_distill_workspace_bytes(int type, int R, int V, int K) {
-  if (type < 0 || type > 2 || R < 0 || V < 1 || K < 1 || K > DIST_MAXK) {
+  if (type < 0 || type > 2 || R < 0 || R > DIST_MAXR || V < 1 || K < 1 || K > DIST_MAXK) {
     serl_set_error("topk_distill: bad type or sizes");
     return -1;
   }
@@ -563,8 +564,8 @@ extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R,
                                  float* workspace, long long workspace_bytes, void* stream) {
   SERL_CHECK_ARG(type >= 0 && type <= 2, "topk_distill: type must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   SERL_CHECK_ARG(teacher_type == type || teacher_type == SERL_F32, "topk_distill: the teacher's type must be the logits' or fp32");
-  SERL_CHECK_ARG(R >= 0 && V >= 1 && V <= 0x3fffffff && K >= 1 && K <= DIST_MAXK,
-                 "topk_distill: R >= 0, V in [1, 2^30) and K in [1, %d]", DIST_MAXK);
+  SERL_CHECK_ARG(R >= 0 && R <= DIST_MAXR && V >= 1 && V <= 0x3fffffff && K >= 1 && K <= DIST_MAXK,
+                 "topk_distill: R in [0, %d], V in [1, 2^30) and K in [1, %d]", DIST_MAXR, DIST_MAXK);
   SERL_CHECK_ARG(temperature >= 0x1p-20f && temperature <= 0x1p20f, "topk_distill: the temperature must be in [2^-20, 2^20]");
   if (R == 0) return SERL_OK;
   SERL_CHECK_ARG(logits && teacher && index && loss, "topk_distill: null pointer");

@@ -12,7 +12,7 @@
 // is joined.  16 elements per thread: with 32 the kernels were 10 to 20 % slower (registers, too few waves).
 //
 // Bound by memory and, to half, by the vector ALU (22 instructions per element forward, 35 backward).  8 x 4096 x 2048 bf16:
-// forward 94 us (4.3 TB/s where a large copy reaches 5.2), backward 163 us (4.1 TB/s).
+// forward 92 us (4.4 TB/s where a large copy reaches 5.2), backward 160 us (4.2 TB/s).
 #include "seqtypes.h"
 
 #define SCAN_CKPT 64        // steps between the states that the forward pass keeps for the backward pass
@@ -611,7 +611,8 @@ static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_rea
 // bytes of channels and 4 elements per thread and step (64 bytes of channels were 10 % slower, 32 elements per thread 10 to 20 %:
 // registers).  Both ways bf16, tile of 64 -> smaller: 256 x 16 x 1024 57 -> 28 us, 181 x 24 x 1536 61 -> 36, 1024 x 10 x 512
 // 106 -> 31.  16-bit types with two workgroups per CU to spare stay with 64 steps, half of which wait while the others work: both
-// ways 256 x 130 x 1024 229 -> 164 us, 64 x 400 x 1024 124 -> 110; with fewer the larger tile is needed to keep enough loads in flight (8 x 4096 x 2048 264 against 344 us).
+// ways 256 x 130 x 1024 229 -> 164 us, 64 x 400 x 1024 124 -> 110; with fewer the larger tile is needed to keep enough loads in
+// flight (8 x 4096 x 2048 264 against 344 us).
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
 #define SCAN_LONG(KERNEL, ...)                                                          \
   do {                                                                                  \

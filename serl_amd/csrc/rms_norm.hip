@@ -7,11 +7,13 @@
 // 16 or 32 vectors of 16 bytes (16: 262144 x 128 bf16 83 -> 42 us, 500000 x 33 both ways 360 -> 128 us against a wave per row), a
 // wave one of up to 128 (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
 // STORED (rounded to the residual's type): later layers and the backward pass see the values that were normed.
-// 16384 x 4096 bf16: forward 82 us (6.5 TB/s: part of it from the caches), backward 110 us (4.9 TB/s) and 5 us for the shares
-// of the weight's gradient; 64 rows to e4m3 4 us.
+// 16384 x 4096 bf16: forward 78 us (6.9 TB/s: part of it from the caches), both ways 177 us (5.3 TB/s), 5 us of it for the shares of
+// the weight's gradient; 64 rows to e4m3 4 us.
 #include "seqtypes.h"
 
 #define RMS_MAXN 32768
+#define RMS_MAXR 0x7fff0000  // a row number and the step to the next one fit 31 bits
+#define RMS_LAUNCH (1 << 21) // rows of one forward launch: at 1024 threads each it has less than 2^32
 #define RMS_PARTS 512        // rows of partial weight gradients: at most this many workgroups in the backward pass,
 #define RMS_MOSTPARTS 8192   // more for short rows
 
@@ -413,7 +415,7 @@ static int rms_check(const char* what, int type, int stream_type, int weight_typ
   SERL_CHECK_ARG(type >= 0 && type <= 2, "%s: type must be 0 (fp32), 1 (bf16) or 2 (fp16)", what);
   SERL_CHECK_ARG(stream_type == type || stream_type == SERL_F32, "%s: the residual's type must be x's or fp32", what);
   SERL_CHECK_ARG(weight_type == type || weight_type == SERL_F32, "%s: the weight's type must be x's or fp32", what);
-  SERL_CHECK_ARG(R >= 0 && N >= 1 && N <= RMS_MAXN, "%s: N must be in [1, %d], R >= 0", what, RMS_MAXN);
+  SERL_CHECK_ARG(R >= 0 && R <= RMS_MAXR && N >= 1 && N <= RMS_MAXN, "%s: N must be in [1, %d], R in [0, %d]", what, RMS_MAXN, RMS_MAXR);
   return SERL_OK;
 }
 
@@ -435,21 +437,31 @@ extern "C" int serl_rms_norm_fwd(int type, int stream_type, int weight_type, int
                     rms_wide(stream_type, V, sum, ldsum) && sq_aligned(weight, 16) &&
                     (y_fp8 ? sq_aligned(y, V) && ldy % V == 0 : rms_wide(type, V, y, ldy));
   RmsArgs a{};
-  a.x = x; a.ldx = ldx; a.res = residual; a.ldres = ldres; a.w = weight; a.w_f32 = weight_type == SERL_F32; a.y = y;
-  a.ldy = ldy; a.scale = scale; a.sum = sum; a.ldsum = ldsum; a.rstd_out = rstd; a.R = R; a.N = N; a.eps = eps;
+  a.ldx = ldx; a.ldres = ldres; a.w = weight; a.w_f32 = weight_type == SERL_F32; a.ldy = ldy; a.ldsum = ldsum; a.N = N;
+  a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
 #define RMS_GO(TX, TR) (y_fp8 ? rms_pick_fwd<TX, TR, true>(a, wide, st) : rms_pick_fwd<TX, TR, false>(a, wide, st))
-  if (type == SERL_F32) RMS_GO(F32, F32);
-  else if (type == SERL_BF16) { if (stream_type == SERL_F32) RMS_GO(BF16, F32); else RMS_GO(BF16, BF16); }
-  else { if (stream_type == SERL_F32) RMS_GO(F16, F32); else RMS_GO(F16, F16); }
+  for (int first = 0; first < R; first += RMS_LAUNCH) {
+    const long long e = sq_size(type), es = sq_size(stream_type);
+    a.R = R - first < RMS_LAUNCH ? R - first : RMS_LAUNCH;
+    a.x = (const char*)x + first * ldx * e;
+    a.res = residual ? (const char*)residual + first * ldres * es : nullptr;
+    a.y = (char*)y + first * ldy * (y_fp8 ? 1 : e);
+    a.sum = sum ? (char*)sum + first * ldsum * es : nullptr;
+    a.scale = scale ? scale + first : nullptr;
+    a.rstd_out = rstd ? rstd + first : nullptr;
+    if (type == SERL_F32) RMS_GO(F32, F32);
+    else if (type == SERL_BF16) { if (stream_type == SERL_F32) RMS_GO(BF16, F32); else RMS_GO(BF16, BF16); }
+    else { if (stream_type == SERL_F32) RMS_GO(F16, F32); else RMS_GO(F16, F16); }
+  }
 #undef RMS_GO
   SERL_CHECK_LAUNCH("rms_norm_fwd");
   return SERL_OK;
 }
 
 extern "C" long long serl_rms_norm_bwd_workspace_bytes(int R, int N) {
-  if (R < 0 || N < 1 || N > RMS_MAXN) {
-    serl_set_error("rms_norm_bwd: N must be in [1, %d], R >= 0", RMS_MAXN);
+  if (R < 0 || R > RMS_MAXR || N < 1 || N > RMS_MAXN) {
+    serl_set_error("rms_norm_bwd: N must be in [1, %d], R in [0, %d]", RMS_MAXN, RMS_MAXR);
     return -1;
   }
   const int most = rms_parts(R, N, 8);

@@ -45,6 +45,14 @@ def _shape(t, name, shape):
         raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+_MOST = 0x7fff0000                      # sizes are 32-bit integers in the C ABI, which would cut them
+
+
+def _sizes(*n):
+    if max(n) > _MOST:
+        raise ValueError(f"no size may be above {_MOST}, got {max(n)}")
+
+
 def _type(t, name, *dtypes):
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
@@ -89,6 +97,7 @@ def _scan_args(gate, x, starts, lengths):
     if not isinstance(gate, torch.Tensor) or gate.ndim != 3:
         raise ValueError("gate must be a (B, T, D) tensor")
     B, T, D = gate.shape
+    _sizes(B, T, D)
     _shape(x, "x", (B, T, D))
     if gate.dtype not in _CODES:
         raise TypeError(f"gate must be float32, bfloat16 or float16, got {gate.dtype}")
@@ -190,6 +199,7 @@ def gated_scan_step(gate, x, h, starts=None, h_out=None):
     if not isinstance(gate, torch.Tensor) or gate.ndim != 2:
         raise ValueError("gate must be a (B, D) tensor")
     B, D = gate.shape
+    _sizes(B, D)
     _shape(x, "x", (B, D))
     if gate.dtype not in _CODES:
         raise TypeError(f"gate must be float32, bfloat16 or float16, got {gate.dtype}")
@@ -227,6 +237,7 @@ def _width(t, name):
         raise ValueError(f"{name} must be a (..., N) tensor")
     if not 1 <= t.shape[-1] <= 32768:
         raise ValueError(f"{name}: N must be in [1, 32768], got {t.shape[-1]}")
+    _sizes(t.numel() // t.shape[-1])
 
 
 def _norm_args(x, weight, residual):
@@ -322,6 +333,7 @@ def topk_distill(logits, teacher, index, temperature=1.0, coef=None, grad=True, 
     if logits.dtype not in _CODES:
         raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
     R, V = logits.shape
+    _sizes(R, V)
     if V < 1:
         raise ValueError("logits must have at least one column")
     if not isinstance(teacher, torch.Tensor) or teacher.ndim != 2:

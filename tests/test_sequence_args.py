@@ -165,3 +165,24 @@ def test_topk_distill_refusals():
     with pytest.raises(ValueError, match="bad type or sizes"):
         ops.topk_distill_workspace_bytes(1, 4, 0, 3)
     assert ops.topk_distill_workspace_bytes(1, 2048, 131072, 128) >= 0
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Nothing is allocated: the rows are one, expanded."""
+    many = 2 ** 32 + 4
+    x, w = t(1, 8).expand(many, 8), t(8)
+    for call in (lambda: sequence.rms_norm(x, w),
+                 lambda: sequence.rms_norm_fp8(t(1, 8, dtype=torch.float16).expand(many, 8), w.half()),
+                 lambda: sequence.rms_norm_backward(x, x, t(1).expand(many), w),
+                 lambda: sequence.topk_distill(x, t(1, 3).expand(many, 3), t(1, 3, dtype=torch.int64).expand(many, 3)),
+                 lambda: sequence.topk_distill(t(1, 1).expand(4, many), t(4, 3), t(4, 3, dtype=torch.int64)),
+                 lambda: sequence.gated_scan_step(x, x, x), lambda: sequence.gated_scan(x[:, None], x[:, None]),
+                 lambda: sequence.gated_scan(x[None], x[None])):
+        with pytest.raises(ValueError, match="no size may be above"):
+            call()
+    with pytest.raises(ValueError, match="R in"):
+        ops.rms_norm_fwd(1, 1, 1, 2 ** 31 - 1, 8, 16, 8, None, 0, 16, 1e-6, 16, 8, 0, None, None, 0, None, 0)
+    with pytest.raises(ValueError, match="R in"):
+        ops.rms_norm_bwd_workspace_bytes(2 ** 31 - 1, 8)
+    with pytest.raises(ValueError, match="R in"):
+        ops.topk_distill(1, 1, 1, 2 ** 31 - 1, 8, 3, 16, 8, 16, 3, 16, 3, 1.0, None, 16, None, 0, None, 0, 0)

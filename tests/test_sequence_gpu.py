@@ -423,6 +423,22 @@ def test_rms_norm_views_shapes_and_empty_rows(dev):
     assert s.rms_norm_fp8(e, i["weight"])[1].shape == (0,)
 
 
+def test_rms_norm_more_rows_than_a_launch(dev):
+    s = seq()
+    R = 2 * 2 ** 21 + 77
+    g = torch.Generator(dev).manual_seed(6)
+    x, res = (torch.randn(R, 8, generator=g, device=dev).bfloat16() for _ in range(2))
+    w = torch.randn(8, generator=g, device=dev).bfloat16()
+    y, total, rstd = s.rms_norm(x, w, res, save=True)
+    q, scale, _ = s.rms_norm_fp8(x, w, res)
+    for a in (0, 2 ** 21 - 50, 2 ** 22 - 50, R - 100):
+        c = slice(a, a + 100)
+        one = s.rms_norm(x[c], w, res[c], save=True)
+        assert torch.equal(y[c], one[0]) and torch.equal(total[c], one[1]) and torch.equal(rstd[c], one[2])
+        one = s.rms_norm_fp8(x[c], w, res[c])
+        assert torch.equal(q[c].view(torch.uint8), one[0].view(torch.uint8)) and torch.equal(scale[c], one[1])
+
+
 def test_rms_norm_special_rows(dev):
     """Rows of zeros, of the type's smallest and largest values, with infinities and NaN; each leaves the others alone."""
     s = seq()
