@@ -676,6 +676,12 @@ static void scan_launch_short(ScanArgs a, bool wide, hipStream_t st) {
   else hipLaunchKernelGGL((scan_short_kernel<T, 1>), grid, blk, 0, st, a);
 }
 
+// a launch has less than 2^32 threads (SCAN_PICK's workgroups)
+static bool scan_fits(const ScanPlan& p, int type, int B, int T) {
+  const int threads = p.vec == 1 ? 1024 : T <= 16 ? 64 : T <= 32 ? 128 : T <= 64 || type == SERL_F32 ? 256 : 512;
+  return (long long)B * p.nseg * p.ndb < (1ll << 32) / threads;
+}
+
 #define SCAN_SHORT 8        // up to this many steps one thread runs them in order: a tile would be mostly empty
 
 extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,
@@ -697,7 +703,7 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
                               scan_rows(type, 16, x, x_bs, x_ts) && scan_rows(type, 16, y, y_bs, y_ts)
                         : scan_wide(type, D, gate_ts) && scan_wide(type, D, x_ts) && scan_wide(type, D, y_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
-  SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll && (long long)B * D <= 0x7fffffffll * SCAN_THREADS,
+  SERL_CHECK_ARG(few ? (long long)B * (wide ? D * sq_size(type) / 16 : D) < (1ll << 32) - SCAN_THREADS : scan_fits(p, type, B, T),
                  "gated_scan_fwd: B * D too large");
   ScanArgs a{};
   a.gate = gate; a.gate_bs = gate_bs; a.gate_ts = gate_ts; a.x = x; a.x_bs = x_bs; a.x_ts = x_ts;
@@ -744,7 +750,7 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
   const bool wide = scan_wide(type, D, gate_ts) && scan_wide(type, D, x_ts) && scan_wide(type, D, dy_ts) &&
                     scan_wide(type, D, dgate_ts) && scan_wide(type, D, dx_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
-  SERL_CHECK_ARG((long long)B * p.nseg * p.ndb <= 0x7fffffffll, "gated_scan_bwd: B * D too large");
+  SERL_CHECK_ARG(scan_fits(p, type, B, T), "gated_scan_bwd: B * D too large");
   SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
                  scan_reach(type, false, D, dgate_ts) && scan_reach(type, false, D, dx_ts),
                  "gated_scan_bwd: 15 steps of a tensor must span less than 2^31 bytes");

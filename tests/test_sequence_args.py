@@ -69,6 +69,10 @@ def test_gated_scan_entry_point_refusals():
         scan(T=9, gate_ts=1 << 26)
     with pytest.raises(ValueError, match=r"workspace of \d+ bytes needed, 0 available"):
         scan(T=5000, gate_bs=40000, x_bs=40000, y_bs=40000)
+    for many in (dict(B=1 << 27, T=16), dict(B=1 << 24, T=60), dict(B=1 << 29, T=1, D=64, y_ts=64, y_bs=64),
+                 dict(B=1 << 23, T=100, D=2)):                    # a launch of 2^32 threads or more
+        with pytest.raises(ValueError, match=r"B \* D too large"):
+            scan(**many)
     with pytest.raises(ValueError, match="bad type or sizes"):
         ops.gated_scan_workspace_bytes(9, 1, 1, 1)
     with pytest.raises(ValueError, match="bad sizes"):
@@ -85,6 +89,8 @@ def test_gated_scan_entry_point_refusals():
         bwd(states=None)
     with pytest.raises(ValueError, match="rows of dgate or dx overlap"):
         bwd(dx_bs=4)
+    with pytest.raises(ValueError, match=r"B \* D too large"):
+        bwd(B=1 << 26)
 
 
 def test_rms_norm_refusals():
