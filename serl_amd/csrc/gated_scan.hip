@@ -547,23 +547,27 @@ struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
 // channels alone leave half of the CUs idle and there are more than 5 tiles.  bf16 forward: 8 x 4000 x 1024 (128 workgroups) 85 ->
 // 68 us; but 12 x 4000 x 1024 (192) 89 -> 132 us, 4 x 512 x 1024 (4 tiles) 11.9 -> 16 us; both ways: 9 x 2000 x 1024 (144) 117 ->
 // 128 us, 12 x 777 x 333 fp32 (132) 52 -> 44 us.
+// 16-bit rows of up to 32 channels, or 65 to 96, are contiguous enough for groups of 32 channels, with fewer idle lanes: both ways
+// 140 x 3000 x 32 bf16 157 -> 88 us, 45 x 14336 x 24 195 -> 123, 140 x 3000 x 80 292 -> 200; with half cache lines of wider rows
+// 8 x 4096 x 2048 252 -> 357 us.
 // How many pieces: a CU holds two workgroups of the forward kernels, one of the backward, so what counts is the rounds of 512 and
 // 256 workgroups, times the tiles of a piece and three quarters of one for its start and end.  Against 512 workgroups or more
 // whatever the rounds, both ways bf16: 1 x 24576 x 2424 468 -> 357 us, 6 x 4000 x 1024 179 -> 150, 6 x 10127 x 83 76 -> 61.
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
   p.vec = wide ? 4 : 1;
-  p.cg = !wide ? 64 : type == SERL_F32 ? 8 : 16;
+  p.cg = !wide ? 64 : type == SERL_F32 || (T > 64 && (D <= 32 || (D > 64 && D <= 96))) ? 8 : 16;
   p.ndb = cdiv(D, p.vec * p.cg);
   p.nseg = 1;
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
-  if (blocks <= 136 && T > 5 * SCAN_TILE) {
+  const int fit = wide && type != SERL_F32 && p.cg == 8 ? 2 : 1;      // half the threads: twice as many workgroups on a CU
+  if (blocks <= 136 * fit && T > 5 * SCAN_TILE) {
     const int tiles = cdiv(T, SCAN_TILE);
     long long best = 0;
     for (int want = SCAN_MAXSEG; want > 1; --want) {
       const int n = cdiv(tiles, want);      // tiles of a piece
-      const long long w = blocks * cdiv(tiles, n), cost = (4ll * n + 3) * (2 * cdivll(w, 512) + cdivll(w, 256));
+      const long long w = blocks * cdiv(tiles, n), cost = (4ll * n + 3) * (2 * cdivll(w, 512 * fit) + cdivll(w, 256 * fit));
       if (!best || cost <= best) {
         best = cost;
         p.seg_len = n * SCAN_TILE;
@@ -612,18 +616,19 @@ static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_rea
 // registers).  Both ways bf16, tile of 64 -> smaller: 256 x 16 x 1024 57 -> 28 us, 181 x 24 x 1536 61 -> 36, 1024 x 10 x 512
 // 106 -> 31.  16-bit types with two workgroups per CU to spare stay with 64 steps, half of which wait while the others work: both
 // ways 256 x 130 x 1024 229 -> 164 us, 64 x 400 x 1024 124 -> 110; with fewer the larger tile is needed to keep enough loads in
-// flight (8 x 4096 x 2048 264 against 344 us).
+// flight (8 x 4096 x 2048 264 against 344 us), and for many steps where rows start inside cache lines, whose parts are then still in
+// the cache when the neighbours come (64 x 3498 x 511 471 against 591 us; 64 x 700 x 511 105 against 97).
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
 #define SCAN_LONG(KERNEL, ...)                                                          \
   do {                                                                                  \
-    if constexpr (T::code == SERL_F32) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);    \
+    if (T::code == SERL_F32 || p.cg == 8) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__); \
     else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                                 \
   } while (0)
 #define SCAN_PICK(KERNEL, ...)                                                          \
   do {                                                                                  \
-    const bool half = T::code != SERL_F32 && (long long)a.B * a.ndb >= 512;             \
+    const bool half = T::code != SERL_F32 && (long long)a.B * a.ndb >= 512 && (!a.share || a.T <= 768); \
     constexpr int C = T::code == SERL_F32 ? 8 : 16, L = T::code == SERL_F32 ? 2 : 4;    \
-    if (a.T > 64 && !half) SCAN_LONG(KERNEL, ##__VA_ARGS__);                            \
+    if (a.T > 64 && (!half || p.cg == 8)) SCAN_LONG(KERNEL, ##__VA_ARGS__);             \
     else if (a.T > 32) SCAN_GO(KERNEL, 4, C, L, 256, ##__VA_ARGS__);                    \
     else if (a.T > 16) SCAN_GO(KERNEL, 4, C, L, 128, ##__VA_ARGS__);                    \
     else SCAN_GO(KERNEL, 4, C, L, 64, ##__VA_ARGS__);                                   \

@@ -101,7 +101,8 @@ def check_scan(i, dtype, with_backward=True):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("B,T,D", [(1, 1, 1), (3, 1, 64), (2, 5, 7), (4, 8, 64), (2, 9, 16), (1, 31, 24), (2, 127, 40), (1, 128, 136),
                                    (2, 129, 33), (3, 257, 96), (2, 385, 65), (1, 640, 12), (2, 641, 10), (34, 645, 256), (35, 643, 256),
-                                   (1, 1100, 8), (2, 1537, 19), (1, 4700, 72), (3, 1030, 701), (2, 2433, 131), (2, 300, 3)])
+                                   (1, 1100, 8), (2, 1537, 19), (1, 4700, 72), (3, 1030, 701), (2, 2433, 131), (2, 300, 3),
+                                   (2, 900, 29), (3, 60, 80), (3, 200, 72), (2, 1500, 96), (150, 700, 90)])
 def test_gated_scan_matches_the_recurrence(dev, dtype, B, T, D):
     for k, opt in enumerate(({}, {"starts": True}, {"lengths": True, "h0": False}, {"starts": True, "lengths": True})):
         check_scan(scan_inputs(dev, dtype, B, T, D, 100 * k + T + D, **opt), dtype)
