@@ -19,6 +19,7 @@
 #define SCAN_TILE 128       // steps of a tile where the time axis may be split
 #define SCAN_THREADS 256    // of the kernel for a few steps
 #define SCAN_MAXD (1 << 26)  // channels
+#define SCAN_MAXT 0x7fff0000 // steps: a step and the tile behind it fit 31 bits
 #define SCAN_MAXSEG 32      // most pieces the time axis is split into
 
 struct ScanArgs {
@@ -152,7 +153,7 @@ struct ScanSpot {
     ch = min(group, a.D - VEC) + slot % VEC;
     chok = wave == 0 && lane < CG * VEC && group < a.D;
     tb = seg * a.seg_len;
-    te = min(a.T, tb + a.seg_len);
+    te = tb + min(a.seg_len, a.T - tb);
     len = min(te, scan_len(a, b));
   }
 };
@@ -546,7 +547,7 @@ struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
 // wide: 4 elements per access.  The time axis is split (two launches, gate and x read twice) only where sequences and
 // channels alone leave half of the CUs idle and there are more than 5 tiles.  bf16 forward: 8 x 4000 x 1024 (128 workgroups) 85 ->
 // 68 us; but 12 x 4000 x 1024 (192) 89 -> 132 us, 4 x 512 x 1024 (4 tiles) 11.9 -> 16 us; both ways: 9 x 2000 x 1024 (144) 117 ->
-// 128 us, 12 x 777 x 333 fp32 (132) 52 -> 44 us.
+// 128 us, 12 x 777 x 333 fp32 (132) 52 -> 42 us.
 // 16-bit rows of up to 32 channels, or 65 to 96, are contiguous enough for groups of 32 channels, with fewer idle lanes: both ways
 // 140 x 3000 x 32 bf16 157 -> 88 us, 45 x 14336 x 24 195 -> 123, 140 x 3000 x 80 292 -> 200; with half cache lines of wider rows
 // 8 x 4096 x 2048 252 -> 357 us.
@@ -581,7 +582,7 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
 static long long scan_ws(const ScanPlan& p, int B, int D) { return p.nseg > 1 ? (long long)B * p.nseg * 2 * D * 4 : 0; }
 
 extern "C" long long serl_gated_scan_workspace_bytes(int type, int B, int T, int D) {
-  if (type < 0 || type > 2 || B < 0 || T < 0 || D < 0 || D > SCAN_MAXD) {
+  if (type < 0 || type > 2 || B < 0 || T < 0 || T >= SCAN_MAXT || D < 0 || D > SCAN_MAXD) {
     serl_set_error("gated_scan: bad type or sizes");
     return -1;
   }
@@ -621,7 +622,8 @@ static bool scan_wide(int type, int D, long long ts) { return D >= 4 && scan_rea
 #define SCAN_GO(KERNEL, V, C, L, N, ...) hipLaunchKernelGGL((KERNEL<T, V, C, L, N, ##__VA_ARGS__>), grid, dim3(N), 0, st, a)
 #define SCAN_LONG(KERNEL, ...)                                                          \
   do {                                                                                  \
-    if (T::code == SERL_F32 || p.cg == 8) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__); \
+    if constexpr (T::code == SERL_F32) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);    \
+    else if (p.cg == 8) SCAN_GO(KERNEL, 4, 8, 4, 256, ##__VA_ARGS__);                   \
     else SCAN_GO(KERNEL, 4, 16, 4, 512, ##__VA_ARGS__);                                 \
   } while (0)
 #define SCAN_PICK(KERNEL, ...)                                                          \
@@ -702,7 +704,7 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG(gate_bs >= 0 && gate_ts >= 0 && x_bs >= 0 && x_ts >= 0 && (!starts || starts_bs >= 0),
                  "gated_scan_fwd: negative stride");
   SERL_CHECK_ARG((T <= 1 || y_ts >= D) && (T == 0 || B <= 1 || y_bs >= D), "gated_scan_fwd: rows of y overlap");
-  SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_fwd: T too large");
+  SERL_CHECK_ARG(T < SCAN_MAXT, "gated_scan_fwd: T too large");
   const bool few = T <= SCAN_SHORT;
   const bool wide = few ? D * sq_size(type) % 16 == 0 && scan_rows(type, 16, gate, gate_bs, gate_ts) &&
                               scan_rows(type, 16, x, x_bs, x_ts) && scan_rows(type, 16, y, y_bs, y_ts)
@@ -750,7 +752,7 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
                  (!starts || starts_bs >= 0), "gated_scan_bwd: negative stride");
   SERL_CHECK_ARG((T <= 1 || (dgate_ts >= D && dx_ts >= D)) && (B <= 1 || (dgate_bs >= D && dx_bs >= D)),
                  "gated_scan_bwd: rows of dgate or dx overlap");
-  SERL_CHECK_ARG(T < 0x7fff0000, "gated_scan_bwd: T too large");
+  SERL_CHECK_ARG(T < SCAN_MAXT, "gated_scan_bwd: T too large");
   if (T == 1) gate_ts = x_ts = dy_ts = dgate_ts = dx_ts = D;      // one step: its strides mean nothing, but rows must not overlap
   const bool wide = scan_wide(type, D, gate_ts) && scan_wide(type, D, x_ts) && scan_wide(type, D, dy_ts) &&
                     scan_wide(type, D, dgate_ts) && scan_wide(type, D, dx_ts);
