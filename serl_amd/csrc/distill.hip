@@ -151,6 +151,48 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
   for (int k = lane; k < a.K; k += 64) d.q[k] = d.idx[k] >= 0 ? d.q[k] * r : 0.f;
   return __any(any);
 }
+// The same in two steps for one slot per lane (K <= 64), so that neither the slots nor the logits they name are waited for: the
+// registers hold them as they lie in memory until dist_finish, a row later.  Same bits as dist_stage.
+struct DistSlot { uint32_t lo, hi, tv; };
+__device__ __forceinline__ long long dist_id(const DistArgs& a, const DistSlot& c) {
+  return a.index64 ? (long long)((unsigned long long)c.hi << 32 | c.lo) : (long long)(int)c.lo;
+}
+template <typename T> __device__ __forceinline__ void dist_fetch(const DistArgs& a, int row, int lane, DistSlot& c) {
+  const int k = lane < a.K ? lane : 0;
+  if (a.index64) {
+    const uint32_t* p = (const uint32_t*)((const long long*)a.index + row * a.ldi + k);
+    c.lo = p[0]; c.hi = p[1];
+  } else {
+    c.lo = ((const uint32_t*)a.index)[row * a.ldi + k]; c.hi = 0;
+  }
+  c.tv = a.teacher_f32 ? ((const uint32_t*)a.teacher)[row * a.ldt + k] : (uint32_t)((const typename T::bits*)a.teacher)[row * a.ldt + k];
+}
+template <typename T> __device__ __forceinline__ bool dist_there(const DistArgs& a, const DistSlot& c, int lane, float& tv) {
+  const long long id = dist_id(a, c);
+  tv = a.teacher_f32 ? __uint_as_float(c.tv) : sq_val(T(), (typename T::bits)c.tv);
+  return lane < a.K && id >= 0 && id < a.V && !(tv == -INFINITY);
+}
+template <typename T> __device__ __forceinline__ typename T::bits dist_gather(const DistArgs& a, int row, const DistSlot& c, int lane) {
+  float tv;
+  const bool ok = dist_there<T>(a, c, lane, tv);
+  return ((const typename T::bits*)a.logits + row * a.ldl)[ok ? dist_id(a, c) : 0];
+}
+template <typename T>
+__device__ __forceinline__ bool dist_finish(const DistArgs& a, const DistSlot& c, typename T::bits lg, const DistTeacher& d, int lane) {
+  float tv;
+  const bool ok = dist_there<T>(a, c, lane, tv);
+  tv *= 1.f / a.tau;
+  float top = ok ? fmaxf(-INFINITY, tv) : -INFINITY;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float e = ok ? expf(tv - top) : 0.f, sum = sq_wave_sum(e);
+  if (lane < a.K) {
+    d.idx[lane] = ok ? (int)dist_id(a, c) : -1;
+    d.q[lane] = ok ? e * (1.f / sum) : 0.f;
+    d.lg[lane] = sq_val(T(), lg);
+  }
+  return __any(ok);
+}
 // loss without c tau^2, by the wave that staged the teacher
 __device__ __forceinline__ float dist_loss(const DistArgs& a, const DistTeacher& d, float m, float sum, int lane) {
   const float k2 = DIST_LOG2E / a.tau, l2 = log2f(sum);
@@ -190,9 +232,12 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
 }
 
 // -------------------------------------------------------------------------------------------- rows held in registers
-template <typename T, int VEC, int THREADS, int NV, bool STREAM>
+// EARLY (one wave, K <= 64): the teacher's slots are fetched two rows ahead, the logits they name one row: 65536 x 1000 bf16 with 32
+// slots 107 -> 79 us, 100000 x 256 123 -> 104.
+template <typename T, int VEC, int THREADS, int NV, bool STREAM, bool EARLY>
 __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
   constexpr int WAVES = THREADS / 64;
+  static_assert(!EARLY || WAVES == 1, "one wave");
   extern __shared__ float tables[];           // 3 x K x {column, q, logit}: of the last, this and the next row
   __shared__ float red[2][WAVES][2];
   __shared__ int alive[3];
@@ -210,7 +255,13 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     dist_load<STREAM>(raw[i], p + w.nh, j < w.nvec ? j : 0);
   }
   extra.load(p + max(0, dist_extra<VEC>(w, t)));
-  if (wave == 0) {
+  DistSlot slot, ahead;
+  bits named = 0;
+  if constexpr (EARLY) {
+    dist_fetch<T>(a, row, lane, slot);
+    dist_fetch<T>(a, min(row + (int)gridDim.x, a.R - 1), lane, ahead);
+    named = dist_gather<T>(a, row, slot, lane);
+  } else if (wave == 0) {
     const bool any = dist_stage<T, false>(a, row, dist_tables(tables, a.K, 0), lane);
     if (lane == 0) alive[0] = any;
   }
@@ -259,8 +310,17 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     }
     m = dist_uniform(m);
     s = dist_uniform(s);
+    bool any_slot;
+    if constexpr (EARLY) {
+      any_slot = dist_finish<T>(a, slot, named, dist_tables(tables, a.K, tab), lane);
+      slot = ahead;
+      named = dist_gather<T>(a, min(row + (int)gridDim.x, a.R - 1), slot, lane);
+      dist_fetch<T>(a, min(row + 2 * (int)gridDim.x, a.R - 1), lane, ahead);
+    } else {
+      any_slot = alive[tab];
+    }
     const float c = a.coef ? a.coef[row] : 1.f;
-    const bool dead = !alive[tab] || c == 0.f;
+    const bool dead = !any_slot || c == 0.f;
     if (wave == 0) {
       const float l = dist_loss(a, dist_tables(tables, a.K, tab), m, s, lane);
       if (lane == 0) a.loss[row] = dead ? 0.f : c * a.tau * a.tau * l;
@@ -298,7 +358,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     last = out && !dead ? row : -1;
     last_m = m; last_inv = inv; last_scale = scale;
     tab = tab == 2 ? 0 : tab + 1;
-    if (wave == 0 && more) {
+    if (!EARLY && wave == 0 && more) {
       const bool any = dist_stage<T, false>(a, next, dist_tables(tables, a.K, tab), lane);
       if (lane == 0) alive[tab] = any;
     }
@@ -487,33 +547,37 @@ static DistPlan dist_plan(int type, int R, int V) {
   return p;
 }
 
-template <typename T, int VEC, int THREADS, int NV, bool STREAM>
+template <typename T, int VEC, int THREADS, int NV, bool STREAM, bool EARLY = false>
 static void dist_go(const DistArgs& a, hipStream_t st) {
   // persistent: as many workgroups as 256 CUs hold at once (asked for once; 128 slots' tables in LDS)
   static const int fit = [] {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV, STREAM>, THREADS,
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV, STREAM, EARLY>, THREADS,
                                                      3 * 3 * 128 * sizeof(float)) != hipSuccess || n < 1) {
       (void)hipGetLastError();
       n = 1;
     }
     return 256 * n;
   }();
-  hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV, STREAM>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
+  hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV, STREAM, EARLY>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
                      3 * 3 * a.K * sizeof(float), st, a);
 }
 // Threads and vectors per thread.  Half the vectors for rows of 65 to 128 halve the exponentials: 20000 x 1000 bf16 30 -> 28 us; fp32
 // has fewer per vector and lost by it (50000 x 512 61 -> 71 us).
+template <typename T, int VEC, bool EARLY>
+static void dist_wave(const DistArgs& a, int n, hipStream_t st) {
+  if (n <= 64) return dist_go<T, VEC, 64, 1, false, EARLY>(a, st);
+  if constexpr (VEC == 8) {
+    if (n <= 128) return dist_go<T, VEC, 64, 2, false, EARLY>(a, st);
+  }
+  if (n <= 256) return dist_go<T, VEC, 64, 4, false, EARLY>(a, st);
+  dist_go<T, VEC, 64, 8, false, EARLY>(a, st);
+}
 template <typename T, int VEC, bool STREAM>
 static void dist_shape(const DistArgs& a, hipStream_t st) {
   const int n = cdiv(a.V, VEC);
   if constexpr (!STREAM) {
-    if (n <= 64) return dist_go<T, VEC, 64, 1, false>(a, st);
-    if constexpr (VEC == 8) {
-      if (n <= 128) return dist_go<T, VEC, 64, 2, false>(a, st);
-    }
-    if (n <= 256) return dist_go<T, VEC, 64, 4, false>(a, st);
-    if (n <= 512) return dist_go<T, VEC, 64, 8, false>(a, st);
+    if (n <= 512) return a.K <= 64 ? dist_wave<T, VEC, true>(a, n, st) : dist_wave<T, VEC, false>(a, n, st);
   }
   if (n <= 1024) dist_go<T, VEC, 128, 8, STREAM>(a, st);
   else if (n <= 2048) dist_go<T, VEC, 256, 8, STREAM>(a, st);
@@ -534,7 +598,8 @@ static bool dist_stream(const DistArgs& a, int type) {
 template <typename T, int VEC>
 static void dist_launch(const DistArgs& a, hipStream_t st) {
   if constexpr (VEC == 1) {
-    dist_go<T, 1, 64, 1, false>(a, st);      // less than two vectors
+    if (a.K <= 64) dist_go<T, 1, 64, 1, false, true>(a, st);      // less than two vectors
+    else dist_go<T, 1, 64, 1, false>(a, st);
   } else if (a.pieces > 1) {
     const dim3 grid((unsigned)(a.R * a.pieces));
     hipLaunchKernelGGL((dist_stats_kernel<T, VEC>), grid, dim3(DIST_CUT), 0, st, a);
