@@ -10,7 +10,7 @@
 // stores overlap.  Few long rows, and rows too long for registers, are cut into pieces of their own workgroups: one launch
 // for the statistics, one that joins them and writes the gradient (it reads the row again, from the caches where they hold it).
 //
-// 2048 x 131072 bf16, 128 slots: 225 us (4.8 TB/s where a large copy reaches 5.2; the first load and the last store of a
+// 2048 x 131072 bf16, 128 slots: 217 us (5.0 TB/s where a large copy reaches 5.2; the first load and the last store of a
 // workgroup's eight rows overlap nothing, and the vector ALU is half busy with two exponentials per column).
 //
 // Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
@@ -137,8 +137,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
     top = ok ? fmaxf(top, tv * inv) : top;
     any |= ok;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = sq_wave_max(top);
   float sum = 0.f;
 #pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
@@ -183,8 +182,7 @@ __device__ __forceinline__ bool dist_finish(const DistArgs& a, const DistSlot& c
   const bool ok = dist_there<T>(a, c, lane, tv);
   tv *= 1.f / a.tau;
   float top = ok ? fmaxf(-INFINITY, tv) : -INFINITY;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = sq_wave_max(top);
   const float e = ok ? expf(tv - top) : 0.f, sum = sq_wave_sum(e);
   if (lane < a.K) {
     d.idx[lane] = ok ? (int)dist_id(a, c) : -1;
@@ -233,7 +231,7 @@ __device__ __forceinline__ void dist_fix(const DistArgs& a, int row, const DistT
 
 // -------------------------------------------------------------------------------------------- rows held in registers
 // EARLY (one wave, K <= 64): the teacher's slots are fetched two rows ahead, the logits they name one row: 65536 x 1000 bf16 with 32
-// slots 107 -> 79 us, 100000 x 256 123 -> 104.
+// slots 107 -> 79 us, 100000 x 256 123 -> 104 (with reductions of the vector ALU 84).
 template <typename T, int VEC, int THREADS, int NV, bool STREAM, bool EARLY>
 __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
   constexpr int WAVES = THREADS / 64;
@@ -283,8 +281,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     float xe[1];
     extra.get(xe);
     m = fmaxf(m, xe[0]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    m = sq_wave_max(m);
     const float wref = dist_ref(m);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -549,7 +546,8 @@ static DistPlan dist_plan(int type, int R, int V) {
 
 template <typename T, int VEC, int THREADS, int NV, bool STREAM, bool EARLY = false>
 static void dist_go(const DistArgs& a, hipStream_t st) {
-  // persistent: as many workgroups as 256 CUs hold at once (asked for once; 128 slots' tables in LDS)
+  // persistent: as many workgroups as 256 CUs hold at once (asked for once; 128 slots' tables in LDS); of one-wave workgroups 28 per CU
+  // instead of 32: 65536 x 1000 bf16 87 -> 79 us, 200000 x 512 187 -> 166
   static const int fit = [] {
     int n = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, dist_row_kernel<T, VEC, THREADS, NV, STREAM, EARLY>, THREADS,
@@ -557,7 +555,7 @@ static void dist_go(const DistArgs& a, hipStream_t st) {
       (void)hipGetLastError();
       n = 1;
     }
-    return 256 * n;
+    return 256 * (n > 28 ? 28 : n);
   }();
   hipLaunchKernelGGL((dist_row_kernel<T, VEC, THREADS, NV, STREAM, EARLY>), dim3(a.R < fit ? a.R : fit), dim3(THREADS),
                      3 * 3 * a.K * sizeof(float), st, a);

@@ -58,18 +58,9 @@ __device__ __forceinline__ void rms_weight(const RmsArgs& a, int n, float (&w)[V
 }
 
 // over a row's lanes of a wave: all of them, or the THREADS of a short row
-template <int THREADS> __device__ __forceinline__ float rms_sum(float v) {
-#pragma unroll
-  for (int o = (THREADS < 64 ? THREADS : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
+template <int THREADS> __device__ __forceinline__ float rms_sum(float v) { return sq_wave_sum<(THREADS < 64 ? THREADS : 64)>(v); }
 template <int THREADS> __device__ __forceinline__ unsigned rms_max(unsigned v) {
-#pragma unroll
-  for (int o = (THREADS < 64 ? THREADS : 64) / 2; o > 0; o >>= 1) {
-    const unsigned p = (unsigned)__shfl_xor((int)v, o);
-    v = v > p ? v : p;
-  }
-  return v;
+  return sq_over_lanes<(THREADS < 64 ? THREADS : 64)>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
 // e4m3 codes of four values: rounded to nearest even, clipped to +-448 (an infinity as well), NaN stays NaN

@@ -169,8 +169,33 @@ static inline bool sq_aligned(const void* p, int bytes) { return ((uintptr_t)p %
 #define SQ_STREAM (5ll << 26)       // a call that moves more bytes gains from streaming accesses (the last cache level has 2^28)
 static inline int sq_size(int code) { return code == SERL_F32 ? 4 : 2; }
 
-__device__ __forceinline__ float sq_wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// f over the 16, 32 or 64 lanes that a lane is one of, the same bits in all of them: lane exchanges of the vector ALU (the halves, the
+// rows of 16, then rotations within them), a fraction of the latency of shuffles through LDS
+// (distillation of 100000 x 64 bf16 97 -> 87 us, 2048 x 131072 224 -> 217).
+template <int N> __device__ __forceinline__ uint32_t sq_rotate(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, false);
+}
+template <int LANES, typename F> __device__ __forceinline__ uint32_t sq_over_lanes(uint32_t v, F f) {
+  if constexpr (LANES == 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(p[0], p[1]);
+  }
+  if constexpr (LANES >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(p[0], p[1]);
+  }
+  v = f(v, sq_rotate<8>(v));
+  v = f(v, sq_rotate<4>(v));
+  v = f(v, sq_rotate<2>(v));
+  return f(v, sq_rotate<1>(v));
+}
+template <int LANES = 64> __device__ __forceinline__ float sq_wave_sum(float v) {
+  return __uint_as_float(sq_over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ float sq_wave_max(float v) {       // NaN lose
+  return __uint_as_float(sq_over_lanes<64>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
 }

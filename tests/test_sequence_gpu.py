@@ -577,7 +577,8 @@ def check_distill(i, dtype, tau):
 
 DISTILL_SIZES = [(1, 1, 1), (5, 3, 2), (4, 17, 5), (6, 64, 64), (300, 256, 8), (3, 257, 9), (7, 1000, 33), (2, 2048, 512), (5, 4099, 100),
                  (2, 8192, 16), (130, 8200, 16), (2, 16387, 100), (131, 20001, 20), (2, 32768, 3), (129, 40003, 50), (1, 65536, 64), (3, 131072, 128),
-                 (130, 131075, 40), (2, 163840, 30), (129, 163841, 7), (2, 200003, 77)]
+                 (130, 131075, 40), (2, 163840, 30), (129, 163841, 7), (2, 200003, 77),
+                 (20000, 101, 20), (16000, 520, 64), (15000, 9, 3), (8000, 1500, 65)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
