@@ -124,7 +124,7 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
   const float inv = 1.f / a.tau;
   float top = -INFINITY;
   bool any = false;
-#pragma unroll(TAKEN ? 4 : 1)      // the kernel that holds rows has no registers to spare
+#pragma unroll TAKEN ? 4 : 1       // the kernel that holds rows has no registers to spare
   for (int k = lane; k < a.K; k += 64) {
     const long long id = dist_column(a, row, k);
     const float tv = a.teacher_f32 ? ((const float*)a.teacher)[row * a.ldt + k]
