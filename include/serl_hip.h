@@ -481,7 +481,8 @@ int serl_learner_timing_reset(serl_learner* h);
  * Gated linear recurrence: f = sigmoid(gate), h_t = f_t (start_t ? 0 : h_{t-1}) + (1 - f_t) x_t, y_t = h_t over (B, T, D)
  * (_bs, _ts: strides of a sequence and of a step; channels are contiguous).  h0 (B, D) or NULL = 0; starts: bytes (B, T),
  * sequence stride starts_bs, or NULL; lengths (B) or NULL: steps t >= lengths[b] (clamped to [0, T]) hold the state and
- * give y = 0 and zero gradients, whatever the inputs hold there.  h_last (B, D) = the state behind the last step; it may be
+ * give y = 0 and zero gradients, whatever the inputs hold there.  Infinities and NaN of an episode reach all its later steps
+ * (backward: its earlier ones) and none of another.  h_last (B, D) = the state behind the last step; it may be
  * h0 itself for T <= 8 (acting: T = 1).  states: NULL, or serl_gated_scan_states_floats floats that the backward pass
  * reads.  workspace: serl_gated_scan_workspace_bytes (0 for most shapes), for either direction, contents undefined.  For
  * T > 8 fifteen steps of a tensor must span less than 2^31 bytes; D <= 2^26. */

@@ -45,13 +45,23 @@ __device__ __forceinline__ void scan_gate(float z, float& f, float& rest) {
   f = z > 0.f ? 1.f - rest : e * rest;
 }
 
-// k c + b where k = 0 cuts whatever c is (0 * NaN = 0 in the legacy product): an infinity or NaN of one episode ends with it
-__device__ __forceinline__ float scan_times(float k, float c) {
+// The k of a map of several steps is 0 where an episode starts in them and only there: k c + b then cuts whatever c is (0 * NaN = 0 in the
+// legacy product), so an infinity or NaN of one episode ends with it.  Products of gates alone stay at SCAN_LEAST or above it, however
+// many (0.9^1000 is below fp32's smallest number), so that elsewhere an infinity or NaN reaches every later step.  Of a finite state c
+// no more than 1.2e-38 c is left too much by it.
+#define SCAN_LEAST 1.17549435e-38f
+__device__ __forceinline__ float scan_apply(float k, float c, float b) {
   float r;
   asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(k), "v"(c));
+  return r + b;
+}
+// k2 k1: 0 if one of them is, else at least SCAN_LEAST
+__device__ __forceinline__ float scan_times(float k2, float k1) {
+  float r, p = k2 * k1;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(k2), "v"(k1), "s"(SCAN_LEAST));
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(p), "v"(r));
   return r;
 }
-__device__ __forceinline__ float scan_apply(float k, float c, float b) { return scan_times(k, c) + b; }
 
 __device__ __forceinline__ int scan_len(const ScanArgs& a, int b) {
   if (!a.lengths) return a.T;
@@ -72,6 +82,12 @@ __device__ __forceinline__ float scan_join_bwd(const ScanArgs& a, int b, int seg
 #pragma unroll 4
   for (int s = a.nseg - 1; s > seg; --s, p -= 2 * (long long)a.D) c = scan_apply(p[0], c, p[a.D]);
   return c;
+}
+
+// a thread's own product of gates, before its starts are looked at
+template <int VEC> __device__ __forceinline__ void scan_floor(float (&k)[VEC]) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) k[v] = fmaxf(k[v], SCAN_LEAST);
 }
 
 // Joins the maps (k, b) of the threads of one channel in the order of time (REV: against it).  In: the thread's own map.
@@ -283,6 +299,7 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
       }
       if (cuts) scan_cut<VEC>(bb, cut >> l & 1, add[l]);
     }
+    scan_floor<VEC>(kk);
     if (cuts) scan_cut<VEC>(kk, cut != 0, 0.f);
     scan_join_tile<VEC, CG, WAVES, false>(kk, bb, carry, all, c, lds[buf], me.wave, me.lane);
     if constexpr (!SUMMARY) {
@@ -395,6 +412,7 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
       for (int v = 0; v < VEC; ++v) cc[v] = k[l][v] * (d[v] + cc[v]);
       if (cuts) scan_cut<VEC>(cc, cut >> l & 1, 0.f);
     }
+    scan_floor<VEC>(kk);
     if (cuts) scan_cut<VEC>(kk, cut != 0, 0.f);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) k2[v] = kk[v];
@@ -471,6 +489,7 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_summary_kernel(const ScanArg
     const int t = tw + me.first;
     float kk[VEC], cc[VEC], in[VEC];
     const unsigned cut = scan_cuts<CG, L>(rs, t, me.len, me.lane);
+    const bool cuts = __any(cut != 0);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { kk[v] = 1.f; cc[v] = 0.f; }
 #pragma unroll
@@ -484,11 +503,13 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_summary_kernel(const ScanArg
       for (int v = 0; v < VEC; ++v) {
         float f, r;
         scan_gate(g[v], f, r);
-        f = cut >> l & 1 ? 0.f : f;
-        cc[v] = scan_times(f, d[v] + cc[v]);
-        kk[v] = scan_times(kk[v], f);
+        cc[v] = f * (d[v] + cc[v]);
+        kk[v] *= f;
       }
+      if (cuts) scan_cut<VEC>(cc, cut >> l & 1, 0.f);
     }
+    scan_floor<VEC>(kk);
+    if (cuts) scan_cut<VEC>(kk, cut != 0, 0.f);
     const int before = t0 - TILE >= me.tb ? me.te : 0;
     gate.fetch(rg, max(tw - TILE, 0), before, a.D);
     dy.fetch(rd, max(tw - TILE, 0), before, a.D);

@@ -137,6 +137,7 @@ def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
 
     gate, x: (B, T, D); h0: (B, D) float32 state before the first step (None: zeros); starts: (B, T) bool, an episode
     begins at the step; lengths: (B,) ints, steps from there on hold the state and give y = 0.  T and B may be 0.
+    An infinity or NaN in the state stays in its channel until an episode begins.
     Returns (y, h_last): y (B, T, D) in gate's type, h_last (B, D) float32; with save=True also the states that
     gated_scan_backward needs."""
     B, T, D = _scan_args(gate, x, starts, lengths)

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_sequence_gpu import norm_inputs, seq
+from test_sequence_gpu import DTYPES, norm_inputs, seq
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,88 @@ def test_e4m3_codes_are_rounded_quotients(dev, dtype, stream):
             q = q.float()
             q[:, 2] = 0
             assert not q[some].any()
+
+
+# ------------------------------------------------------------------------------------------------- gated recurrence
+# every way through time: single steps in order, tiles of 16 to 128 steps, many tiles, a split time axis, narrow rows of each, groups of
+# 8 and 16 threads, two workgroups per CU
+SCAN_PLANS = [(2, 6, 24), (2, 6, 3), (2, 14, 24), (2, 30, 24), (2, 60, 24), (2, 120, 24), (2, 400, 72), (1, 3000, 72), (1, 3000, 24), (2, 2500, 90),
+              (1, 3000, 3), (2, 500, 3), (20, 700, 512), (130, 300, 256), (300, 100, 130)]
+
+
+def alike(got, want, keep, what):
+    """The same bits wherever `keep` is."""
+    assert torch.equal(got[keep], want[keep]), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", SCAN_PLANS)
+@pytest.mark.parametrize("shift", [-5.0, 1.0], ids=["forgetting", "remembering"])
+def test_what_is_not_finite_stays_until_an_episode_starts(dev, dtype, B, T, D, shift):
+    """f is above 0 for every gate above -87, so a NaN or an infinity in h0, x, dy or dh_last reaches every step behind (before) it up to
+    the next start, however small the product of the gates between; other channels, and steps it cannot reach, keep their bits."""
+    s = seq()
+    g = torch.Generator().manual_seed(T + D)
+    r = lambda *n: torch.randn(n, generator=g)  # noqa: E731
+    gate, x, dy = ((r(B, T, D) + c).to(dtype).to(dev) for c in (shift, 0, 0))
+    h0, dh = r(B, D).to(dev), r(B, D).to(dev)
+    stop = 4 * T // 5
+    starts = torch.zeros((B, T), dtype=torch.bool, device=dev)
+    starts[B - 1, stop] = True                       # the last sequence alone is cut
+    b, c = B - 1, D // 2
+    at = T // 4
+
+    def both(x=x, h0=h0, dy=dy, dh=dh, st=None):
+        y, h, saved = s.gated_scan(gate, x, h0, starts=st, save=True)
+        return (y, h) + s.gated_scan_backward(gate, x, saved, dy, dh, starts=st)
+
+    def put(t, *where, v=math.nan):
+        t = t.clone()
+        t[where] = v
+        return t
+    clean, cut = both(), both(st=starts)
+    spots = torch.zeros((B, T, D), dtype=torch.bool, device=dev)
+    state = torch.zeros((B, D), dtype=torch.bool, device=dev)
+    state[b, c] = True
+
+    def span(lo, hi):
+        m = spots.clone()
+        m[b, lo:hi, c] = True
+        return m
+    nothing = torch.zeros_like(state)
+    for name, arg, st, ys, hs, dgs, dxs, d0s in (
+            # what is NaN: y, h_last, dgate, dx, dh0
+            ("x", dict(x=put(x, b, at, c)), None, span(at, T), state, span(at, T), span(0, 0), nothing),
+            ("h0", dict(h0=put(h0, b, c)), None, span(0, T), state, span(0, T), span(0, 0), nothing),
+            ("dy", dict(dy=put(dy, b, T - 1 - at, c)), None, span(0, 0), nothing, span(0, T - at), span(0, T - at), state),
+            ("dh_last", dict(dh=put(dh, b, c)), None, span(0, 0), nothing, span(0, T), span(0, T), state),
+            ("x, cut", dict(x=put(x, b, at, c)), starts, span(at, stop), nothing, span(at, stop), span(0, 0), nothing),
+            ("h0, cut", dict(h0=put(h0, b, c)), starts, span(0, stop), nothing, span(0, stop), span(0, 0), nothing),
+            ("dy, cut", dict(dy=put(dy, b, T - 1, c)), starts, span(0, 0), nothing, span(stop, T), span(stop, T), nothing),
+            ("dh_last, cut", dict(dh=put(dh, b, c)), starts, span(0, 0), nothing, span(stop, T), span(stop, T), nothing)):
+        got, want = both(**arg, st=st), clean if st is None else cut
+        for out, u, v, nan in zip(("y", "h_last", "dgate", "dx", "dh0"), got, want, (ys, hs, dgs, dxs, d0s)):
+            assert bool(u[nan].isnan().all()), f"{name} in {out}: {int((~u[nan].isnan()).sum())} of {int(nan.sum())} finite"
+            alike(u, v, ~nan, f"{name} in {out}")
+    y, h, *_ = both(h0=put(h0, b, c, v=-math.inf))
+    assert bool((y[b, :, c] == -math.inf).all()) and float(h[b, c]) == -math.inf
+    y, h, *_ = both(x=put(x, b, at, c, v=math.inf))
+    assert bool((y[b, at:, c] == math.inf).all()) and float(h[b, c]) == math.inf
+    *_, dx, d0 = both(dh=put(dh, b, c, v=math.inf))
+    assert bool((dx[b, :, c] == math.inf).all()) and float(d0[b, c]) == math.inf
+    *_, dx, d0 = both(dy=put(dy, b, T - 1 - at, c, v=-math.inf))
+    assert bool((dx[b, :T - at, c] == -math.inf).all()) and float(d0[b, c]) == -math.inf
+    alike(dx, clean[3], ~span(0, T - at), "dx")
+
+
+@pytest.mark.parametrize("T", [6, 100, 3000])
+def test_gates_of_zero_do_not_hide_a_nan(dev, T):
+    """Where f itself is 0 in 32 bits, f h is still NaN for a NaN h."""
+    s = seq()
+    gate = torch.full((1, T, 40), -200.0, device=dev)
+    x, h0 = torch.ones_like(gate), torch.zeros(1, 40, device=dev)
+    h0[0, 7] = math.nan
+    y, h = s.gated_scan(gate, x, h0)
+    assert bool(y[0, :, 7].isnan().all()) and bool(h[0, 7].isnan())
+    y[0, :, 7] = h[0, 7] = 1
+    assert bool((y == 1).all()) and bool((h == 1).all())
