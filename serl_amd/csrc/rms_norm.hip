@@ -288,8 +288,15 @@ __global__ __launch_bounds__(THREADS <= 64 ? 256 : THREADS) void rms_bwd_kernel(
       if (a.ds) rd[HOLD ? i : 0].get(d);
 #pragma unroll
       for (int v = 0; v < VEC; ++v) d[v] = fmaf(rstd, fmaf(-(x[v] * rstd), dot, y[v] * w[HOLD ? i : 0][v]), d[v]);
+      typename TS::bits* dx = (typename TS::bits*)a.y + row * a.ldy + at.n;
       rs[i].put(d);
-      if (at.in) rs[i].template store<LOOSE>((typename TS::bits*)a.y + row * a.ldy + at.n);
+      if (LOOSE && WAVES > 1 && at.skip > 0) {       // its own columns alone: dx may be ds, of which the left neighbour, of another wave, may have
+#pragma unroll
+        for (int v = 1; v < VEC; ++v)   // stored the first ones over what was read here
+          if (v >= at.skip && at.in) dx[v] = sq_bits(TS(), d[v]);
+      } else if (at.in) {
+        rs[i].template store<LOOSE>(dx);
+      }
     }
   }
   if constexpr (THREADS < 64) {          // the wave's rows side by side

@@ -37,6 +37,38 @@ def test_e4m3_codes_are_rounded_quotients(dev, dtype, stream):
             assert not q[some].any()
 
 
+# ------------------------------------------------------------------------------- calls in place (raw pointers)
+INPLACE = [(5, 5), (9, 61), (7, 130), (5, 520), (40, 777), (6, 2047), (3, 2048), (4, 4101), (3, 8193), (300, 9001), (6, 12289), (3, 16384),
+           (4, 16385), (4, 16390), (600, 16390), (4, 16903), (4, 17409), (3, 20000), (3, 32761), (3, 32768)]
+
+
+@pytest.mark.parametrize("dtype,stream", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)], ids=str)
+def test_rms_norm_in_place(dev, dtype, stream):
+    """y over x and the sum over the residual forward; dx over ds, or over the sum, backward: the bits of separate buffers."""
+    from serl_amd import ops
+    s = seq()
+    code = {torch.float32: ops.F32, torch.bfloat16: ops.BF16, torch.float16: ops.F16}
+    st = torch.cuda.current_stream(dev).cuda_stream
+    for R, N in INPLACE:
+        i = norm_inputs(dev, dtype, stream, R, N, N)
+        w = i["weight"]
+        y, total, rstd = s.rms_norm(i["x"], w, i["residual"], save=True)
+        dx, dw = s.rms_norm_backward(i["dy"], total, rstd, w, i["ds"])
+        x, res = i["x"].clone(), i["residual"].clone()
+        ops.rms_norm_fwd(code[dtype], code[stream], code[dtype], R, N, x.data_ptr(), N, res.data_ptr(), N, w.data_ptr(), 1e-6, x.data_ptr(),
+                         N, False, None, res.data_ptr(), N, None, st)
+        assert torch.equal(x, y) and torch.equal(res, total), (R, N)
+        n = ops.rms_norm_bwd_workspace_bytes(R, N)
+        ws = torch.empty(max(1, n // 4), device=dev)
+        dw2 = torch.empty(N, device=dev)
+        for over in ("ds", "sum"):
+            sm, ds = total.clone(), i["ds"].clone()
+            out = ds if over == "ds" else sm
+            ops.rms_norm_bwd(code[dtype], code[stream], code[dtype], R, N, i["dy"].data_ptr(), N, sm.data_ptr(), N, rstd.data_ptr(),
+                             w.data_ptr(), ds.data_ptr(), N, out.data_ptr(), N, dw2.data_ptr(), ws.data_ptr(), n, st)
+            assert torch.equal(out, dx) and torch.equal(dw2, dw), (R, N, over)
+
+
 # ------------------------------------------------------------------------------------------------- gated recurrence
 # every way through time: single steps in order, tiles of 16 to 128 steps, many tiles, a split time axis, narrow rows of each, groups of
 # 8 and 16 threads, two workgroups per CU
