@@ -505,12 +505,13 @@ int serl_gated_scan_bwd(int type, int B, int T, int D, const void* gate, long lo
  * 1 <= N <= 32768; x and y of `type`; residual / sum of `stream_type` = type or fp32 (both NULL: s = x); weight of
  * `weight_type` = type or fp32.  y_fp8: y is OCP e4m3 bytes and scale (R) the fp32 it is to be multiplied with,
  * max(max |row| / 448, 2^-126), or 1 for a row of zeros; a row that holds a NaN has the scale NaN.  rstd (R) or NULL.  sum may be the residual
- * and y may be x. */
+ * and y may be x, their rows at the same addresses. */
 int serl_rms_norm_fwd(int type, int stream_type, int weight_type, int R, int N, const void* x, long long ldx,
                       const void* residual, long long ldres, const void* weight, float eps, void* y, long long ldy,
                       int y_fp8, float* scale, void* sum, long long ldsum, float* rstd, void* stream);
 /* dy of `type`; sum, ds (gradient of the stored sum, or NULL) and dx (the gradient of x and of the residual alike) of
- * `stream_type`; dweight (N) fp32, summed over the rows in a fixed order through the workspace; dx may be ds or sum. */
+ * `stream_type`; dweight (N) fp32, summed over the rows in a fixed order through the workspace; dx may be ds or sum, with the
+ * same row stride. */
 long long serl_rms_norm_bwd_workspace_bytes(int R, int N);
 int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int R, int N, const void* dy, long long lddy,
                       const void* sum, long long ldsum, const float* rstd, const void* weight, const void* ds,

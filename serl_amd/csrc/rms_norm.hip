@@ -450,6 +450,8 @@ extern "C" int serl_rms_norm_fwd(int type, int stream_type, int weight_type, int
   SERL_CHECK_ARG(!y_fp8 || scale, "rms_norm_fwd: 8-bit output needs the scales' buffer");
   SERL_CHECK_ARG(ldx >= 0 && ldres >= 0 && (R <= 1 || (ldy >= N && (!sum || ldsum >= N))),
                  "rms_norm_fwd: negative row stride, or output rows overlap");
+  SERL_CHECK_ARG(R <= 1 || ((y != x || ldy * (y_fp8 ? 1 : sq_size(type)) == ldx * sq_size(type)) && (!sum || sum != residual || ldsum == ldres)),
+                 "rms_norm_fwd: in place needs the same row stride");
   const int V = type == SERL_F32 ? 4 : 8;
   const bool wide = N % V == 0 && rms_wide(type, V, x, ldx) && rms_wide(stream_type, V, residual, ldres) &&
                     rms_wide(stream_type, V, sum, ldsum) && sq_aligned(weight, 16) &&
@@ -495,6 +497,7 @@ extern "C" int serl_rms_norm_bwd(int type, int stream_type, int weight_type, int
   SERL_CHECK_ARG(dweight && (R == 0 || (dy && sum && rstd && weight && dx)), "rms_norm_bwd: null pointer");
   SERL_CHECK_ARG(lddy >= 0 && ldsum >= 0 && ldds >= 0 && (R <= 1 || lddx >= N),
                  "rms_norm_bwd: negative row stride, or output rows overlap");
+  SERL_CHECK_ARG(R <= 1 || ((dx != ds || lddx == ldds) && (dx != sum || lddx == ldsum)), "rms_norm_bwd: in place needs the same row stride");
   const int V = type == SERL_F32 ? 4 : 8;
   const bool wide = N % V == 0 && rms_wide(type, V, dy, lddy) && rms_wide(stream_type, V, sum, ldsum) &&
                     rms_wide(stream_type, V, ds, ldds) && rms_wide(stream_type, V, dx, lddx) && sq_aligned(weight, 16);

@@ -1,0 +1,29 @@
+"""Calls of the operators of sequence policies that could only give wrong results are refused before anything is launched (no GPU
+needed: the pointers are never followed)."""
+import pytest
+
+from serl_amd import ops
+
+
+def norm_fwd(**k):
+    return ops.rms_norm_fwd(*{**dict(dtype=1, stream=1, weight=1, R=4, N=8, x=16, ldx=8, residual=32, ldres=8, w=48, eps=1e-6, y=64, ldy=8,
+                                     y_fp8=0, scale=None, sum=80, ldsum=8, rstd=None, st=0), **k}.values())
+
+
+def norm_bwd(**k):
+    return ops.rms_norm_bwd(*{**dict(dtype=1, stream=1, weight=1, R=4, N=8, dy=16, lddy=8, sum=32, ldsum=8, rstd=48, w=64, ds=80, ldds=8,
+                                     dx=96, lddx=8, dw=112, ws=None, n=0, st=0), **k}.values())
+
+
+def test_norm_in_place_at_another_row_stride():
+    for kw in (dict(y=16, ldy=9), dict(y=16, ldx=16), dict(y=16, ldx=0), dict(sum=32, ldsum=12), dict(sum=32, ldres=0),
+               dict(y=16, y_fp8=1, scale=96), dict(y=16, y_fp8=1, scale=96, ldy=8, ldx=8), dict(y=16, y_fp8=1, scale=96, ldy=16, ldx=16)):
+        with pytest.raises(ValueError, match="in place needs the same row stride"):
+            norm_fwd(**kw)
+    for kw in (dict(dx=80, lddx=9), dict(dx=80, ldds=0), dict(dx=32, ldsum=16), dict(dx=32, ds=None, ldsum=0)):
+        with pytest.raises(ValueError, match="in place needs the same row stride"):
+            norm_bwd(**kw)
+    # rows at the same addresses go on to the next check, the workspace's
+    for kw in (dict(dx=80), dict(dx=32), dict(dx=32, ldsum=9, lddx=9), dict(R=1, dx=80, lddx=9)):
+        with pytest.raises(ValueError, match="workspace"):
+            norm_bwd(**kw)
