@@ -377,8 +377,7 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
       rx[l].get(w[l]);
       rc[l] = rd[l];
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) scan_gate(g[v], k[l][v], rest[l][v]);
-      if (cuts) scan_cut<VEC>(k[l], cut >> l & 1, 0.f);
+      for (int v = 0; v < VEC; ++v) scan_gate(g[v], k[l][v], rest[l][v]);      // k stays f at a start: what it leads to is cut, below
     }
     float h = kept;
     {                                    // the tile before (none: nothing is read)
@@ -419,7 +418,6 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
     scan_join_tile<VEC, CG, WAVES, false>(kk, hh, h, all, hin, lds[buf][0], me.wave, me.lane);
     scan_join_tile<VEC, CG, WAVES, true>(k2, cc, carry, all, cin, lds[buf][1], me.wave, me.lane);
     // forwards: h_{t-1} of every step, folded at once into w = (h_{t-1} - x) f (1 - f); where an episode starts h_{t-1} is 0
-    // and f, which k no longer holds, is 1 - rest
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       float add[VEC];
@@ -434,7 +432,7 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
         asm volatile("");
         float old[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) old[v] = -add[v] * (1.f - rest[l][v]);
+        for (int v = 0; v < VEC; ++v) old[v] = -add[v] * k[l][v];
         scan_cut<VEC>(w[l], cut >> l & 1, old);
         scan_cut<VEC>(hin, cut >> l & 1, add);
       }

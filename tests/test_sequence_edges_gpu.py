@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_sequence_gpu import DTYPES, norm_inputs, seq
+from test_sequence_gpu import DTYPES, HALF, SMALL, U, norm_inputs, scan_inputs, seq, within
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,33 @@ def test_gates_of_zero_do_not_hide_a_nan(dev, T):
     assert bool(y[0, :, 7].isnan().all()) and bool(h[0, 7].isnan())
     y[0, :, 7] = h[0, 7] = 1
     assert bool((y == 1).all()) and bool((h == 1).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", [(2, 6, 16), (2, 70, 16), (3, 200, 40), (1, 1500, 24), (2, 90, 3)])
+def test_gate_gradient_at_a_start_keeps_small_gates(dev, dtype, B, T, D):
+    """At an episode's first step dgate = -G x f (1 - f), to the relative accuracy of f: gates far below 0 too."""
+    s = seq()
+    i = scan_inputs(dev, dtype, B, T, D, T, h0=True)
+    starts = torch.zeros((B, T), dtype=torch.bool, device=dev)
+    starts[:, ::5] = True
+    gate = i["gate"].clone()
+    gate[:, ::5] = torch.tensor([-10.0, -17.0, -30.0, -60.0, 4.0], device=dev).to(dtype)[torch.arange(D, device=dev) % 5]
+    _, _, saved = s.gated_scan(gate, i["x"], i["h0"], starts=starts, save=True)
+    dgate, _, _ = s.gated_scan_backward(gate, i["x"], saved, i["dy"], i["dh_last"], starts=starts)
+    z, x, dy = (t.double().cpu() for t in (gate, i["x"], i["dy"]))
+    keep = torch.sigmoid(z) * ~starts.cpu()[..., None]
+    f, rest = torch.sigmoid(z), torch.sigmoid(-z)
+    C = i["dh_last"].double().cpu()
+    size, want, tol = C.abs(), torch.zeros_like(z), torch.zeros_like(z)
+    for t in range(T - 1, -1, -1):
+        G, big = dy[:, t] + C, dy[:, t].abs() + size
+        want[:, t] = -G * x[:, t] * f[:, t] * rest[:, t]
+        # f and 1 - f: the exponent's |z| roundings and 4 more each, 3 products; G: at most 5 steps back to the next start, each with f's
+        # roundings, a product and a sum, and the joins of threads, waves and tiles on the way (2 each, 16 at most), of the sum's size
+        tol[:, t] = ((2 * z[:, t].abs() + 11) * G.abs() + (5 * (4 + 4 + 2) + 32) * big) * U * (x[:, t] * f[:, t] * rest[:, t]).abs()
+        C, size = keep[:, t] * G, keep[:, t] * big
+    at = starts.cpu()[..., None].expand(B, T, D)
+    # a stored value's own rounding, or half a step among the type's smallest numbers
+    least = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: SMALL}[dtype]
+    within(dgate.cpu()[at], want[at], (tol + HALF[dtype] * want.abs() + least)[at], "dgate")
