@@ -182,3 +182,72 @@ def test_gate_gradient_at_a_start_keeps_small_gates(dev, dtype, B, T, D):
     # a stored value's own rounding, or half a step among the type's smallest numbers
     least = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: SMALL}[dtype]
     within(dgate.cpu()[at], want[at], (tol + HALF[dtype] * want.abs() + least)[at], "dgate")
+
+
+# --------------------------------------------------------------------------------------- the recurrence, element by element
+def running(i):
+    """The recurrence and its gradients in 64 bits, with what a count of roundings makes of each element: (values, bounds)."""
+    z, x, dy = (i[k].double().cpu() for k in ("gate", "x", "dy"))
+    B, T, D = z.shape
+    live = torch.ones((B, T, 1), dtype=torch.bool)
+    if i["lengths"] is not None:
+        live = (torch.arange(T)[None] < i["lengths"].cpu().long()[:, None])[..., None]
+    go = torch.ones((B, T, 1), dtype=torch.float64)
+    if i["starts"] is not None:
+        go = (~i["starts"].cpu())[..., None].double()
+    f, rest = torch.sigmoid(z), torch.sigmoid(-z)
+    # per step: f or 1 - f (its exponent's |z| roundings and 4 more), the product and the sum; 2 more for the joins that a tile hands on to
+    # the next one, 40 roundings in 64 steps or more
+    c = (z.abs() + 8) * U
+    h = torch.zeros((B, D), dtype=torch.float64) if i["h0"] is None else i["h0"].double().cpu()
+    size, err = h.abs(), torch.zeros_like(h)
+    out, tol = {}, {}
+    ys, ye, hs, he = [], [], [], []
+    for t in range(T):
+        k = f[:, t] * go[:, t]
+        hs.append(h * go[:, t])
+        # the tree of joins a state comes through: 4 levels in a wave, 16 waves, 2 roundings each
+        he.append((err + 40 * U * size) * go[:, t])
+        n, m = k * h + rest[:, t] * x[:, t], k * size + rest[:, t] * x[:, t].abs()
+        e = k * err + c[:, t] * m
+        h, size, err = (torch.where(live[:, t], u, v) for u, v in ((n, h), (m, size), (e, err)))
+        ys.append(torch.where(live[:, t], h, torch.zeros_like(h)))
+        ye.append(err + 40 * U * size)
+    out["y"], tol["y"] = torch.stack(ys, 1), torch.stack(ye, 1)
+    out["h_last"], tol["h_last"] = h, err + 40 * U * size
+    C = i["dh_last"].double().cpu()
+    size, err = C.abs(), torch.zeros_like(C)
+    dg, dge, dx, dxe = ([None] * T for _ in range(4))
+    for t in range(T - 1, -1, -1):
+        lv = live[:, t]
+        G, m, e = dy[:, t] + C, dy[:, t].abs() + size, err + U * (dy[:, t].abs() + size)
+        eg = e + 40 * U * m
+        ff, w = f[:, t] * rest[:, t], hs[t] - x[:, t]
+        we = he[t] + U * (hs[t].abs() + x[:, t].abs())
+        dg[t] = torch.where(lv, G * w * ff, torch.zeros_like(G))
+        dge[t] = (eg * (w.abs() + we) + G.abs() * we + (2 * z[:, t].abs() + 12) * U * (G * w).abs()) * ff
+        dx[t] = torch.where(lv, G * rest[:, t], torch.zeros_like(G))
+        dxe[t] = (eg + (z[:, t].abs() + 6) * U * G.abs()) * rest[:, t]
+        k = f[:, t] * go[:, t]
+        C, size, err = (torch.where(lv, u, v) for u, v in ((k * G, C), (k * m, size), (k * e + c[:, t] * k * m, err)))
+    for name, v, e in (("dgate", dg, dge), ("dx", dx, dxe)):
+        out[name], tol[name] = torch.stack(v, 1), torch.stack(e, 1)
+    out["dh0"], tol["dh0"] = C, err + 40 * U * size
+    return out, tol
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("B,T,D", [(2, 5, 7), (2, 8, 64), (2, 14, 24), (3, 31, 24), (2, 60, 40), (2, 129, 33), (3, 257, 96), (1, 1100, 8),
+                                   (2, 1537, 19), (2, 300, 3), (2, 900, 3), (40, 650, 256), (300, 100, 130)])
+def test_gated_scan_within_the_roundings_of_each_element(dev, dtype, B, T, D):
+    """Bounds that follow each element's own size, where those of test_gated_scan_matches_the_recurrence take the largest."""
+    s = seq()
+    for k, opt in enumerate(({}, {"starts": True}, {"starts": True, "lengths": True})):
+        i = scan_inputs(dev, dtype, B, T, D, 7 * k + T + D, **opt)
+        want, tol = running(i)
+        y, h, saved = s.gated_scan(i["gate"], i["x"], i["h0"], i["starts"], i["lengths"], save=True)
+        dg, dx, d0 = s.gated_scan_backward(i["gate"], i["x"], saved, i["dy"], i["dh_last"], i["starts"], i["lengths"])
+        least = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: SMALL}[dtype]
+        for name, got in (("y", y), ("h_last", h), ("dgate", dg), ("dx", dx), ("dh0", d0)):
+            stored = HALF[dtype] * want[name].abs() + least if got.dtype == dtype and dtype != torch.float32 else 2.0 ** -149
+            within(got, want[name], tol[name] * (1 + 2.0 ** -6) + stored, name)
