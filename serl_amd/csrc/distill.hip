@@ -115,7 +115,8 @@ __device__ __forceinline__ DistTeacher dist_tables(float* lds, int K, int buf) {
 __device__ __forceinline__ long long dist_column(const DistArgs& a, int row, int k) {
   return a.index64 ? ((const long long*)a.index)[row * a.ldi + k] : (long long)((const int*)a.index)[row * a.ldi + k];
 }
-// By one wave.  A slot is absent if its column is outside [0, V) or its logit is -inf; NaN and +inf are carried on.
+// By one wave.  A slot is absent if its column is outside [0, V) or its logit is -inf; NaN and +inf are carried on.  As with the
+// student, differences are taken before the temperature: slots that all hold the type's lowest value weigh the same.
 // TAKEN: the student's logits are those that dist_stats_kernel took (the row may be half overwritten by now).
 // Returns whether any slot is there.
 template <typename T, bool TAKEN>
@@ -132,16 +133,16 @@ __device__ __forceinline__ bool dist_stage(const DistArgs& a, int row, const Dis
     const bool ok = id >= 0 && id < a.V && !(tv == -INFINITY);
     const float lg = TAKEN ? a.taken[(long long)row * a.K + k] : sq_val(T(), logits[ok ? id : 0]);
     d.idx[k] = ok ? (int)id : -1;
-    d.q[k] = tv * inv;
+    d.q[k] = tv;
     d.lg[k] = lg;
-    top = ok ? fmaxf(top, tv * inv) : top;
+    top = ok ? fmaxf(top, tv) : top;
     any |= ok;
   }
   top = sq_wave_max(top);
   float sum = 0.f;
 #pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
-    const float e = d.idx[k] >= 0 ? expf(d.q[k] - top) : 0.f;
+    const float e = d.idx[k] >= 0 ? expf((d.q[k] - top) * inv) : 0.f;
     d.q[k] = e;
     sum += e;
   }
@@ -180,10 +181,9 @@ template <typename T>
 __device__ __forceinline__ bool dist_finish(const DistArgs& a, const DistSlot& c, typename T::bits lg, const DistTeacher& d, int lane) {
   float tv;
   const bool ok = dist_there<T>(a, c, lane, tv);
-  tv *= 1.f / a.tau;
   float top = ok ? fmaxf(-INFINITY, tv) : -INFINITY;
   top = sq_wave_max(top);
-  const float e = ok ? expf(tv - top) : 0.f, sum = sq_wave_sum(e);
+  const float e = ok ? expf((tv - top) * (1.f / a.tau)) : 0.f, sum = sq_wave_sum(e);
   if (lane < a.K) {
     d.idx[lane] = ok ? (int)dist_id(a, c) : -1;
     d.q[lane] = ok ? e * (1.f / sum) : 0.f;

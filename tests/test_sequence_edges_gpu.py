@@ -251,3 +251,45 @@ def test_gated_scan_within_the_roundings_of_each_element(dev, dtype, B, T, D):
         for name, got in (("y", y), ("h_last", h), ("dgate", dg), ("dx", dx), ("dh0", d0)):
             stored = HALF[dtype] * want[name].abs() + least if got.dtype == dtype and dtype != torch.float32 else 2.0 ** -149
             within(got, want[name], tol[name] * (1 + 2.0 ** -6) + stored, name)
+
+
+# -------------------------------------------------------------------------------------------- top-logit distillation
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("tau", [0.5, 2.0 ** -20, 1.0, 3.0])
+@pytest.mark.parametrize("R,V,K", [(6, 300, 6), (6, 12, 6), (6, 3000, 100), (6, 9001, 7), (150, 20000, 130), (6, 170000, 9)])
+def test_teachers_at_the_ends_of_their_type(dev, dtype, tau, R, V, K):
+    """Differences of a teacher's logits count, whatever their size over the temperature: slots that all hold the type's lowest (or the
+    same largest) value weigh the same, one above the others' lowest takes everything."""
+    s = seq()
+    low, top = torch.finfo(dtype).min, torch.finfo(dtype).max
+    g = torch.Generator().manual_seed(V)
+    # a student whose columns lie within 4 tau of each other
+    logits = (torch.rand((R, V), generator=g) * 4 * tau).to(dtype).to(dev)
+    index = torch.stack([torch.randperm(V, generator=g)[:K] if K <= V else torch.arange(K) for _ in range(R)]).to(dev)
+    teacher = torch.zeros((R, K), dtype=dtype, device=dev)
+    q = torch.full((R, K), 1 / K, dtype=torch.float64)
+    teacher[0] = low
+    teacher[1] = top
+    teacher[2] = low
+    teacher[2, K - 1] = 0
+    q[2] = 0
+    q[2, K - 1] = 1
+    teacher[3] = 1e30
+    teacher[4] = low
+    teacher[4, 1] = top
+    q[4] = 0
+    q[4, 1] = 1
+    teacher[5] = low
+    teacher[5, ::2] = -math.inf
+    q[5] = 0
+    q[5, 1::2] = 1 / len(range(1, K, 2))
+    loss, d = s.topk_distill(logits, teacher, index, temperature=tau)
+    logp = torch.log_softmax(logits.double().cpu() / tau, 1)
+    want = tau * torch.exp(logp).scatter_add(1, index.cpu(), -q)
+    # p and q <= 1: exponents of at most 4 with 3 roundings each, sums of up to 100 in a row (as check_distill), 1 for the difference
+    n = (3 * 4 + 120) * U
+    within(d, want, tau * n * (torch.exp(logp) + torch.zeros_like(logp).scatter_add(1, index.cpu(), q)) + HALF[dtype] * want.abs(), "dlogits")
+    lp = logp.gather(1, index.cpu())
+    rl = tau * tau * (torch.special.xlogy(q, q) - q * lp).sum(1)
+    # log q, log p of at most 5 + log V <= 18, summed over at most 130 slots
+    within(loss, rl, tau * tau * (n + (K + 20) * U) * 18, "loss")
