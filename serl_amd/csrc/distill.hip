@@ -191,14 +191,15 @@ __device__ __forceinline__ bool dist_finish(const DistArgs& a, const DistSlot& c
   }
   return __any(ok);
 }
-// loss without c tau^2, by the wave that staged the teacher
+// The loss over c tau, by the wave that staged the teacher: sum of q (tau (log q + log sum) - (logit - m)).  A column's logit is not scaled
+// by 1 / tau and log2(e) on the way, which the type's lowest value (a masked column) would not bear.
 __device__ __forceinline__ float dist_loss(const DistArgs& a, const DistTeacher& d, float m, float sum, int lane) {
-  const float k2 = DIST_LOG2E / a.tau, l2 = log2f(sum);
+  const float lsum = log2f(sum) * DIST_LN2;
   float s = 0.f;
 #pragma unroll 1
   for (int k = lane; k < a.K; k += 64) {
     const float q = d.q[k];
-    s += q == 0.f ? 0.f : q * (logf(q) - ((d.lg[k] - m) * k2 - l2) * DIST_LN2);
+    s += q == 0.f ? 0.f : q * (a.tau * (logf(q) + lsum) - (d.lg[k] - m));
   }
   return sq_wave_sum(s);
 }
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(THREADS) void dist_row_kernel(const DistArgs a) {
     const bool dead = !any_slot || c == 0.f;
     if (wave == 0) {
       const float l = dist_loss(a, dist_tables(tables, a.K, tab), m, s, lane);
-      if (lane == 0) a.loss[row] = dead ? 0.f : c * a.tau * a.tau * l;
+      if (lane == 0) a.loss[row] = dead ? 0.f : c * a.tau * l;
     }
     const int next = row + (int)gridDim.x;
     const bool more = next < a.R;
@@ -475,7 +476,7 @@ __global__ __launch_bounds__(DIST_CUT + 64) void dist_grad_kernel(const DistArgs
     if (lane == 0) alive = any;
     if (piece == 0) {
       const float l = dist_loss(a, d, m, s, lane);
-      if (lane == 0) a.loss[row] = any && c != 0.f ? c * a.tau * a.tau * l : 0.f;
+      if (lane == 0) a.loss[row] = any && c != 0.f ? c * a.tau * l : 0.f;
     }
   } else if (a.dlogits && c != 0.f) {
     for (int jb = j0; jb < j1; jb += DIST_CUT * U) {

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_sequence_gpu import DTYPES, HALF, SMALL, U, norm_inputs, scan_inputs, seq, within
+from test_sequence_gpu import DTYPES, HALF, SMALL, U, distill_reference, norm_inputs, scan_inputs, seq, within
 
 pytestmark = pytest.mark.gpu
 
@@ -293,3 +293,28 @@ def test_teachers_at_the_ends_of_their_type(dev, dtype, tau, R, V, K):
     rl = tau * tau * (torch.special.xlogy(q, q) - q * lp).sum(1)
     # log q, log p of at most 5 + log V <= 18, summed over at most 130 slots
     within(loss, rl, tau * tau * (n + (K + 20) * U) * 18, "loss")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tau", [0.25, 1.0, 2.0])
+@pytest.mark.parametrize("R,V,K", [(4, 300, 6), (4, 12, 6), (4, 3000, 100), (150, 20000, 70), (4, 170000, 9)])
+def test_loss_of_a_column_that_holds_the_lowest_value(dev, dtype, tau, R, V, K):
+    """A student's column at the type's lowest value is masked, not impossible: tau q |low| is the loss, finite where the type of the
+    sum holds it."""
+    s = seq()
+    low = torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn((R, V), generator=g).to(dtype).to(dev)
+    index = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(R)]).to(dev)
+    teacher = torch.randn((R, K), generator=g).to(dtype).to(dev)
+    logits[0, index[0, 2]] = low
+    logits[1, index[1, :3]] = low
+    coef = torch.full((R,), 0.25, device=dev)
+    i = dict(logits=logits, teacher=teacher, index=index, coef=coef)
+    rl, _, q, lp, _ = distill_reference(i, tau)
+    loss, d = s.topk_distill(logits, teacher, index, temperature=tau, coef=coef)
+    assert bool((rl[:2] > 0.2 * tau * -low * q.gather(1, torch.full((R, 1), 2))[:2, 0]).all()) and bool(d.isfinite().all())
+    # the terms are all above 0 but for log q: q's roundings (exponents of at most 12 / tau, K slots), those of log p (200 as for the
+    # gradient, its own and the products)
+    size = 0.25 * tau * tau * (q * (torch.log(q.clamp_min(1e-300)).abs() + lp.abs())).sum(1)
+    within(loss, rl, (3 * 12 / tau + K + 230) * U * size, "loss")
