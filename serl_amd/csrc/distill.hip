@@ -641,7 +641,8 @@ extern "C" int serl_topk_distill(int type, int teacher_type, int index64, int R,
   const long long need = dist_ws(p, R, K);
   SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                  "topk_distill: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
-  SERL_CHECK_ARG((long long)R * p.pieces <= 0x7fffffffll, "topk_distill: too many rows");
+  SERL_CHECK_ARG(p.pieces == 1 || (long long)R * p.pieces * (DIST_CUT + 64) < (1ll << 32),      // a launch has less than 2^32 threads
+                 "topk_distill: too many rows of this length: R at most %lld", ((1ll << 32) - 1) / (DIST_CUT + 64) / p.pieces);
   DistArgs a{};
   a.logits = logits; a.ldl = ldl; a.teacher = teacher; a.ldt = ldt; a.index = index; a.ldi = ldi; a.dlogits = dlogits;
   a.ldd = ldd; a.coef = coef; a.loss = loss; a.part = workspace;

@@ -27,3 +27,18 @@ def test_norm_in_place_at_another_row_stride():
     for kw in (dict(dx=80), dict(dx=32), dict(dx=32, ldsum=9, lddx=9), dict(R=1, dx=80, lddx=9)):
         with pytest.raises(ValueError, match="workspace"):
             norm_bwd(**kw)
+
+
+def distill(**k):
+    return ops.topk_distill(*{**dict(dtype=1, tt=1, i64=1, R=4, V=9, K=3, logits=16, ldl=0, teacher=16, ldt=0, index=16, ldi=0, tau=1.0,
+                                     coef=None, loss=16, d=None, ldd=0, ws=16, n=1 << 60, st=0), **k}.values())
+
+
+def test_distillation_of_more_long_rows_than_a_launch():
+    """Expanded logits alone make so many: rows of 163 841 16-bit columns are cut in 6 pieces of 320 threads."""
+    most = (2 ** 32 - 1) // 320 // 6
+    for R in (most + 1, 2 ** 24, 2 ** 31 - 2 ** 16):
+        with pytest.raises(ValueError, match=f"too many rows of this length: R at most {most}"):
+            distill(R=R, V=163841)
+    with pytest.raises(ValueError, match="R at most"):
+        distill(dtype=0, tt=0, R=2 ** 24, V=2 ** 29)
