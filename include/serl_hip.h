@@ -492,7 +492,8 @@ int serl_gated_scan_fwd(int type, int B, int T, int D, const void* gate, long lo
                         const void* x, long long x_bs, long long x_ts, const float* h0, const unsigned char* starts,
                         long long starts_bs, const int* lengths, void* y, long long y_bs, long long y_ts, float* h_last,
                         float* states, float* workspace, long long workspace_bytes, void* stream);
-/* dy (B, T, D), dh_last (B, D) or NULL -> dgate, dx (B, T, D), dh0 (B, D); T >= 1; the outputs overlap no input */
+/* dy (B, T, D), dh_last (B, D) or NULL -> dgate, dx (B, T, D), dh0 (B, D); T >= 1; the outputs' rows overlap neither
+ * each other (refused) nor an input */
 int serl_gated_scan_bwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,
                         const void* x, long long x_bs, long long x_ts, const unsigned char* starts, long long starts_bs,
                         const int* lengths, const float* states, const void* dy, long long dy_bs, long long dy_ts,

@@ -708,6 +708,29 @@ static bool scan_fits(const ScanPlan& p, int type, int B, int T) {
   return (long long)B * p.nseg * p.ndb < (1ll << 32) / threads;
 }
 
+// Rows of D elements of one output that share no memory with each other: sequences of steps, or steps of sequences.
+static bool scan_apart(long long B, long long T, long long D, long long bs, long long ts) {
+  if (B <= 1 || T <= 1) return (B <= 1 || bs >= D) && (T <= 1 || ts >= D);
+  return bs >= D && ts >= D && (bs >= (T - 1) * (__int128)ts + D || ts >= (B - 1) * (__int128)bs + D);
+}
+// Whether two outputs whose rows lie alike, `delta` elements from each other, share memory: some |delta + b bs + t ts| < D with |b| < B,
+// |t| < T.  One of the two strides spans all of the other (scan_apart), so of each the multiples next to what is left come in question.
+static bool scan_meet(long long delta, long long B, long long T, long long D, long long bs, long long ts) {
+  const __int128 span = (B > 1 ? (B - 1) * (__int128)bs : 0) + (T > 1 ? (T - 1) * (__int128)ts : 0) + D;
+  if (delta >= span || -delta >= span) return false;      // two buffers
+  const bool time = B <= 1 || (T > 1 && ts > bs);      // the wider stride is that of time
+  const __int128 n1 = time ? T : B, n2 = time ? B : T, s1 = time ? ts : bs, s2 = time ? bs : ts;
+  for (int i = -1; i <= 1; ++i) {
+    const __int128 k1 = n1 > 1 ? -delta / s1 + i : i, left = delta + k1 * s1;
+    if (k1 <= -n1 || k1 >= n1) continue;
+    for (int j = -1; j <= 1; ++j) {
+      const __int128 k2 = n2 > 1 ? -left / s2 + j : j, d = left + k2 * s2;
+      if (k2 > -n2 && k2 < n2 && -D < d && d < D) return true;
+    }
+  }
+  return false;
+}
+
 #define SCAN_SHORT 8        // up to this many steps one thread runs them in order: a tile would be mostly empty
 
 extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* gate, long long gate_bs, long long gate_ts,
@@ -723,6 +746,7 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG(gate_bs >= 0 && gate_ts >= 0 && x_bs >= 0 && x_ts >= 0 && (!starts || starts_bs >= 0),
                  "gated_scan_fwd: negative stride");
   SERL_CHECK_ARG((T <= 1 || y_ts >= D) && (T == 0 || B <= 1 || y_bs >= D), "gated_scan_fwd: rows of y overlap");
+  SERL_CHECK_ARG(T <= SCAN_SHORT || h_last != h0, "gated_scan_fwd: h_last may be h0 for up to %d steps", SCAN_SHORT);
   SERL_CHECK_ARG(T < SCAN_MAXT, "gated_scan_fwd: T too large");
   const bool few = T <= SCAN_SHORT;
   const bool wide = few ? D * sq_size(type) % 16 == 0 && scan_rows(type, 16, gate, gate_bs, gate_ts) &&
@@ -731,6 +755,9 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG(few ? (long long)B * (wide ? D * sq_size(type) / 16 : D) < (1ll << 32) - SCAN_THREADS : scan_fits(p, type, B, T),
                  "gated_scan_fwd: B * D too large");
+  SERL_CHECK_ARG(few || (scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, y_ts)),
+                 "gated_scan_fwd: 15 steps of a tensor must span less than 2^31 bytes");
+  SERL_CHECK_ARG(T == 0 || scan_apart(B, T, D, y_bs, y_ts), "gated_scan_fwd: rows of y overlap");
   ScanArgs a{};
   a.gate = gate; a.gate_bs = gate_bs; a.gate_ts = gate_ts; a.x = x; a.x_bs = x_bs; a.x_ts = x_ts;
   a.y = y; a.y_bs = y_bs; a.y_ts = y_ts; a.h0 = h0; a.h_last = h_last; a.starts = starts; a.starts_bs = starts_bs;
@@ -743,8 +770,6 @@ extern "C" int serl_gated_scan_fwd(int type, int B, int T, int D, const void* ga
     else if (type == SERL_BF16) scan_launch_short<BF16>(a, wide, st);
     else scan_launch_short<F16>(a, wide, st);
   } else {
-    SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, y_ts),
-                   "gated_scan_fwd: 15 steps of a tensor must span less than 2^31 bytes");
     const long long need = scan_ws(p, B, D);
     SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                    "gated_scan_fwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);
@@ -780,6 +805,10 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
   SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
                  scan_reach(type, false, D, dgate_ts) && scan_reach(type, false, D, dx_ts),
                  "gated_scan_bwd: 15 steps of a tensor must span less than 2^31 bytes");
+  SERL_CHECK_ARG(scan_apart(B, T, D, dgate_bs, dgate_ts) && scan_apart(B, T, D, dx_bs, dx_ts) && dgate != dx &&
+                     ((B > 1 && dgate_bs != dx_bs) || (T > 1 && dgate_ts != dx_ts) ||
+                      !scan_meet(((const char*)dx - (const char*)dgate) / sq_size(type), B, T, D, dgate_bs, dgate_ts)),
+                 "gated_scan_bwd: rows of dgate or dx overlap");
   const long long need = scan_ws(p, B, D);
   SERL_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                  "gated_scan_bwd: workspace of %lld bytes needed, %lld available", need, workspace ? workspace_bytes : 0);

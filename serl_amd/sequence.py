@@ -161,7 +161,7 @@ def gated_scan(gate, x, h0=None, starts=None, lengths=None, save=False):
 def gated_scan_backward(gate, x, saved, dy, dh_last=None, starts=None, lengths=None, out=None):
     """Gradients of gated_scan: (dgate, dx) in gate's type, dh0 (B, D) float32.  `saved` and the other arguments as in the
     forward call; dy (B, T, D), dh_last (B, D) float32 or None.  out: (dgate, dx) tensors to write, for instance the two
-    halves of one projection's gradient; they share no memory with the inputs."""
+    halves of one projection's gradient; they share no memory with each other or the inputs."""
     B, T, D = _scan_args(gate, x, starts, lengths)
     _shape(saved, "saved", (B, -(-T // 64), D))
     _type(saved, "saved", torch.float32)

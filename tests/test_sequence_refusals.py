@@ -42,3 +42,42 @@ def test_distillation_of_more_long_rows_than_a_launch():
             distill(R=R, V=163841)
     with pytest.raises(ValueError, match="R at most"):
         distill(dtype=0, tt=0, R=2 ** 24, V=2 ** 29)
+
+
+def scan_fwd(**k):
+    return ops.gated_scan_fwd(*{**dict(dtype=0, B=2, T=5000, D=8, gate=16, gate_bs=40000, gate_ts=8, x=16, x_bs=40000, x_ts=8, h0=None, starts=None,
+                                       starts_bs=0, lengths=None, y=16, y_bs=40000, y_ts=8, h_last=16, states=None, ws=None, n=0, st=0), **k}.values())
+
+
+def scan_bwd(**k):
+    return ops.gated_scan_bwd(*{**dict(dtype=0, B=2, T=5000, D=8, gate=16, gate_bs=40000, gate_ts=8, x=16, x_bs=40000, x_ts=8, starts=None,
+                                       starts_bs=0, lengths=None, states=16, dy=16, dy_bs=40000, dy_ts=8, dh_last=None, dgate=1 << 20,
+                                       dgate_bs=40000, dgate_ts=8, dx=1 << 21, dx_bs=40000, dx_ts=8, dh0=16, ws=None, n=0, st=0), **k}.values())
+
+
+def test_recurrence_whose_outputs_share_memory():
+    # rows of one output: sequences a step apart, the last step over the next sequence's first
+    for bs, ts in ((8, 8), (39996, 8), (7, 40000), (8, 15), (0, 8), (40000, 0)):
+        with pytest.raises(ValueError, match="rows of y overlap"):
+            scan_fwd(y_bs=bs, y_ts=ts)
+        with pytest.raises(ValueError, match="rows of dgate or dx overlap"):
+            scan_bwd(dgate_bs=bs, dgate_ts=ts)
+        with pytest.raises(ValueError, match="rows of dgate or dx overlap"):
+            scan_bwd(dx_bs=bs, dx_ts=ts)
+    # the two outputs over each other: the same tensor, halves that are not apart, one a step or a sequence on, time-major ones
+    at, half = 1 << 20, dict(dgate_bs=80000, dgate_ts=16, dx_bs=80000, dx_ts=16)
+    for kw in (dict(dx=at), dict(dx=at, dx_ts=16, dx_bs=80000), dict(dx=at + 4), dict(dx=at + 32 * 4999), dict(dx=at - 32), dict(dx=at + 40000 * 4),
+               dict(half, dx=at + 28), dict(half, dx=at + 64 * 17 - 4), dict(half, dx=at - 80000 * 4 + 64),
+               dict(dgate_bs=8, dgate_ts=16, dx_bs=8, dx_ts=16, dx=at + 32)):
+        with pytest.raises(ValueError, match="rows of dgate or dx overlap"):
+            scan_bwd(**kw)
+    # outputs that lie apart go on to the next check, the workspace's
+    for kw in (dict(), dict(half, dx=at + 32), dict(half, dx=at - 32), dict(half, dx=at + 64 * 17 + 32), dict(dx=at + 40000 * 2 * 4),
+               dict(dgate_bs=8, dgate_ts=32, dx_bs=8, dx_ts=32, dx=at + 64)):
+        with pytest.raises(ValueError, match="workspace"):
+            scan_bwd(**kw)
+    for bs, ts in ((40000, 8), (8, 16), (8, 64), (80000, 16)):
+        with pytest.raises(ValueError, match="workspace"):
+            scan_fwd(y_bs=bs, y_ts=ts)
+    with pytest.raises(ValueError, match="h_last may be h0 for up to 8 steps"):
+        scan_fwd(h0=16)
