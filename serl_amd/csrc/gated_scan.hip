@@ -175,27 +175,43 @@ struct ScanSpot {
 };
 
 // One (B, T, D) tensor as a wave sees it: `base` is its sequence (uniform), `off` the thread's byte offset from its wave's
-// first row, or behind everything for channels that do not exist.
-template <typename T, int VEC, int L, typename Spot>
+// first row, or behind everything for channels that do not exist.  FAR (VEC = 1, where a wave's rows are one thread's):
+// steps may lie any distance apart; beyond 2^27 bytes each row is addressed by itself (done always, narrow rows took 1.3 to 1.7 times as long).
+template <typename T, int VEC, int L, typename Spot, bool FAR = false>
 struct ScanRows {
   const char* base;
   long long ts;          // bytes from step to step
   uint32_t off;
+  __device__ __forceinline__ bool far() const { return FAR && VEC == 1 && ts > 1 << 27; }
   __device__ __forceinline__ ScanRows(const Spot& me, const void* p, long long bs, long long step) {
     constexpr int E = sizeof(typename T::bits);
     base = (const char*)p + me.b * bs * E;
     ts = step * E;
+    static_assert(VEC > 1 || (Spot::ROWS == L && L <= 8), "a wave's rows are each thread's; seven steps and a row are below 2^31 bytes");
     off = me.dok ? (uint32_t)(me.first * ts) + (uint32_t)(me.d0 * E) : SQ_NOWHERE;
   }
   // the wave's rows from step t on, as far as they are before `te` (a row is D wide)
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int t, int te, int D) const {
     const int rows = min(te - t, Spot::ROWS);
-    return sq_buffer(base + t * ts, rows > 0 ? (rows - 1) * (int)ts + D * (int)sizeof(typename T::bits) : 0);
+    return sq_buffer(base + t * ts, rows > 0 ? (int)((uint32_t)(rows - 1) * (uint32_t)ts + (uint32_t)(D * (int)sizeof(typename T::bits))) : 0);
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t one(int t, int te, int D) const {
+    return sq_buffer(base + t * ts, t < te ? D * (int)sizeof(typename T::bits) : 0);
   }
   template <bool STREAM = false> __device__ __forceinline__ void fetch(Raw<T, VEC> (&r)[L], int t, int te, int D) const {
-    const __amdgpu_buffer_rsrc_t b = at(t, te, D);
+    if (far()) {
 #pragma unroll
-    for (int l = 0; l < L; ++l) sq_load<STREAM>(r[l], b, off + l * (uint32_t)ts);
+      for (int l = 0; l < L; ++l) sq_load<STREAM>(r[l], one(t + l, te, D), off);
+    } else {
+      const __amdgpu_buffer_rsrc_t b = at(t, te, D);
+#pragma unroll
+      for (int l = 0; l < L; ++l) sq_load<STREAM>(r[l], b, off + l * (uint32_t)ts);
+    }
+  }
+  // row l of those from step t on, `b` = at(t, te, D)
+  template <bool STREAM> __device__ __forceinline__ void put(const Raw<T, VEC>& r, __amdgpu_buffer_rsrc_t b, int l, int t, int te, int D) const {
+    if (far()) sq_store<STREAM>(r, one(t + l, te, D), off);
+    else sq_store<STREAM>(r, b, off + l * (uint32_t)ts);
   }
 };
 
@@ -317,7 +333,7 @@ __global__ __launch_bounds__(THREADS) void scan_fwd_kernel(const ScanArgs a) {
         Raw<T, VEC> r;
         r.put(c);
         if (!whole) scan_mask(r, t + l < me.len, 0);
-        sq_store<STREAM == 2>(r, out, y.off + l * (uint32_t)y.ts);
+        y.template put<STREAM == 2>(r, out, l, tw, me.te, a.D);
       }
     }
   }
@@ -342,7 +358,7 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
   __shared__ __attribute__((aligned(16))) float lds[2][2][WAVES * 2 * VEC * CG];
   typedef ScanSpot<VEC, CG, L> Spot;
   const Spot me(a);
-  typedef ScanRows<T, VEC, L, Spot> Rows;
+  typedef ScanRows<T, VEC, L, Spot, true> Rows;
   const Rows gate(me, a.gate, a.gate_bs, a.gate_ts), x(me, a.x, a.x_bs, a.x_ts), dy(me, a.dy, a.dy_bs, a.dy_ts);
   const Rows dgate(me, a.dgate, a.dgate_bs, a.dgate_ts), dx(me, a.dx, a.dx_bs, a.dx_ts);
   const unsigned char* starts = a.starts ? a.starts + me.b * a.starts_bs : nullptr;
@@ -459,8 +475,8 @@ __global__ __launch_bounds__(THREADS) void scan_bwd_kernel(const ScanArgs a) {
         scan_mask(r1, t + l < me.len, 0);
         scan_mask(r2, t + l < me.len, 0);
       }
-      sq_store<STREAM>(r1, og, dgate.off + l * (uint32_t)dgate.ts);
-      sq_store<STREAM>(r2, ox, dx.off + l * (uint32_t)dx.ts);
+      dgate.template put<STREAM>(r1, og, l, tw, me.te, a.D);
+      dx.template put<STREAM>(r2, ox, l, tw, me.te, a.D);
     }
   }
   if (me.seg == 0 && me.chok) a.dh0[state] = carry;
@@ -618,7 +634,8 @@ extern "C" long long serl_gated_scan_states_floats(int B, int T, int D) {
   return (long long)B * cdivll(T, SCAN_CKPT) * D;
 }
 
-// A wave addresses its rows of a tile (at most 32; narrow: 16) with 31-bit byte offsets from the first.
+// A wave addresses its rows of a tile (wide: at most 32, narrow: 8) with 31-bit byte offsets from the first.  Up to SCAN_SHORT steps there
+// is no limit: the forward pass runs them in order, the backward pass addresses far rows one by one (ScanRows).
 static bool scan_reach(int type, bool wide, int D, long long ts) {
   return ts < (1ll << 40) && ((wide ? 31 : 15) * ts + D) * sq_size(type) < (1ll << 31);
 }
@@ -802,8 +819,8 @@ extern "C" int serl_gated_scan_bwd(int type, int B, int T, int D, const void* ga
                     scan_wide(type, D, dgate_ts) && scan_wide(type, D, dx_ts);
   const ScanPlan p = scan_plan(type, B, T, D, wide);
   SERL_CHECK_ARG(scan_fits(p, type, B, T), "gated_scan_bwd: B * D too large");
-  SERL_CHECK_ARG(scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
-                 scan_reach(type, false, D, dgate_ts) && scan_reach(type, false, D, dx_ts),
+  SERL_CHECK_ARG(T <= SCAN_SHORT || (scan_reach(type, false, D, gate_ts) && scan_reach(type, false, D, x_ts) && scan_reach(type, false, D, dy_ts) &&
+                                     scan_reach(type, false, D, dgate_ts) && scan_reach(type, false, D, dx_ts)),
                  "gated_scan_bwd: 15 steps of a tensor must span less than 2^31 bytes");
   SERL_CHECK_ARG(scan_apart(B, T, D, dgate_bs, dgate_ts) && scan_apart(B, T, D, dx_bs, dx_ts) && dgate != dx &&
                      ((B > 1 && dgate_bs != dx_bs) || (T > 1 && dgate_ts != dx_ts) ||

@@ -318,3 +318,40 @@ def test_loss_of_a_column_that_holds_the_lowest_value(dev, dtype, tau, R, V, K):
     # gradient, its own and the products)
     size = 0.25 * tau * tau * (q * (torch.log(q.clamp_min(1e-300)).abs() + lp.abs())).sum(1)
     within(loss, rl, (3 * 12 / tau + K + 230) * U * size, "loss")
+
+
+# ------------------------------------------------------------------------------------------------- short windows
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("T", [2, 3, 5, 8])
+def test_short_windows_whose_steps_lie_far_apart(dev, dtype, T):
+    """Up to 8 steps a tensor's rows may be any distance apart, backward as forward: time-major batches, 2^29 bytes and more a step.
+    The gaps stay as they were."""
+    s = seq()
+    B, D = 3, 24
+    e = 4 if dtype == torch.float32 else 2
+    far = (1 << 30) // e if T <= 5 else (1 << 29) // e          # (T - 1) steps: 2^30 .. 2^32 bytes
+    i = scan_inputs(dev, dtype, B, T, D, T, starts=True, lengths=True)
+    store = torch.zeros((T - 1) * far + 5 * B * D, dtype=dtype, device=dev)
+    view = lambda k: torch.as_strided(store, (B, T, D), (D, far, 1), k * B * D)  # noqa: E731
+    gate, x, dy, dgate, dx = (view(k) for k in range(5))
+    gate.copy_(i["gate"])
+    x.copy_(i["x"])
+    dy.copy_(i["dy"])
+    opt = dict(starts=i["starts"], lengths=i["lengths"])
+    want = s.gated_scan(i["gate"], i["x"], i["h0"], save=True, **opt)
+    got = s.gated_scan(gate, x, i["h0"], save=True, **opt)
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+    wg = s.gated_scan_backward(i["gate"], i["x"], want[2], i["dy"], i["dh_last"], **opt)
+    gg = s.gated_scan_backward(gate, x, want[2], dy, i["dh_last"], out=(dgate, dx), **opt)
+    assert gg[0] is dgate and gg[1] is dx
+    # threads join in another order than with near rows: 8 steps of at most 10 roundings each, |G| <= 9 * 5, |h| + |x| <= 10
+    tol = 8 * 10 * U * 45
+    for k, (u, v) in enumerate(zip(gg, wg)):
+        within(u, v, 2 * ((tol * 10 / 4 if k == 0 else tol) + HALF[dtype] * v.double().abs().cpu() + SMALL), "far steps")
+    again = s.gated_scan_backward(gate, x, want[2], dy, i["dh_last"], **opt)
+    assert all(torch.equal(u, v) for u, v in zip(again, gg))
+    assert torch.equal(gate, i["gate"]) and torch.equal(x, i["x"]) and torch.equal(dy, i["dy"])
+    inner = store.clone()
+    for k in range(5):
+        torch.as_strided(inner, (B, T, D), (D, far, 1), k * B * D).zero_()
+    assert not inner.any()
