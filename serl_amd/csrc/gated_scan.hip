@@ -46,10 +46,10 @@ __device__ __forceinline__ void scan_gate(float z, float& f, float& rest) {
 }
 
 // The k of a map of several steps is 0 where an episode starts in them and only there: k c + b then cuts whatever c is (0 * NaN = 0 in the
-// legacy product), so an infinity or NaN of one episode ends with it.  Products of gates alone stay at SCAN_LEAST or above it, however
-// many (0.9^1000 is below fp32's smallest number), so that elsewhere an infinity or NaN reaches every later step.  Of a finite state c
-// no more than 1.2e-38 c is left too much by it.
-#define SCAN_LEAST 1.17549435e-38f
+// legacy product), so an infinity or NaN of one episode ends with it.  Products of gates alone stay at SCAN_LEAST, fp32's smallest
+// number, or above it, however many (0.9^1000 is below it), so that elsewhere an infinity or NaN reaches every later step; of a finite
+// state c it leaves 1.4e-45 c, less than 5e-7 of the largest.
+#define SCAN_LEAST 0x1p-149f
 __device__ __forceinline__ float scan_apply(float k, float c, float b) {
   float r;
   asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(k), "v"(c));

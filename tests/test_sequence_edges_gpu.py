@@ -355,3 +355,21 @@ def test_short_windows_whose_steps_lie_far_apart(dev, dtype, T):
     for k in range(5):
         torch.as_strided(inner, (B, T, D), (D, far, 1), k * B * D).zero_()
     assert not inner.any()
+
+
+@pytest.mark.parametrize("T", [6, 100, 3000])
+def test_gates_of_zero_forget_the_largest_states(dev, T):
+    """What is left of a state of fp32's largest size behind gates that are 0, or whose product is, is below 1e-6."""
+    s = seq()
+    for dtype in DTYPES:
+        for low, at in ((-math.inf, 0), (-200.0, 0), (-80.0, 2), (-20.0, 5)):      # f^at h0 is below 1e-6, and behind it the x of the last steps
+            gate = torch.full((2, T, 40), low, dtype=dtype, device=dev)
+            x, h0 = torch.full_like(gate, 0.5), torch.full((2, 40), 3e38, device=dev)
+            y, h, saved = s.gated_scan(gate, x, h0, save=True)
+            within(y[:, at:], torch.full((2, T - at, 40), 0.5), 2.0 ** -20 + HALF[dtype], "y")
+            within(h, torch.full((2, 40), 0.5), 2.0 ** -20, "h_last")
+            _, _, d0 = s.gated_scan_backward(gate, x, saved, x, torch.full_like(h0, 3e38))
+            # dh0 = sum of f^(t+1) dy_t + f^T dh_last
+            f = 1 / (1 + math.exp(min(700.0, -low)))
+            want = 0.5 * f / (1 - f) + (3e38 * f ** T if f ** T > 1e-60 else 0)
+            within(d0, torch.full((2, 40), want), 2.0 ** -20 + abs(want) * T * 60 * U, "dh0")
