@@ -11,7 +11,8 @@
 // for the statistics, one that joins them and writes the gradient (it reads the row again, from the caches where they hold it).
 //
 // 2048 x 131072 bf16, 128 slots: 217 us (5.0 TB/s where a large copy reaches 5.2; the first load and the last store of a
-// workgroup's eight rows overlap nothing, and the vector ALU is half busy with two exponentials per column).
+// workgroup's eight rows overlap nothing, and the vector ALU is half busy with two exponentials per column); the value alone 108 us,
+// 2048 x 65536 fp32 226.
 //
 // Rows start at any alignment: the columns before the first 16-byte boundary and behind the last whole piece are taken by
 // single threads (`head` and `tail`); the gradient is stored in the logits' pieces, which may lie at any element of its rows

@@ -11,8 +11,8 @@
 // reaches it.  Every input is read once and every output written once; the next tile's loads are issued before the current tile
 // is joined.  16 elements per thread: with 32 the kernels were 10 to 20 % slower (registers, too few waves).
 //
-// Bound by memory and, to half, by the vector ALU (22 instructions per element forward, 35 backward).  8 x 4096 x 2048 bf16:
-// forward 92 us (4.4 TB/s where a large copy reaches 5.2), backward 160 us (4.2 TB/s).
+// Bound by memory and, to half, by the vector ALU (26 instructions per element forward, 46 backward).  8 x 4096 x 2048 bf16:
+// forward 95 us (4.2 TB/s where a large copy reaches 5.2), backward 164 us (4.1 TB/s).
 #include "seqtypes.h"
 
 #define SCAN_CKPT 64        // steps between the states that the forward pass keeps for the backward pass
@@ -582,13 +582,15 @@ struct ScanPlan { int vec, cg, ndb, nseg, seg_len; };
 // wide: 4 elements per access.  The time axis is split (two launches, gate and x read twice) only where sequences and
 // channels alone leave half of the CUs idle and there are more than 5 tiles.  bf16 forward: 8 x 4000 x 1024 (128 workgroups) 85 ->
 // 68 us; but 12 x 4000 x 1024 (192) 89 -> 132 us, 4 x 512 x 1024 (4 tiles) 11.9 -> 16 us; both ways: 9 x 2000 x 1024 (144) 117 ->
-// 128 us, 12 x 777 x 333 fp32 (132) 52 -> 42 us.
+// 128 us, 12 x 777 x 333 fp32 (132) 52 -> 44 us.
 // 16-bit rows of up to 32 channels, or 65 to 96, are contiguous enough for groups of 32 channels, with fewer idle lanes: both ways
 // 140 x 3000 x 32 bf16 157 -> 88 us, 45 x 14336 x 24 195 -> 123, 140 x 3000 x 80 292 -> 200; with half cache lines of wider rows
 // 8 x 4096 x 2048 252 -> 357 us.
 // How many pieces: a CU holds two workgroups of the forward kernels, one of the backward, so what counts is the rounds of 512 and
 // 256 workgroups, times the tiles of a piece and three quarters of one for its start and end.  Against 512 workgroups or more
 // whatever the rounds, both ways bf16: 1 x 24576 x 2424 468 -> 357 us, 6 x 4000 x 1024 179 -> 150, 6 x 10127 x 83 76 -> 61.
+// fp32 has workgroups of 256 threads too, but its 128 bytes are 32 channels: counted as two to a CU it gained in one case (5 x 3000 x
+// 1024 both ways 177 -> 158 us) and lost in most (8 x 3000 x 1024 186 -> 235, 12 x 700 x 500 49 -> 56, 2 x 4000 x 333 44 -> 55).
 static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   ScanPlan p;
   p.vec = wide ? 4 : 1;
@@ -597,7 +599,7 @@ static ScanPlan scan_plan(int type, int B, int T, int D, bool wide) {
   p.nseg = 1;
   p.seg_len = T;
   const long long blocks = (long long)B * p.ndb;
-  const int fit = wide && type != SERL_F32 && p.cg == 8 ? 2 : 1;      // half the threads: twice as many workgroups on a CU
+  const int fit = wide && type != SERL_F32 && p.cg == 8 ? 2 : 1;      // half the threads and registers: twice as many workgroups on a CU
   if (blocks <= 136 * fit && T > 5 * SCAN_TILE) {
     const int tiles = cdiv(T, SCAN_TILE);
     long long best = 0;

@@ -7,8 +7,8 @@
 // 16 or 32 vectors of 16 bytes (16: 262144 x 128 bf16 83 -> 42 us, 500000 x 33 both ways 360 -> 128 us against a wave per row), a
 // wave one of up to 128 (no LDS, no barrier), a workgroup of 256 or 1024 threads a longer one.  The norm is of the sum as it is
 // STORED (rounded to the residual's type): later layers and the backward pass see the values that were normed.
-// 16384 x 4096 bf16: forward 78 us (6.9 TB/s: part of it from the caches), both ways 177 us (5.3 TB/s), 5 us of it for the shares of
-// the weight's gradient; 64 rows to e4m3 4 us.
+// 16384 x 4096 bf16: forward call after call 79 us (6.8 TB/s: part of it from the caches), both ways 93 + 82 + 5 us (5.2 TB/s), the 5 for
+// the shares of the weight's gradient; to e4m3 74 us, 64 rows 4 us.
 #include "seqtypes.h"
 
 #define RMS_MAXN 32768

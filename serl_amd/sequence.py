@@ -273,6 +273,7 @@ def rms_norm(x, weight, residual=None, eps=1e-6, save=False):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension (1 .. 32768), s = x + residual.
 
     residual: x's shape, in x's type or float32 (a residual stream kept in 32 bits); weight (N,) in x's type or float32.
+    The squares are summed in float32: a row with values beyond some 1e19 gives y = 0.
     Returns (y, s): y in x's type, s in the residual's (rounded to it before it is normed), or x itself without a residual;
     with save=True also rstd (...,) float32 for rms_norm_backward."""
     y, _, total, rstd = _norm(x, weight, residual, eps, False, save)

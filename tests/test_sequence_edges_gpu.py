@@ -58,6 +58,12 @@ def test_rms_norm_in_place(dev, dtype, stream):
         ops.rms_norm_fwd(code[dtype], code[stream], code[dtype], R, N, x.data_ptr(), N, res.data_ptr(), N, w.data_ptr(), 1e-6, x.data_ptr(),
                          N, False, None, res.data_ptr(), N, None, st)
         assert torch.equal(x, y) and torch.equal(res, total), (R, N)
+        q, scale, _ = s.rms_norm_fp8(i["x"], w, i["residual"])
+        x, res, scale2 = i["x"].clone(), i["residual"].clone(), torch.empty(R, device=dev)
+        e = x.element_size()                # the codes at the head of the row that they are made from
+        ops.rms_norm_fwd(code[dtype], code[stream], code[dtype], R, N, x.data_ptr(), N, res.data_ptr(), N, w.data_ptr(), 1e-6, x.data_ptr(),
+                         N * e, True, scale2.data_ptr(), res.data_ptr(), N, None, st)
+        assert torch.equal(x.view(torch.uint8)[:, :N], q.view(torch.uint8)) and torch.equal(scale2, scale) and torch.equal(res, total), (R, N)
         n = ops.rms_norm_bwd_workspace_bytes(R, N)
         ws = torch.empty(max(1, n // 4), device=dev)
         dw2 = torch.empty(N, device=dev)
